@@ -19,6 +19,8 @@ LIB_PATH = Path(os.environ.get("GSWARP_AMD_LIB", Path(__file__).resolve().parent
 GS_OK = 0
 GS_RECORD_FLOATS = 12
 GS_GRAD_FLOATS = 10
+GS_FP32, GS_BF16, GS_FP16 = 0, 1, 2
+GS_REDUCE_NONE, GS_REDUCE_SUM, GS_REDUCE_MEAN = 0, 1, 2
 
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
@@ -96,6 +98,21 @@ SIGNATURES = {
         ctypes.c_int,
         [_i32, _i32, _i32, _vp, _vp, _vp, _vp, _f32, _vp, _vp, _vp, _vp, _f32, _f32, _f32, _f32, _vp, _vp, _vp, _vp,
          _i32, _i32, _vp, _vp, _vp, _i32, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    ),
+    "gs_embed_fwd": (ctypes.c_int, [_i64, _i32, _i32, _i32, _vp, _i32, _vp, _i64, _f32, _vp, _vp]),
+    "gs_embed_bwd_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
+    "gs_embed_bwd": (
+        ctypes.c_int, [_i64, _i32, _i32, _i32, _vp, _i32, _vp, _f32, _i64, _vp, _vp, _sz, _vp]),
+    "gs_xent_fwd_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i64, _i64]),
+    "gs_xent_fwd": (
+        ctypes.c_int,
+        [_i64, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _f32, _i32, _vp, _vp, _vp, _vp, _sz, _vp],
+    ),
+    "gs_xent_bwd_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i64, _i64, _i32, _i32]),
+    "gs_xent_bwd": (
+        ctypes.c_int,
+        [_i64, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _f32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
+         _vp],
     ),
 }
 

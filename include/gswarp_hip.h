@@ -562,6 +562,76 @@ int gs_preprocess_bwd(int32_t P, int32_t sh_coeffs, int32_t degree, const float*
                       float* grad_scales, float* grad_rotations, float* grad_cov3d, float* grad_sh,
                       float* grad_opacity, float* grad_colors, void* stream);
 
+/*
+ * Vocabulary operators: a learned table of `vocab` rows of `dim` values, read
+ * by token and scored against.  dtype is that of the table, the features and
+ * their gradients; sums are held in fp32 or more whatever it is.  Tokens and
+ * targets are int32 or int64 (`*_bits` 32 or 64).  These have no counterpart
+ * in the reference.
+ */
+#define GS_FP32 0
+#define GS_BF16 1
+#define GS_FP16 2
+
+#define GS_REDUCE_NONE 0
+#define GS_REDUCE_SUM 1
+#define GS_REDUCE_MEAN 2
+
+/*
+ * out[i, :] = scale * table[tokens[i], :] (n x dim, contiguous, rounded once).
+ * ld_table: elements between the table's rows.  A token outside [0, vocab)
+ * reads nothing and gives a row of NaN.
+ */
+int gs_embed_fwd(int64_t n, int32_t vocab, int32_t dim, int32_t dtype, const void* tokens, int32_t token_bits,
+                 const void* table, int64_t ld_table, float scale, void* out, void* stream);
+
+/*
+ * grad_table[v, :] = scale * sum over the positions i with tokens[i] = v of
+ * grad_out[i, :]; every row is written (zero where no token names it), sums in
+ * fp32 in an order that only the tokens fix.  padding_index (-1: none) and
+ * tokens outside [0, vocab) bring no gradient.  workspace:
+ * gs_embed_bwd_workspace_bytes(n, vocab, dim, dtype) bytes on 256, of any content.
+ */
+size_t gs_embed_bwd_workspace_bytes(int64_t n, int32_t vocab, int32_t dim, int32_t dtype);
+int gs_embed_bwd(int64_t n, int32_t vocab, int32_t dim, int32_t dtype, const void* tokens, int32_t token_bits,
+                 const void* grad_out, float scale, int64_t padding_index, void* grad_table, void* workspace,
+                 size_t workspace_bytes, void* stream);
+
+/*
+ * Softmax cross entropy of `rows` features (rows x dim, ld_features elements
+ * between rows) against every row of the table, without the logits in memory:
+ * s_ij = logit_scale <features_i, table_j>, loss_i = log sum_j exp s_ij -
+ * s_{i, targets_i}.  Rows whose target is ignore_index give 0 and do not
+ * count, whatever they hold; any other target outside [0, vocab) gives NaN.
+ * loss: `rows` fp32 for GS_REDUCE_NONE, else one (the sum, or the mean over
+ * the rows that count; over none, NaN).  lse (rows fp32, may be NULL if no
+ * backward follows) receives the base-2 logarithm of sum_j exp s_ij, count the number of rows
+ * that count; gs_xent_bwd takes both.  features and table must be 16-byte
+ * aligned unless they are fp32 or have a dim or row distance that is not a
+ * multiple of 8 (those are laid out in the workspace first).  workspace:
+ * gs_xent_fwd_workspace_bytes bytes on 256, of any content.
+ */
+size_t gs_xent_fwd_workspace_bytes(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, int64_t ld_features,
+                                   int64_t ld_table);
+int gs_xent_fwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void* features, int64_t ld_features,
+                const void* table, int64_t ld_table, const void* targets, int32_t target_bits, int64_t ignore_index,
+                float logit_scale, int32_t reduction, float* loss, float* lse, int64_t* count, void* workspace,
+                size_t workspace_bytes, void* stream);
+
+/*
+ * The gradients of gs_xent_fwd: grad_features (rows x dim) and grad_table
+ * (vocab x dim), contiguous, either may be NULL (not computed); the logits
+ * are formed again, a piece of rows and vocabulary at a time.  grad_loss:
+ * `rows` fp32 for GS_REDUCE_NONE, else one.  Rows that do not count get zero
+ * and bring nothing, whatever their features hold.  The other arguments are the forward's.
+ */
+size_t gs_xent_bwd_workspace_bytes(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, int64_t ld_features,
+                                   int64_t ld_table, int32_t want_features, int32_t want_table);
+int gs_xent_bwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void* features, int64_t ld_features,
+                const void* table, int64_t ld_table, const void* targets, int32_t target_bits, int64_t ignore_index,
+                float logit_scale, int32_t reduction, const float* lse, const int64_t* count, const float* grad_loss,
+                void* grad_features, void* grad_table, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
