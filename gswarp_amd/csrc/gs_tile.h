@@ -75,73 +75,86 @@ struct Pack<_Float16> {
   typedef f16x4 v4;
 };
 
-// One operand's part of a K step: BT rows (m or n) x 64 columns of K.
+// One operand's part of a K step, BT rows (m or n) x 64 columns of K, loaded
+// straight into LDS: each load instruction of a wave fills 1024 bytes, lane l
+// the 16 bytes at 16 l, so the arrangement in LDS is made by the choice of what
+// each lane reads.
 //
-// LDS layouts (bytes), 16-byte chunks permuted so that no read or write of a
-// wave meets a bank twice:
+// LDS layouts (bytes), 16-byte chunks permuted so that no read of a wave meets a
+// bank twice:
 //   K contiguous: row i at i * 128, its chunk c at (c ^ ((i >> 1) & 7)) * 16:
 //     the 16 rows that one phase of a 16-byte read takes lie in 16 different
 //     chunks of the 256 bytes of the banks;
-//   K rows: K row k at k * 2 BT, its 32-byte chunk c at (c ^ 2 (k & 3)) * 32:
-//     the four K rows that the transposing load takes per 16 lanes lie apart.
-template <bool kAlongK, int BT, int kThreads>
+//   K rows: K row k at k * 2 BT, its 32-byte chunk c at (c ^ turn(k)) * 32: the
+//     four K rows that the transposing load takes per 16 lanes lie apart.
+template <bool kAlongK, int BT, int kWaves>
 struct Stage {
-  static constexpr int kVectors = BT * 8 / kThreads;  // 16-byte loads of a thread
   static constexpr int kBytes = BT * 128;
-  static constexpr int kRowVectors = kAlongK ? 8 : BT / 8;
-  u32x4 r[kVectors];
+  static constexpr int kLoads = kBytes / 1024 / kWaves;         // load instructions of a wave
+  static constexpr int kRowVectors = kAlongK ? 8 : BT / 8;      // 16-byte chunks of a row of the layout
+  static constexpr int kLoadRows = 64 / kRowVectors;            // rows of the layout that an instruction fills
+  static_assert(kLoads * kWaves * 1024 == kBytes, "every wave issues the same loads");
 
-  // The K step at k0 of plane `plane`, rows (or columns) from i0; K and the
-  // operand's extent bound what is read, and everything outside is zero.
-  // row_mask (K rows only): bit k of it drops K row k0 + k when clear.
-  __device__ __forceinline__ void load(const Operand& o, int plane, int i0, int64_t k0, int64_t K, uint64_t row_mask) {
-    const int vec = threadIdx.x % kRowVectors;
-    const int row = threadIdx.x / kRowVectors;
-    constexpr int kRowStep = kThreads / kRowVectors;
-    const uint16_t* base;
-    uint32_t bytes;
-    bool in;
-    const uint32_t ld2 = (uint32_t)o.ld * 2u;
-    if (kAlongK) {
-      base = o.p + (int64_t)plane * o.plane + (int64_t)i0 * o.ld + k0;
-      const int rows = min(BT, o.extent - i0);
-      bytes = (uint32_t)(rows - 1) * ld2 + (uint32_t)min((int64_t)kBK, (K - k0 + 7) & ~7ll) * 2u;
-      in = k0 + vec * 8 < K;
-    } else {
-      base = o.p + (int64_t)plane * o.plane + k0 * o.ld + i0;
-      const int rows = (int)min((int64_t)kBK, K - k0);
-      bytes = (uint32_t)(rows - 1) * ld2 + (uint32_t)min(BT, (o.extent - i0 + 7) & ~7) * 2u;
-      in = i0 + vec * 8 < o.extent;
-    }
-    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bytes, 0x00020000);
+  static __device__ __forceinline__ int turn(int k) { return BT >= 128 ? 2 * (k & 3) : 2 * ((k >> 1) & 1); }
+
+  // Byte offsets of the lane's chunk from the step's first element, for
+  // instructions of even and of odd number (the permutation repeats every two).
+  uint32_t offset[2];
+  int32_t chunk[2];  // the chunk's number in its row (K contiguous)
+
+  __device__ __forceinline__ void init(const Operand& o, int i0) {
+    const int lane = threadIdx.x & 63;
+    const int row = lane / kRowVectors, at = lane % kRowVectors;
 #pragma unroll
-    for (int j = 0; j < kVectors; ++j) {
-      const int rr = row + j * kRowStep;
-      uint32_t off = (uint32_t)rr * ld2 + vec * 16u;
-      bool use = in;
-      if (!kAlongK) use = use && ((row_mask >> rr) & 1);
-      r[j] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, use ? off : kOutOfRange, 0, 0);
+    for (int p = 0; p < 2; ++p) {
+      const int r = p * kLoadRows + row;
+      if (kAlongK) chunk[p] = at ^ ((r >> 1) & 7);
+      else chunk[p] = (((at >> 1) ^ turn(r)) << 1) | (at & 1);
+      offset[p] = (uint32_t)row * (uint32_t)o.ld * 2u + chunk[p] * 16u;
+      if (!kAlongK && i0 + chunk[p] * 8 >= o.extent) offset[p] = kOutOfRange;
     }
   }
 
-  __device__ __forceinline__ void store(char* lds) const {
-    const int vec = threadIdx.x % kRowVectors;
-    const int row = threadIdx.x / kRowVectors;
-    constexpr int kRowStep = kThreads / kRowVectors;
+  // Starts the loads of the K step at k0 of plane `plane` into lds; K and the
+  // operand's extent bound what is read, and everything outside is zero.
+  // row_mask (K rows only): K row k0 + k counts as zero where bit k is clear.
+  __device__ __forceinline__ void load(const Operand& o, int plane, int i0, int32_t k0, int32_t K, uint64_t row_mask,
+                                       char* __restrict__ lds) const {
+    typedef __attribute__((address_space(3))) void lds_void;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t ld2 = (uint32_t)o.ld * 2u;
+    const uint16_t* base;
+    uint32_t bytes, off[2] = {offset[0], offset[1]};
+    if (kAlongK) {
+      base = o.p + (int64_t)plane * o.plane + (int64_t)i0 * o.ld + k0;
+      const int left = K - k0;
+      bytes = (uint32_t)(min(BT, o.extent - i0) - 1) * ld2 + (uint32_t)min(kBK, (left + 7) & ~7) * 2u;
+      if (left < kBK) {
 #pragma unroll
-    for (int j = 0; j < kVectors; ++j) {
-      const int rr = row + j * kRowStep;
-      int at;
-      if (kAlongK) at = rr * 128 + ((vec ^ ((rr >> 1) & 7)) << 4);
-      else at = rr * (BT * 2) + ((((vec >> 1) ^ (2 * (rr & 3))) << 5) | ((vec & 1) << 4));
-      *reinterpret_cast<u32x4*>(lds + at) = r[j];
+        for (int p = 0; p < 2; ++p)
+          if (chunk[p] * 8 >= left) off[p] = kOutOfRange;
+      }
+    } else {
+      base = o.p + (int64_t)plane * o.plane + (int64_t)k0 * o.ld + i0;
+      bytes = (uint32_t)(min(kBK, K - k0) - 1) * ld2 + (uint32_t)min(BT, (o.extent - i0 + 7) & ~7) * 2u;
+    }
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bytes, 0x00020000);
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int number = wave * kLoads + j;
+      uint32_t at = off[number & 1] + (uint32_t)(number * kLoadRows) * ld2;
+      if (!kAlongK && row_mask != ~0ull) {
+        const int k = number * kLoadRows + (threadIdx.x & 63) / kRowVectors;
+        if (!((row_mask >> k) & 1)) at = kOutOfRange;
+      }
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(lds + number * 1024), 16, at, 0, 0, 0);
     }
   }
 
   // Matrix-core operand of 32 rows from i (a multiple of 32) and K columns
   // 16 ks .. 16 ks + 15 of the step: lane l holds row l % 32, columns 8 (l / 32) ..+7.
   template <typename T>
-  static __device__ __forceinline__ typename Pack<T>::v8 fragment(const char* lds, int i, int ks) {
+  static __device__ __forceinline__ typename Pack<T>::v8 fragment(const char* __restrict__ lds, int i, int ks) {
     const int lane = threadIdx.x & 63;
     if (kAlongK) {
       const int row = i + (lane & 31);
@@ -153,7 +166,7 @@ struct Stage {
       const int j = lane & 15, group = lane >> 4;
       const int k = 16 * ks + 8 * (group >> 1) + (j >> 2);
       const int m = i + 16 * (group & 1);
-      const char* at = lds + k * (BT * 2) + (((m >> 4) ^ (2 * (k & 3))) << 5) + (j & 3) * 8;
+      const char* at = lds + k * (BT * 2) + (((m >> 4) ^ turn(k)) << 5) + (j & 3) * 8;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 4 * BT * 2));
       const s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -167,7 +180,7 @@ template <int kBM, int kBN, int kWavesM_, int kWavesN_>
 struct Shape {
   static constexpr int BM = kBM, BN = kBN;
   static constexpr int kWavesM = kWavesM_, kWavesN = kWavesN_;
-  static constexpr int kThreads = 64 * kWavesM * kWavesN;
+  static constexpr int kWaves = kWavesM * kWavesN, kThreads = 64 * kWaves;
   static constexpr int kWaveM = BM / kWavesM, kWaveN = BN / kWavesN;
   static constexpr int kMB = kWaveM / 32, kNB = kWaveN / 32;
   static constexpr int kLdsBytes = 2 * (BM + BN) * 128;
@@ -189,72 +202,106 @@ __device__ __forceinline__ int wave_n() {
   return (threadIdx.x >> 6) % S::kWavesN * S::kWaveN;
 }
 
+// acc += the step held at lds.  The fragments of 16 columns of K are read while
+// the matrix cores work on the 16 before.
+template <class S, typename T, class StageX, class StageY>
+__device__ __forceinline__ void multiply(Accumulators<S>& acc, int wm, int wn, const char* __restrict__ lds) {
+  typename Pack<T>::v8 fx[2][S::kMB], fy[2][S::kNB];
+  auto read = [&](int ks) {
+#pragma unroll
+    for (int a = 0; a < S::kMB; ++a) fx[ks & 1][a] = StageX::template fragment<T>(lds, wm + 32 * a, ks);
+#pragma unroll
+    for (int b = 0; b < S::kNB; ++b)
+      fy[ks & 1][b] = StageY::template fragment<T>(lds + StageX::kBytes, wn + 32 * b, ks);
+  };
+  read(0);
+#pragma unroll
+  for (int ks = 0; ks < kBK / 16; ++ks) {
+    if (ks + 1 < kBK / 16) read(ks + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int a = 0; a < S::kMB; ++a)
+#pragma unroll
+      for (int b = 0; b < S::kNB; ++b) acc.c[a][b] = mfma(fx[ks & 1][a], fy[ks & 1][b], acc.c[a][b]);
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // acc = the tile at (m0, n0), over K columns [k_begin, k_end) of products
 // `products` (1, or 6 for fp32 planes).  Every element outside the operands
 // counts as zero.  x_rows (X in K rows only, may be null): one bit per K row
 // (k_begin on a multiple of 64); rows whose bit is clear count as zero whatever
 // they hold.  lds: S::kLdsBytes, free for the caller after a barrier.
 //
-// Two LDS buffers: the loads of step t + 1 are in flight (in registers) while
-// the matrix cores work on step t; one barrier per step.
+// Two LDS buffers: the loads of step t + 1 go straight into one while the matrix
+// cores work on the other; one barrier per step.
 template <class S, typename T, bool kXAlongK, bool kYAlongK>
 __device__ __forceinline__ void product(Accumulators<S>& acc, const Operand& x, const Operand& y, int m0, int n0,
-                                        int64_t k_begin, int64_t k_end, int products, const uint64_t* x_rows,
+                                        int32_t k_begin, int32_t k_end, int products, const uint64_t* x_rows,
                                         char* lds) {
-  typedef Stage<kXAlongK, S::BM, S::kThreads> StageX;
-  typedef Stage<kYAlongK, S::BN, S::kThreads> StageY;
+  typedef Stage<kXAlongK, S::BM, S::kWaves> StageX;
+  typedef Stage<kYAlongK, S::BN, S::kWaves> StageY;
 #pragma unroll
   for (int a = 0; a < S::kMB; ++a)
 #pragma unroll
     for (int b = 0; b < S::kNB; ++b) acc.c[a][b] = f32x16{};
-  const int steps = (int)((k_end - k_begin + kBK - 1) / kBK);
+  const int steps = (k_end - k_begin + kBK - 1) / kBK;
   const int total = steps * products;
   if (total <= 0) return;
   StageX sx;
   StageY sy;
+  sx.init(x, m0);
+  sy.init(y, n0);
   int step = 0, prod = 0;
-  auto load = [&]() {
-    const int64_t k0 = k_begin + (int64_t)step * kBK;
+  constexpr int kBuffer = StageX::kBytes + StageY::kBytes;
+  // the masks of 64 steps, a lane each
+  uint64_t masks = 0;
+  const bool masked = !kXAlongK && x_rows;
+  auto load = [&](char* to) {
+    const int32_t k0 = k_begin + step * kBK;
     const int px = products == 1 ? 0 : product_plane(kPlanesX, prod);
     const int py = products == 1 ? 0 : product_plane(kPlanesY, prod);
-    const uint64_t mask = (!kXAlongK && x_rows) ? x_rows[k0 / kBK] : ~0ull;
-    sx.load(x, px, m0, k0, k_end, mask);
-    sy.load(y, py, n0, k0, k_end, ~0ull);
+    uint64_t mask = ~0ull;
+    if (masked) {
+      if ((step & 63) == 0) {
+        const int at = step + (threadIdx.x & 63);
+        masks = at < steps ? x_rows[k_begin / kBK + at] : 0;
+      }
+      mask = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(masks >> 32), step & 63) << 32 |
+             (uint32_t)__builtin_amdgcn_readlane((int)masks, step & 63);
+    }
+    sx.load(x, px, m0, k0, k_end, mask, to);
+    sy.load(y, py, n0, k0, k_end, ~0ull, to + StageX::kBytes);
     if (++step == steps) {
       step = 0;
       ++prod;
     }
   };
-  constexpr int kBuffer = StageX::kBytes + StageY::kBytes;
-  load();
-  sx.store(lds);
-  sy.store(lds + StageX::kBytes);
+  load(lds);
   __syncthreads();
   const int wm = wave_m<S>(), wn = wave_n<S>();
   for (int t = 0; t < total; ++t) {
-    const bool more = t + 1 < total;
-    if (more) load();
-    const char* lx = lds + (t & 1) * kBuffer;
-    const char* ly = lx + StageX::kBytes;
-#pragma unroll
-    for (int ks = 0; ks < kBK / 16; ++ks) {
-      typename Pack<T>::v8 fx[S::kMB], fy[S::kNB];
-#pragma unroll
-      for (int a = 0; a < S::kMB; ++a) fx[a] = StageX::template fragment<T>(lx, wm + 32 * a, ks);
-#pragma unroll
-      for (int b = 0; b < S::kNB; ++b) fy[b] = StageY::template fragment<T>(ly, wn + 32 * b, ks);
-#pragma unroll
-      for (int a = 0; a < S::kMB; ++a)
-#pragma unroll
-        for (int b = 0; b < S::kNB; ++b) acc.c[a][b] = mfma(fx[a], fy[b], acc.c[a][b]);
-    }
-    if (more) {
-      char* next = lds + ((t + 1) & 1) * kBuffer;
-      sx.store(next);
-      sy.store(next + StageX::kBytes);
-    }
+    if (t + 1 < total) load(lds + ((t + 1) & 1) * kBuffer);
+    multiply<S, T, StageX, StageY>(acc, wm, wn, lds + (t & 1) * kBuffer);
     __syncthreads();
   }
+}
+
+// The tile of a block: blocks go to the 8 XCDs (each with an L2 of its own) in
+// turn, so each XCD is given a run of consecutive tiles, in bands of 8 tiles
+// of m, m first inside a band: tiles that run side by side share operands.
+struct TileAt {
+  int m, n;
+};
+__device__ __forceinline__ TileAt tile_at(int tiles_m, int tiles_n) {
+  const int total = tiles_m * tiles_n;
+  const int id = blockIdx.x, q = total / 8, r = total % 8, xcd = id % 8;
+  const int t = xcd * q + min(xcd, r) + id / 8;
+  const int band = t / (8 * tiles_n);
+  const int height = min(8, tiles_m - 8 * band), in = t - band * 8 * tiles_n;
+  return {8 * band + in % height, in / height};
 }
 
 }  // namespace gs_tile

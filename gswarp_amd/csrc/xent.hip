@@ -1,8 +1,8 @@
 // Softmax cross entropy of features against every row of a vocabulary table,
 // without keeping the logits, and its gradients.
 //
-//   s_ij = c <h_i, w_j>,  lse_i = log sum_j exp s_ij,  loss_i = lse_i - s_{i, t_i}
-//   ds_ij = g_i (exp(s_ij - lse_i) - [j = t_i])
+//   s_ij = c <h_i, w_j>,  loss_i = log sum_j exp s_ij - s_{i, t_i}
+//   ds_ij = g_i (exp(s_ij) / sum_k exp s_ik - [j = t_i])
 //   dh_i = c sum_j ds_ij w_j,  dw_j = c sum_i ds_ij h_i
 //
 // Forward: one product kernel over tiles of (vocabulary x rows) reduces each
@@ -14,6 +14,8 @@
 // beyond one piece.
 #include "gs_capi.h"
 #include "gs_tile.h"
+
+#include <type_traits>
 
 namespace gs_xent {
 
@@ -95,57 +97,70 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, in
 
 // ------------------------------------------------------------------ forward
 // The logits of a tile (vocabulary m x rows n), reduced to one pair per row:
-// stats[tile * rows + row] = (max of s log2 e, sum of 2^(s log2 e - max)).
-// The tile that holds a row's target also writes that logit.
+// stats[tile * rows + row] = (max, sum of 2^(s log2 e - max)), max the largest
+// s log2 e rounded to fp32 (the exponents are formed from the unrounded product).
+// The tile that holds a row's target also writes its dot product.
 template <class S, typename T>
 __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, Operand features, int dim,
                                                                  int products, float scale2, Targets targets,
-                                                                 int tiles_m, float2* __restrict__ stats,
+                                                                 int tiles_m, int tiles_n,
+                                                                 float2* __restrict__ stats,
                                                                  float* __restrict__ label_logit) {
   __shared__ __attribute__((aligned(16))) char lds[S::kLdsBytes];
-  const int tile_m = blockIdx.x % tiles_m, tile_n = blockIdx.x / tiles_m;
-  const int m0 = tile_m * S::BM, n0 = tile_n * S::BN;
+  const gs_tile::TileAt tile = gs_tile::tile_at(tiles_m, tiles_n);
+  const int m0 = tile.m * S::BM, n0 = tile.n * S::BN;
   Accumulators<S> acc;
   gs_tile::product<S, T, true, true>(acc, table, features, m0, n0, 0, dim, products, nullptr, lds);
 
   const int lane = threadIdx.x & 63;
   const int wm = gs_tile::wave_m<S>(), wn = gs_tile::wave_n<S>();
   float2* red = reinterpret_cast<float2*>(lds);  // [kWavesM][BN]
-  const bool whole = m0 + S::BM <= table.extent;
-#pragma unroll
-  for (int b = 0; b < S::kNB; ++b) {
+  // kWhole: no m of the tile lies past the vocabulary
+  auto reduce = [&](auto kWhole, int b) {
     const int n = n0 + wn + 32 * b + (lane & 31);
-    const bool row_in = n < features.extent;
-    const int64_t target = row_in ? targets.at(n) : -1;
-    const int64_t first = m0 + wm + 4 * (lane >> 5);  // the lane's first m
-    float top = -INFINITY;
-#pragma unroll
-    for (int a = 0; a < S::kMB; ++a)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        float v = acc.c[a][b][e] * scale2;
-        const int64_t m = first + 32 * a + 8 * (e >> 2) + (e & 3);
-        if (!whole && m >= table.extent) v = -INFINITY;
-        acc.c[a][b][e] = v;
-        top = fmaxf(top, v);
-      }
+    const int first = m0 + wm + 4 * (lane >> 5);  // the lane's first m
+    const auto past = [&](int a, int e) {
+      return !kWhole && first + 32 * a + 8 * (e >> 2) + (e & 3) >= table.extent;
+    };
+    const int64_t target = n < features.extent ? targets.at(n) : -1;
     const bool here = target >= m0 + wm && target < m0 + wm + S::kWaveM && target < table.extent;
     if (__any(here)) {
 #pragma unroll
       for (int a = 0; a < S::kMB; ++a)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (target == first + 32 * a + 8 * (e >> 2) + (e & 3) && here) label_logit[n] = acc.c[a][b][e];
+          if (here && target == first + 32 * a + 8 * (e >> 2) + (e & 3)) label_logit[n] = acc.c[a][b][e];
     }
-    top = fmaxf(top, __shfl_xor(top, 32));
+    // the largest logit: under a negative scale the least product
+    float raw = scale2 < 0.0f ? INFINITY : -INFINITY;
+#pragma unroll
+    for (int a = 0; a < S::kMB; ++a)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float v = past(a, e) ? raw : acc.c[a][b][e];
+        raw = scale2 < 0.0f ? fminf(raw, v) : fmaxf(raw, v);
+      }
+    const float other = __shfl_xor(raw, 32);
+    raw = scale2 < 0.0f ? fminf(raw, other) : fmaxf(raw, other);
+    const float top = scale2 == 0.0f ? 0.0f : raw * scale2;
     const float ref = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
 #pragma unroll
     for (int a = 0; a < S::kMB; ++a)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(acc.c[a][b][e] - ref);
+      for (int e = 0; e < 16; ++e) {
+        const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[a][b][e], scale2, -ref));
+        sum += past(a, e) ? 0.0f : v;
+      }
     sum += __shfl_xor(sum, 32);
     if (lane < 32) red[(wm / S::kWaveM) * S::BN + wn + 32 * b + lane] = make_float2(top, sum);
+  };
+  if (m0 + S::BM <= table.extent) {
+#pragma unroll
+    for (int b = 0; b < S::kNB; ++b) reduce(std::true_type{}, b);
+  } else {
+#pragma unroll
+    for (int b = 0; b < S::kNB; ++b) reduce(std::false_type{}, b);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < S::BN; i += S::kThreads) {
@@ -158,7 +173,7 @@ __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, 
       r.y = r.y * __builtin_amdgcn_exp2f(r.x - ref) + o.y * __builtin_amdgcn_exp2f(o.x - ref);
       r.x = top;
     }
-    stats[(int64_t)tile_m * features.extent + n0 + i] = r;
+    stats[(int64_t)tile.m * features.extent + n0 + i] = r;
   }
 }
 
@@ -193,44 +208,48 @@ __device__ __forceinline__ void write_total(Sum s, int reduction, float* loss, i
 }
 
 // Joins the tiles' pairs of each row (kLanes lanes a row, in a fixed order):
-// lse (base 2) and the loss; ignored rows give 0, targets outside the
+// norm = (maximum, 1 / sum), from which the backward forms the probabilities
+// 2^(s log2 e - maximum) / sum to fp32's relative precision, and the loss; ignored rows give 0, targets outside the
 // vocabulary NaN.  The block's sum goes to partial[block], or, when there is one block in all, to the result.
 template <int kLanes>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float2* __restrict__ stats,
                                                             const float* __restrict__ label_logit, int rows,
-                                                            int tiles, int vocab, Targets targets, int reduction,
-                                                            float* __restrict__ lse2, float* __restrict__ loss_rows,
+                                                            int tiles, int vocab, float scale2, Targets targets,
+                                                            int reduction, float2* __restrict__ norm,
+                                                            float* __restrict__ loss_rows,
                                                             Sum* __restrict__ partial, bool last,
                                                             float* __restrict__ loss, int64_t* __restrict__ count) {
   __shared__ Sum lds[kJoinThreads / 64];
   const int sub = threadIdx.x % kLanes;
   const int64_t row = (int64_t)blockIdx.x * (kJoinThreads / kLanes) + threadIdx.x / kLanes;
-  float top = -INFINITY, sum = 0.0f;
+  // the sum in 64 bits: tiles far below a row's maximum count, however many they are
+  float top = -INFINITY;
+  double sum = 0.0;
+  auto add = [&](float otop, double osum) {
+    const float m = fmaxf(top, otop), ref = m == -INFINITY ? 0.0f : m;
+    sum = sum * (double)__builtin_amdgcn_exp2f(top - ref) + osum * (double)__builtin_amdgcn_exp2f(otop - ref);
+    top = m;
+  };
   if (row < rows) {
     for (int t = sub; t < tiles; t += kLanes) {
       const float2 o = stats[(int64_t)t * rows + row];
-      const float m = fmaxf(top, o.x), ref = m == -INFINITY ? 0.0f : m;
-      sum = sum * __builtin_amdgcn_exp2f(top - ref) + o.y * __builtin_amdgcn_exp2f(o.x - ref);
-      top = m;
+      add(o.x, (double)o.y);
     }
   }
 #pragma unroll
-  for (int off = kLanes / 2; off; off >>= 1) {
-    const float otop = __shfl_xor(top, off), osum = __shfl_xor(sum, off);
-    const float m = fmaxf(top, otop), ref = m == -INFINITY ? 0.0f : m;
-    sum = sum * __builtin_amdgcn_exp2f(top - ref) + osum * __builtin_amdgcn_exp2f(otop - ref);
-    top = m;
-  }
+  for (int off = kLanes / 2; off; off >>= 1) add(__shfl_xor(top, off), __shfl_xor(sum, off));
   Sum mine = {0.0, 0};
   if (row < rows && sub == 0) {
-    const float l = top + __builtin_amdgcn_logf(sum);
     const int64_t t = targets.at(row);
     float value = 0.0f;
     if (t != targets.ignore) {
-      value = t >= 0 && t < vocab ? (float)((double)(l - label_logit[row]) * kLn2) : __builtin_nanf("");
+      // in 64 bits, the maximum kept apart: small losses do not drown in the logits' size
+      value = t >= 0 && t < vocab
+                  ? (float)(log(sum) + kLn2 * ((double)top - (double)label_logit[row] * (double)scale2))
+                  : __builtin_nanf("");
       mine = {(double)value, 1};
     }
-    if (lse2) lse2[row] = l;
+    if (norm) norm[row] = make_float2(top, (float)(1.0 / sum));
     if (loss_rows) loss_rows[row] = value;
   }
   const Sum s = block_sum(mine, lds);
@@ -321,15 +340,15 @@ __device__ __forceinline__ bool row_counts(const uint64_t* counts, int64_t row) 
 template <class S, typename T, int kPlanes>
 __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, Operand features, int dim,
                                                                  int products, float scale2, Targets targets,
-                                                                 int64_t m_base, int tiles_m,
-                                                                 const float* __restrict__ lse2,
+                                                                 int64_t m_base, int tiles_m, int tiles_n,
+                                                                 const float2* __restrict__ norm,
                                                                  const float* __restrict__ factor,
                                                                  const uint64_t* __restrict__ counts,
                                                                  uint16_t* __restrict__ ds, int64_t ld,
                                                                  int64_t plane) {
   __shared__ __attribute__((aligned(16))) char lds[S::kLdsBytes];
-  const int tile_m = blockIdx.x % tiles_m, tile_n = blockIdx.x / tiles_m;
-  const int m0 = tile_m * S::BM, n0 = tile_n * S::BN;
+  const gs_tile::TileAt tile = gs_tile::tile_at(tiles_m, tiles_n);
+  const int m0 = tile.m * S::BM, n0 = tile.n * S::BN;
   Accumulators<S> acc;
   gs_tile::product<S, T, true, true>(acc, table, features, m0, n0, 0, dim, products, nullptr, lds);
   const int lane = threadIdx.x & 63;
@@ -340,7 +359,7 @@ __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, 
     if (n >= features.extent) continue;
     const int first = m0 + wm + 4 * (lane >> 5);
     const int64_t target = targets.at(n) - m_base;
-    const float l = lse2[n], f = factor[n];
+    const float top = norm[n].x, f = factor[n], share = f * norm[n].y;
     const bool use = row_counts(counts, n);
     uint16_t* out = ds + (int64_t)n * ld + first;
 #pragma unroll
@@ -351,8 +370,8 @@ __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int m = first + 32 * a + 8 * q + j;
-          float v = __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[a][b][4 * q + j], scale2, -l));
-          v = (v - (m == target ? 1.0f : 0.0f)) * f;
+          float v = __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[a][b][4 * q + j], scale2, -top));
+          v = __builtin_fmaf(v, share, m == target ? -f : 0.0f);
           v = use && m < table.extent ? v : 0.0f;
 #pragma unroll
           for (int p = 0; p < kPlanes; ++p) {
@@ -374,17 +393,18 @@ __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, 
 // what is there if `add`); else out = alpha * tile in the result's type.
 // rows_count (dh): rows that do not count are zero.
 template <class S, typename T, typename Out, bool kTableGrad>
-__global__ __launch_bounds__(S::kThreads) void grad_kernel(Operand x, Operand ds, int64_t K, int64_t k_part,
+__global__ __launch_bounds__(S::kThreads) void grad_kernel(Operand x, Operand ds, int32_t K, int32_t k_part,
                                                            int products, const uint64_t* __restrict__ counts,
-                                                           int tiles_m, float* __restrict__ part, int64_t part_plane,
+                                                           int tiles_m, int tiles_n, float* __restrict__ part, int64_t part_plane,
                                                            bool add, const float* __restrict__ alpha,
                                                            Out* __restrict__ out) {
   __shared__ __attribute__((aligned(16))) char lds[S::kLdsBytes];
-  const int tile_m = blockIdx.x % tiles_m, tile_n = blockIdx.x / tiles_m;
-  const int m0 = tile_m * S::BM, n0 = tile_n * S::BN;
+  const gs_tile::TileAt tile = gs_tile::tile_at(tiles_m, tiles_n);
+  const int m0 = tile.m * S::BM, n0 = tile.n * S::BN;
   const int D = x.extent;
-  const int64_t k_begin = (int64_t)blockIdx.y * k_part;
-  const int64_t k_end = min(K, k_begin + k_part);
+  // a part past the end (k_part is rounded up) has nothing to add
+  const int32_t k_begin = (int32_t)min((int64_t)K, (int64_t)blockIdx.y * k_part);
+  const int32_t k_end = (int32_t)min((int64_t)K, (int64_t)k_begin + k_part);
   Accumulators<S> acc;
   gs_tile::product<S, T, false, !kTableGrad>(acc, x, ds, m0, n0, k_begin, k_end, products,
                                              kTableGrad ? counts : nullptr, lds);
@@ -528,10 +548,10 @@ static void launch_logits_fwd(const Problem& p, const ForwardPlan& f, const Oper
                               float scale2, Targets targets, hipStream_t s) {
   const int64_t tiles = f.tiles_m * ceil_div(features.extent, Tile::BN);
   logits_fwd_kernel<Tile, T><<<(unsigned)tiles, Tile::kThreads, 0, s>>>(
-      table, features, (int)p.dp(), p.products(), scale2, targets, (int)f.tiles_m, f.stats, f.label);
+      table, features, (int)p.dp(), p.products(), scale2, targets, (int)f.tiles_m, (int)ceil_div(features.extent, Tile::BN), f.stats, f.label);
 }
 
-static int forward(const Problem& p, Targets targets, float logit_scale, int reduction, float* loss, float* lse2,
+static int forward(const Problem& p, Targets targets, float logit_scale, int reduction, float* loss, float2* norm,
                    int64_t* count, const ForwardPlan& f, hipStream_t s) {
   if (p.rows == 0) {
     total_kernel<<<1, kJoinThreads, 0, s>>>(nullptr, 0, reduction, loss, count);
@@ -547,8 +567,8 @@ static int forward(const Problem& p, Targets targets, float logit_scale, int red
     else launch_logits_fwd<__bf16>(p, f, table, features, scale2, targets.from(r), s);
     const int64_t blocks = ceil_div(rows, kJoinThreads / f.lanes);
     auto* join = f.lanes == 64 ? join_kernel<64> : join_kernel<1>;
-    join<<<(unsigned)blocks, kJoinThreads, 0, s>>>(f.stats, f.label, (int)rows, (int)f.tiles_m, p.vocab, targets.from(r),
-                                                   reduction, lse2 ? lse2 + r : nullptr,
+    join<<<(unsigned)blocks, kJoinThreads, 0, s>>>(f.stats, f.label, (int)rows, (int)f.tiles_m, p.vocab, scale2,
+                                                   targets.from(r), reduction, norm ? norm + r : nullptr,
                                                    reduction == GS_REDUCE_NONE ? loss + r : nullptr,
                                                    f.partial + block, f.blocks == 1, loss, count);
     block += blocks;
@@ -603,7 +623,7 @@ struct BackwardPlan {
 static unsigned finish_blocks(int64_t n) { return (unsigned)min(ceil_div(n, 256), (int64_t)8192); }
 
 template <typename T, typename Out, int kPlanes>
-static int backward(const Problem& p, Targets targets, float logit_scale, int reduction, const float* lse2,
+static int backward(const Problem& p, Targets targets, float logit_scale, int reduction, const float2* norm,
                     const int64_t* count, const float* grad_loss, Out* grad_features, Out* grad_table,
                     const BackwardPlan& b, hipStream_t s) {
   const float scale2 = logit_scale * kLog2e;
@@ -630,28 +650,28 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
       piece.extent = cols;
       const int tiles_v = (int)ceil_div(cols, Tile::BM);
       logits_bwd_kernel<Tile, T, kPlanes><<<(unsigned)(tiles_v * ceil_div(rows, Tile::BN)), Tile::kThreads, 0, s>>>(
-          piece, features, (int)p.dp(), p.products(), scale2, targets.from(r), c, tiles_v, lse2 + r, b.factor + r,
+          piece, features, (int)p.dp(), p.products(), scale2, targets.from(r), c, tiles_v, (int)ceil_div(rows, Tile::BN), norm + r, b.factor + r,
           counts, b.ds, b.ld, ds_plane);
       if (grad_features) {
         const Operand ds = {b.ds, b.ld, ds_plane, (int32_t)rows};
         Operand x = piece;  // D columns of the piece's rows
         x.extent = D;
-        const int64_t k_part = round_up(ceil_div(cols, b.parts_h), kBK);
+        const int32_t k_part = (int32_t)round_up(ceil_div(cols, b.parts_h), kBK);
         grad_kernel<Tile, T, Out, false><<<dim3((unsigned)(tiles_d * ceil_div(rows, Tile::BN)), b.parts_h),
                                            Tile::kThreads, 0, s>>>(
-            x, ds, cols, k_part, p.products(), counts, tiles_d, b.direct_h ? nullptr : b.part_h, rows * D, c > 0,
+            x, ds, cols, k_part, p.products(), counts, tiles_d, (int)ceil_div(rows, Tile::BN), b.direct_h ? nullptr : b.part_h, rows * D, c > 0,
             b.alpha, grad_features + r * D);
       }
       if (grad_table) {
         const Operand ds = {b.ds, b.ld, ds_plane, cols};
         Operand x = features;
         x.extent = D;
-        const int64_t k_part = round_up(ceil_div(rows, b.parts_t), kBK);
+        const int32_t k_part = (int32_t)round_up(ceil_div(rows, b.parts_t), kBK);
         float* part = b.direct_t ? nullptr : b.part_t + (b.row_pieces > 1 ? c * D : 0);
         const int64_t part_plane = (b.row_pieces > 1 ? (int64_t)p.vocab : cols) * D;
         grad_kernel<Tile, T, Out, true><<<dim3((unsigned)(tiles_d * ceil_div(cols, Tile::BN)), b.parts_t),
                                           Tile::kThreads, 0, s>>>(
-            x, ds, rows, k_part, p.products(), counts, tiles_d, part, part_plane, r > 0, b.alpha, grad_table + c * D);
+            x, ds, (int32_t)rows, k_part, p.products(), counts, tiles_d, (int)ceil_div(cols, Tile::BN), part, part_plane, r > 0, b.alpha, grad_table + c * D);
         if (part && b.row_pieces == 1)
           finish_kernel<<<finish_blocks((int64_t)cols * D), 256, 0, s>>>(part, b.parts_t, part_plane, (int64_t)cols * D,
                                                                         D, nullptr, b.alpha, grad_table + c * D);
@@ -691,7 +711,7 @@ extern "C" size_t gs_xent_fwd_workspace_bytes(int64_t rows, int32_t vocab, int32
 extern "C" int gs_xent_fwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void* features,
                            int64_t ld_features, const void* table, int64_t ld_table, const void* targets,
                            int32_t target_bits, int64_t ignore_index, float logit_scale, int32_t reduction, float* loss,
-                           float* lse, int64_t* count, void* workspace, size_t workspace_bytes, void* stream) {
+                           float* norm, int64_t* count, void* workspace, size_t workspace_bytes, void* stream) {
   const Problem p = {rows, vocab, dim, dtype, features, ld_features, table, ld_table};
   int status = gs_xent::check(p);
   if (status != GS_OK) return status;
@@ -703,7 +723,7 @@ extern "C" int gs_xent_fwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dty
   if (rows > 0 && (!workspace || workspace_bytes < gs_xent::ForwardPlan(p, nullptr).bytes)) return GS_ERR_SCRATCH_TOO_SMALL;
   if (rows == 0) workspace = nullptr;
   const gs_xent::ForwardPlan f(p, workspace);
-  return gs_xent::forward(p, {targets, target_bits, ignore_index}, logit_scale, reduction, loss, lse, count, f,
+  return gs_xent::forward(p, {targets, target_bits, ignore_index}, logit_scale, reduction, loss, (float2*)norm, count, f,
                           (hipStream_t)stream);
 }
 
@@ -718,7 +738,7 @@ extern "C" size_t gs_xent_bwd_workspace_bytes(int64_t rows, int32_t vocab, int32
 extern "C" int gs_xent_bwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void* features,
                            int64_t ld_features, const void* table, int64_t ld_table, const void* targets,
                            int32_t target_bits, int64_t ignore_index, float logit_scale, int32_t reduction,
-                           const float* lse, const int64_t* count, const float* grad_loss, void* grad_features,
+                           const float* norm, const int64_t* count, const float* grad_loss, void* grad_features,
                            void* grad_table, void* workspace, size_t workspace_bytes, void* stream) {
   const Problem p = {rows, vocab, dim, dtype, features, ld_features, table, ld_table};
   int status = gs_xent::check(p);
@@ -733,7 +753,7 @@ extern "C" int gs_xent_bwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dty
     }
     return gs_status_from_hip(hipGetLastError());
   }
-  if (!targets || !lse || !grad_loss || !count) return GS_ERR_INVALID_ARGUMENT;
+  if (!targets || !norm || !grad_loss || !count) return GS_ERR_INVALID_ARGUMENT;
   if ((status = gs_xent::check_pointers(p)) != GS_OK) return status;
   if ((uintptr_t)workspace & 255) return GS_ERR_MISALIGNED;
   const bool want_h = grad_features != nullptr, want_t = grad_table != nullptr;
@@ -742,11 +762,11 @@ extern "C" int gs_xent_bwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dty
   const gs_xent::BackwardPlan b(p, want_h, want_t, workspace);
   const gs_xent::Targets t = {targets, target_bits, ignore_index};
   if (dtype == GS_FP32)
-    return gs_xent::backward<__bf16, float, 3>(p, t, logit_scale, reduction, lse, count, grad_loss,
+    return gs_xent::backward<__bf16, float, 3>(p, t, logit_scale, reduction, (const float2*)norm, count, grad_loss,
                                                (float*)grad_features, (float*)grad_table, b, s);
   if (dtype == GS_BF16)
-    return gs_xent::backward<__bf16, __bf16, 1>(p, t, logit_scale, reduction, lse, count, grad_loss,
+    return gs_xent::backward<__bf16, __bf16, 1>(p, t, logit_scale, reduction, (const float2*)norm, count, grad_loss,
                                                 (__bf16*)grad_features, (__bf16*)grad_table, b, s);
-  return gs_xent::backward<_Float16, _Float16, 1>(p, t, logit_scale, reduction, lse, count, grad_loss,
+  return gs_xent::backward<_Float16, _Float16, 1>(p, t, logit_scale, reduction, (const float2*)norm, count, grad_loss,
                                                   (_Float16*)grad_features, (_Float16*)grad_table, b, s);
 }

@@ -141,12 +141,12 @@ def embed_tokens(tokens: torch.Tensor, table: torch.Tensor, *, scale: float = 1.
 # ---------------------------------------------------------------- cross entropy
 
 def _entropy_forward(features, table, targets, ignore_index, reduction, logit_scale, keep: bool):
-    """(loss, lse or None, count) for 2-D features and 1-D targets."""
+    """(loss, norm or None, count) for 2-D features and 1-D targets."""
     device, n, (vocab, dim) = table.device, features.shape[0], table.shape
     lib = _lib.load()
     code, reduce = _DTYPES[table.dtype], _REDUCTIONS[reduction]
     loss = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=device)
-    lse = torch.empty((n,), dtype=torch.float32, device=device) if keep else None
+    norm = torch.empty((n, 2), dtype=torch.float32, device=device) if keep else None
     with torch.cuda.device(device), _workspace.device_lock(device):
         nbytes = lib.gs_xent_fwd_workspace_bytes(n, vocab, dim, code, _row_stride(features), _row_stride(table))
         # the count of rows sits in front of the workspace
@@ -155,23 +155,23 @@ def _entropy_forward(features, table, targets, ignore_index, reduction, logit_sc
         base = _aligned(space)
         lib.call("gs_xent_fwd", n, vocab, dim, code, features.data_ptr(), _row_stride(features), table.data_ptr(),
                  _row_stride(table), targets.data_ptr(), _INDEX_BITS[targets.dtype], ignore_index, logit_scale, reduce,
-                 loss.data_ptr(), _lib.ptr(lse), count.data_ptr() if keep else base, base if keep else base + 256,
+                 loss.data_ptr(), _lib.ptr(norm), count.data_ptr() if keep else base, base if keep else base + 256,
                  nbytes, _stream(device))
-    return loss, lse, count
+    return loss, norm, count
 
 
 class LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, features, table, targets, ignore_index, reduction, logit_scale):
-        loss, lse, count = _entropy_forward(features, table, targets, ignore_index, reduction, logit_scale, True)
-        ctx.save_for_backward(features, table, targets, lse, count)
+        loss, norm, count = _entropy_forward(features, table, targets, ignore_index, reduction, logit_scale, True)
+        ctx.save_for_backward(features, table, targets, norm, count)
         ctx.options = (ignore_index, reduction, logit_scale)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
-        features, table, targets, lse, count = ctx.saved_tensors
+        features, table, targets, norm, count = ctx.saved_tensors
         ignore_index, reduction, logit_scale = ctx.options
         want_features, want_table = ctx.needs_input_grad[:2]
         device, n, (vocab, dim) = table.device, features.shape[0], table.shape
@@ -186,7 +186,7 @@ class LinearCrossEntropy(torch.autograd.Function):
             space = _workspace_of(nbytes, device)
             lib.call("gs_xent_bwd", n, vocab, dim, code, features.data_ptr(), ldf, table.data_ptr(), ldt,
                      targets.data_ptr(), _INDEX_BITS[targets.dtype], ignore_index, logit_scale, _REDUCTIONS[reduction],
-                     lse.data_ptr(), count.data_ptr(), grad_loss.data_ptr(), _lib.ptr(grad_features),
+                     norm.data_ptr(), count.data_ptr(), grad_loss.data_ptr(), _lib.ptr(grad_features),
                      _lib.ptr(grad_table), _aligned(space), nbytes, _stream(device))
         return grad_features, grad_table, None, None, None, None
 
