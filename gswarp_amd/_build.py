@@ -36,6 +36,10 @@ HIPCC_FLAGS = (
     "-target-feature",
     "-Xclang",
     "-packed-fp32-ops",
+    # matrix-core accumulators in ordinary registers: the epilogues read them
+    # without a move each (only xent.hip holds matrix instructions)
+    "-mllvm",
+    "-amdgpu-mfma-vgpr-form",
     "-Wall",
     "-Wno-unused-function",
 )

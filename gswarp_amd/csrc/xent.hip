@@ -95,15 +95,28 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, in
   }
 }
 
+// m of element e of accumulator block a, from the lane's first m.
+__device__ __forceinline__ constexpr int block_m(int a, int e) { return 32 * a + 8 * (e >> 2) + (e & 3); }
+
+// A target as a distance from the lane's first m (base: the piece's first row of
+// the table, vocab: the piece's rows); -1 outside the piece or the wave's part of
+// the tile (a distance may still belong to the other half of the wave).
+__device__ __forceinline__ int from_first(int64_t target, int64_t base, int first, int wave_m, int vocab) {
+  if (target < base || target >= base + vocab) return -1;
+  const int d = (int)(target - base) - first;
+  return d >= 0 && d < wave_m ? d : -1;
+}
+
 // ------------------------------------------------------------------ forward
 // The logits of a tile (vocabulary m x rows n), reduced to one pair per row:
 // stats[tile * rows + row] = (max, sum of 2^(s log2 e - max)), max the largest
 // s log2 e rounded to fp32 (the exponents are formed from the unrounded product).
-// The tile that holds a row's target also writes its dot product.
+// The tile that holds a row's target also writes its dot product.  scale2 > 0;
+// flip: the dot products change their signs first (a negative scale).
 template <class S, typename T>
 __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, Operand features, int dim,
-                                                                 int products, float scale2, Targets targets,
-                                                                 int tiles_m, int tiles_n,
+                                                                 int products, float scale2, bool flip,
+                                                                 Targets targets, int tiles_m, int tiles_n,
                                                                  float2* __restrict__ stats,
                                                                  float* __restrict__ label_logit) {
   __shared__ __attribute__((aligned(16))) char lds[S::kLdsBytes];
@@ -115,52 +128,55 @@ __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, 
   const int lane = threadIdx.x & 63;
   const int wm = gs_tile::wave_m<S>(), wn = gs_tile::wave_n<S>();
   float2* red = reinterpret_cast<float2*>(lds);  // [kWavesM][BN]
-  // kWhole: no m of the tile lies past the vocabulary
-  auto reduce = [&](auto kWhole, int b) {
+  if (flip) {
+#pragma unroll
+    for (int a = 0; a < S::kMB; ++a)
+#pragma unroll
+      for (int b = 0; b < S::kNB; ++b) acc.c[a][b] = -acc.c[a][b];
+  }
+  const int first = m0 + wm + 4 * (lane >> 5);  // the lane's first m
+#pragma unroll
+  for (int b = 0; b < S::kNB; ++b) {
     const int n = n0 + wn + 32 * b + (lane & 31);
-    const int first = m0 + wm + 4 * (lane >> 5);  // the lane's first m
-    const auto past = [&](int a, int e) {
-      return !kWhole && first + 32 * a + 8 * (e >> 2) + (e & 3) >= table.extent;
-    };
-    const int64_t target = n < features.extent ? targets.at(n) : -1;
-    const bool here = target >= m0 + wm && target < m0 + wm + S::kWaveM && target < table.extent;
-    if (__any(here)) {
+    const int label_at = from_first(n < features.extent ? targets.at(n) : -1, 0, first, S::kWaveM, table.extent);
+    if (__any(label_at >= 0)) {
+      float label = 0.0f;
+      bool mine = false;
 #pragma unroll
       for (int a = 0; a < S::kMB; ++a)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (here && target == first + 32 * a + 8 * (e >> 2) + (e & 3)) label_logit[n] = acc.c[a][b][e];
+          if (label_at == block_m(a, e)) {
+            label = acc.c[a][b][e];
+            mine = true;
+          }
+      if (mine) label_logit[n] = label;
     }
-    // the largest logit: under a negative scale the least product
-    float raw = scale2 < 0.0f ? INFINITY : -INFINITY;
+    if (m0 + S::BM > table.extent) {
+#pragma unroll
+      for (int a = 0; a < S::kMB; ++a)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (first + block_m(a, e) >= table.extent) acc.c[a][b][e] = -INFINITY;
+    }
+    float raw = acc.c[0][b][0];
 #pragma unroll
     for (int a = 0; a < S::kMB; ++a)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float v = past(a, e) ? raw : acc.c[a][b][e];
-        raw = scale2 < 0.0f ? fminf(raw, v) : fmaxf(raw, v);
-      }
-    const float other = __shfl_xor(raw, 32);
-    raw = scale2 < 0.0f ? fminf(raw, other) : fmaxf(raw, other);
-    const float top = scale2 == 0.0f ? 0.0f : raw * scale2;
+      for (int e = 0; e < 16; ++e) raw = fmaxf(raw, acc.c[a][b][e]);
+    raw = fmaxf(raw, __shfl_xor(raw, 32));
+    const float top = raw * scale2;
     const float ref = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
+    // four sums, so that no addition waits for the one before
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int a = 0; a < S::kMB; ++a)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[a][b][e], scale2, -ref));
-        sum += past(a, e) ? 0.0f : v;
-      }
-    sum += __shfl_xor(sum, 32);
-    if (lane < 32) red[(wm / S::kWaveM) * S::BN + wn + 32 * b + lane] = make_float2(top, sum);
-  };
-  if (m0 + S::BM <= table.extent) {
-#pragma unroll
-    for (int b = 0; b < S::kNB; ++b) reduce(std::true_type{}, b);
-  } else {
-#pragma unroll
-    for (int b = 0; b < S::kNB; ++b) reduce(std::false_type{}, b);
+      for (int e = 0; e < 16; ++e)
+        sum[e & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[a][b][e], scale2, -ref));
+    float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    all += __shfl_xor(all, 32);
+    if (lane < 32) red[(wm / S::kWaveM) * S::BN + wn + 32 * b + lane] = make_float2(top, all);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < S::BN; i += S::kThreads) {
@@ -353,36 +369,68 @@ __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, 
   gs_tile::product<S, T, true, true>(acc, table, features, m0, n0, 0, dim, products, nullptr, lds);
   const int lane = threadIdx.x & 63;
   const int wm = gs_tile::wave_m<S>(), wn = gs_tile::wave_n<S>();
+  const int first = m0 + wm + 4 * (lane >> 5);  // the lane's first m
 #pragma unroll
   for (int b = 0; b < S::kNB; ++b) {
-    const int n = n0 + wn + 32 * b + (lane & 31);
-    if (n >= features.extent) continue;
-    const int first = m0 + wm + 4 * (lane >> 5);
-    const int64_t target = targets.at(n) - m_base;
-    const float top = norm[n].x, f = factor[n], share = f * norm[n].y;
-    const bool use = row_counts(counts, n);
-    uint16_t* out = ds + (int64_t)n * ld + first;
+    const int n = min(n0 + wn + 32 * b + (lane & 31), features.extent - 1);
+    const int label_at = from_first(targets.at(n), m_base, first, S::kWaveM, table.extent);
+    const float2 z = norm[n];
+    const float f = factor[n], share = f * z.y;
 #pragma unroll
     for (int a = 0; a < S::kMB; ++a)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        typename gs_tile::Pack<T>::v4 held[kPlanes];
+      for (int e = 0; e < 16; ++e)
+        acc.c[a][b][e] = share * __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[a][b][e], scale2, -z.x));
+    if (__any(label_at >= 0)) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int m = first + 32 * a + 8 * q + j;
-          float v = __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[a][b][4 * q + j], scale2, -top));
-          v = __builtin_fmaf(v, share, m == target ? -f : 0.0f);
-          v = use && m < table.extent ? v : 0.0f;
+      for (int a = 0; a < S::kMB; ++a)
 #pragma unroll
-          for (int p = 0; p < kPlanes; ++p) {
-            held[p][j] = (T)v;
-            v -= (float)held[p][j];
+        for (int e = 0; e < 16; ++e) acc.c[a][b][e] -= label_at == block_m(a, e) ? f : 0.0f;
+    }
+    if (m0 + S::BM > table.extent) {
+#pragma unroll
+      for (int a = 0; a < S::kMB; ++a)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (first + block_m(a, e) >= table.extent) acc.c[a][b][e] = 0.0f;
+    }
+  }
+  // Through LDS, so that the stores are 16 bytes of whole rows: BN rows of BM
+  // values, 16 bytes apart from a multiple of the banks, which keeps both sides free of conflicts.
+  constexpr int kPitch = S::BM * 2 + 16;
+  static_assert(S::BN * kPitch <= S::kLdsBytes, "the tile of ds fits where the operands were");
+#pragma unroll
+  for (int p = 0; p < kPlanes; ++p) {
+    if (p > 0) __syncthreads();
+#pragma unroll
+    for (int b = 0; b < S::kNB; ++b) {
+      const int row = wn + 32 * b + (lane & 31);
+      const uint32_t use = n0 + row < features.extent && row_counts(counts, n0 + row) ? ~0u : 0u;
+#pragma unroll
+      for (int a = 0; a < S::kMB; ++a)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          typename gs_tile::Pack<T>::v4 held;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float v = acc.c[a][b][4 * q + j];
+            held[j] = (T)v;
+            if (kPlanes > 1) acc.c[a][b][4 * q + j] = v - (float)held[j];
           }
+          // a row that does not count holds zeros whatever came out above
+          gs_tile::u32x2 bits = __builtin_bit_cast(gs_tile::u32x2, held);
+          bits &= use;
+          *reinterpret_cast<gs_tile::u32x2*>(lds + row * kPitch + (wm + 32 * a + 8 * q + 4 * (lane >> 5)) * 2) = bits;
         }
-#pragma unroll
-        for (int p = 0; p < kPlanes; ++p)
-          *reinterpret_cast<typename gs_tile::Pack<T>::v4*>(out + p * plane + 32 * a + 8 * q) = held[p];
-      }
+    }
+    __syncthreads();
+    constexpr int kRowVectors = S::BM / 8;
+    for (int i = threadIdx.x; i < S::BN * kRowVectors; i += S::kThreads) {
+      const int row = i / kRowVectors, v = i % kRowVectors;
+      if (n0 + row >= features.extent) break;
+      *reinterpret_cast<gs_tile::u32x4*>(ds + p * plane + (int64_t)(n0 + row) * ld + m0 + v * 8) =
+          *reinterpret_cast<const gs_tile::u32x4*>(lds + row * kPitch + v * 16);
+    }
   }
 }
 
@@ -514,6 +562,13 @@ static Operand operand(const Problem& p, const void* src, int64_t ld, int64_t fi
   return {space, p.dp(), rows * p.dp(), (int32_t)rows};
 }
 
+// The logits' scale in base 2.  Zero becomes the least normal number: the same
+// flat distribution, and minus infinity (what lies past the vocabulary) stays that.
+static float base2_scale(float logit_scale) {
+  const float scale2 = logit_scale * kLog2e;
+  return scale2 == 0.0f ? 1.17549435e-38f : scale2;
+}
+
 struct ForwardPlan {
   int64_t rows_piece, tiles_m, blocks;
   int lanes;
@@ -548,7 +603,7 @@ static void launch_logits_fwd(const Problem& p, const ForwardPlan& f, const Oper
                               float scale2, Targets targets, hipStream_t s) {
   const int64_t tiles = f.tiles_m * ceil_div(features.extent, Tile::BN);
   logits_fwd_kernel<Tile, T><<<(unsigned)tiles, Tile::kThreads, 0, s>>>(
-      table, features, (int)p.dp(), p.products(), scale2, targets, (int)f.tiles_m, (int)ceil_div(features.extent, Tile::BN), f.stats, f.label);
+      table, features, (int)p.dp(), p.products(), fabsf(scale2), scale2 < 0.0f, targets, (int)f.tiles_m, (int)ceil_div(features.extent, Tile::BN), f.stats, f.label);
 }
 
 static int forward(const Problem& p, Targets targets, float logit_scale, int reduction, float* loss, float2* norm,
@@ -557,7 +612,7 @@ static int forward(const Problem& p, Targets targets, float logit_scale, int red
     total_kernel<<<1, kJoinThreads, 0, s>>>(nullptr, 0, reduction, loss, count);
     return gs_status_from_hip(hipGetLastError());
   }
-  const float scale2 = logit_scale * kLog2e;
+  const float scale2 = base2_scale(logit_scale);
   const Operand table = operand(p, p.table, p.ld_table, 0, p.vocab, f.table, s);
   int64_t block = 0;
   for (int64_t r = 0; r < p.rows; r += f.rows_piece) {
@@ -567,7 +622,7 @@ static int forward(const Problem& p, Targets targets, float logit_scale, int red
     else launch_logits_fwd<__bf16>(p, f, table, features, scale2, targets.from(r), s);
     const int64_t blocks = ceil_div(rows, kJoinThreads / f.lanes);
     auto* join = f.lanes == 64 ? join_kernel<64> : join_kernel<1>;
-    join<<<(unsigned)blocks, kJoinThreads, 0, s>>>(f.stats, f.label, (int)rows, (int)f.tiles_m, p.vocab, scale2,
+    join<<<(unsigned)blocks, kJoinThreads, 0, s>>>(f.stats, f.label, (int)rows, (int)f.tiles_m, p.vocab, fabsf(scale2),
                                                    targets.from(r), reduction, norm ? norm + r : nullptr,
                                                    reduction == GS_REDUCE_NONE ? loss + r : nullptr,
                                                    f.partial + block, f.blocks == 1, loss, count);
@@ -626,7 +681,7 @@ template <typename T, typename Out, int kPlanes>
 static int backward(const Problem& p, Targets targets, float logit_scale, int reduction, const float2* norm,
                     const int64_t* count, const float* grad_loss, Out* grad_features, Out* grad_table,
                     const BackwardPlan& b, hipStream_t s) {
-  const float scale2 = logit_scale * kLog2e;
+  const float scale2 = base2_scale(logit_scale);
   const int D = p.dim;
   int largest_n = 0;
   if (reduction == GS_REDUCE_NONE) {
