@@ -10,11 +10,15 @@
 // and the two gradients) read the same row-major matrices, and nothing is ever
 // transposed in memory.
 //
-// fp32 operands are held as three bf16 planes whose sum is the value exactly
-// (8 + 8 + 8 significant bits); the six products of planes that matter at fp32's
-// precision (each dropped one is below 2^-26 of the product) run through the
-// same kernel as six times the K steps, smallest first.  The matrix cores' own
-// fp32 form has a sixteenth of the bf16 rate, so this is faster by 16 / 6.
+// fp32 operands are held as fp16 planes, hi + lo / 2^11, of the values times a
+// power of two that brings the matrix's largest magnitude to 2^13..2^14 (its
+// unit; the results are multiplied by it).  Together they have 22 bits, down to
+// 2^-28 of the largest magnitude, and below it an error of 2^-50 of that.  Three
+// products of planes (lo hi and hi lo, whose sum is then divided by 2^11, and hi
+// hi; lo lo is below 2^-24 of the product, as fp32's own rounding) run through
+// the same kernel as three times the K steps.  The matrix cores' own fp32 form
+// has a sixteenth of the fp16 rate, so this is faster by 16 / 3.  An operand Y of
+// wider range (gradients of the logits: probabilities) adds a third plane, + tiny / 2^22, and a fourth product.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -49,12 +53,19 @@ struct Operand {
   int32_t extent;
 };
 
-// Which planes of X and Y the s-th product takes (4 bits each, low first).
-__device__ __forceinline__ int product_plane(uint32_t planes, int s) { return (planes >> (4 * s)) & 15; }
-constexpr uint32_t kPlanesX = 0x001012u;
-constexpr uint32_t kPlanesY = 0x010210u;
-constexpr int kSplitPlanes = 3;
-constexpr int kSplitProducts = 6;
+constexpr int kSplitPlanes = 2, kWidePlanes = 3;      // of an fp32 operand, of one of wide range
+constexpr int kSplitProducts = 3, kWideProducts = 4;  // of two fp32 operands, with a wide Y
+constexpr float kPlaneStep = 2048.0f;                 // what each plane is held times more than the one before
+// The planes of X and Y that product s of `products` takes: (hi, tiny) if there are
+// four, (lo, hi), (hi, lo), (hi, hi).  Before (lo, hi), if not the first, and
+// before (hi, hi) the sums so far are divided by a step.
+__device__ __forceinline__ int plane_x(int products, int s) { return products > 1 && s == products - 3; }
+__device__ __forceinline__ int plane_y(int products, int s) {
+  return products == 1 ? 0 : s == products - 2 ? 1 : s == products - 4 ? 2 : 0;
+}
+__device__ __forceinline__ bool steps_down(int products, int s) {
+  return (s > 0 && s == products - 3) || (products > 1 && s == products - 1);
+}
 
 __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -175,15 +186,16 @@ struct Stage {
   }
 };
 
-// The tile shape: kWavesM x kWavesN waves, each (BM / kWavesM) x (BN / kWavesN).
-template <int kBM, int kBN, int kWavesM_, int kWavesN_>
+// The tile shape: kWavesM x kWavesN waves, each (BM / kWavesM) x (BN / kWavesN),
+// kStages steps of K in LDS.
+template <int kBM, int kBN, int kWavesM_, int kWavesN_, int kStages_ = 2>
 struct Shape {
   static constexpr int BM = kBM, BN = kBN;
-  static constexpr int kWavesM = kWavesM_, kWavesN = kWavesN_;
+  static constexpr int kWavesM = kWavesM_, kWavesN = kWavesN_, kStages = kStages_;
   static constexpr int kWaves = kWavesM * kWavesN, kThreads = 64 * kWaves;
   static constexpr int kWaveM = BM / kWavesM, kWaveN = BN / kWavesN;
   static constexpr int kMB = kWaveM / 32, kNB = kWaveN / 32;
-  static constexpr int kLdsBytes = 2 * (BM + BN) * 128;
+  static constexpr int kLdsBytes = kStages * (BM + BN) * 128;
 };
 
 // The accumulators of a wave.  Block (a, b) covers rows m = wave_m + 32 a and
@@ -229,14 +241,15 @@ __device__ __forceinline__ void multiply(Accumulators<S>& acc, int wm, int wn, c
   }
 }
 
-// acc = the tile at (m0, n0), over K columns [k_begin, k_end) of products
-// `products` (1, or 6 for fp32 planes).  Every element outside the operands
+// acc = the tile at (m0, n0), over K columns [k_begin, k_end) of
+// `products` products of planes (1, 3 or 4).  Every element outside the operands
 // counts as zero.  x_rows (X in K rows only, may be null): one bit per K row
 // (k_begin on a multiple of 64); rows whose bit is clear count as zero whatever
 // they hold.  lds: S::kLdsBytes, free for the caller after a barrier.
 //
-// Two LDS buffers: the loads of step t + 1 go straight into one while the matrix
-// cores work on the other; one barrier per step.
+// LDS holds a ring of kStages steps: while the matrix cores work on step t, the
+// loads of the kStages - 1 steps behind it are on their way into the ring; one
+// barrier per step, passed when the wave's own loads of step t have arrived.
 template <class S, typename T, bool kXAlongK, bool kYAlongK>
 __device__ __forceinline__ void product(Accumulators<S>& acc, const Operand& x, const Operand& y, int m0, int n0,
                                         int32_t k_begin, int32_t k_end, int products, const uint64_t* x_rows,
@@ -261,8 +274,7 @@ __device__ __forceinline__ void product(Accumulators<S>& acc, const Operand& x, 
   const bool masked = !kXAlongK && x_rows;
   auto load = [&](char* to) {
     const int32_t k0 = k_begin + step * kBK;
-    const int px = products == 1 ? 0 : product_plane(kPlanesX, prod);
-    const int py = products == 1 ? 0 : product_plane(kPlanesY, prod);
+    const int px = plane_x(products, prod), py = plane_y(products, prod);
     uint64_t mask = ~0ull;
     if (masked) {
       if ((step & 63) == 0) {
@@ -279,14 +291,42 @@ __device__ __forceinline__ void product(Accumulators<S>& acc, const Operand& x, 
       ++prod;
     }
   };
-  load(lds);
-  __syncthreads();
+  constexpr int kAhead = S::kStages - 1, kLoads = StageX::kLoads + StageY::kLoads;
+  static_assert(S::kStages == 2 || (kXAlongK && kYAlongK), "the masks' loads would count among the steps'");
+  int to = 0;  // the stage that the next loads fill
+#pragma unroll
+  for (int t = 0; t < kAhead; ++t)
+    if (t < total) {
+      load(lds + to * kBuffer);
+      to = to + 1 == S::kStages ? 0 : to + 1;
+    }
   const int wm = wave_m<S>(), wn = wave_n<S>();
+  int at = 0, product_at = 0, next = 0;
   for (int t = 0; t < total; ++t) {
-    if (t + 1 < total) load(lds + ((t + 1) & 1) * kBuffer);
-    multiply<S, T, StageX, StageY>(acc, wm, wn, lds + (t & 1) * kBuffer);
-    __syncthreads();
+    // loads return in order: at most those of the steps behind step t may be under
+    // way; and the reads of the stage that is filled next are over
+    if (t + kAhead <= total) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kAhead - 1) * kLoads) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (t + kAhead < total) {
+      load(lds + to * kBuffer);
+      to = to + 1 == S::kStages ? 0 : to + 1;
+    }
+    if (t == next) {  // the first step of a product
+      if (steps_down(products, product_at)) {
+#pragma unroll
+        for (int a = 0; a < S::kMB; ++a)
+#pragma unroll
+          for (int b = 0; b < S::kNB; ++b) acc.c[a][b] *= 1.0f / kPlaneStep;
+      }
+      ++product_at;
+      next += steps;
+    }
+    multiply<S, T, StageX, StageY>(acc, wm, wn, lds + at * kBuffer);
+    at = at + 1 == S::kStages ? 0 : at + 1;
   }
+  __syncthreads();
 }
 
 // The tile of a block: blocks go to the 8 XCDs (each with an L2 of its own) in

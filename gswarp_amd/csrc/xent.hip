@@ -23,17 +23,29 @@ using gs_tile::Accumulators;
 using gs_tile::kBK;
 using gs_tile::Operand;
 
-typedef gs_tile::Shape<128, 128, 2, 2> Tile;
+// The tile shapes (BM, BN, waves along each, stages).  Big has twice Mid's reuse
+// of what it loads and one workgroup a CU; Mid wastes less on small sides and
+// two of its workgroups overlap.  Narrow: gradients of at most 64 columns.
+// Thin: few rows, where the table streams through once and what counts is how
+// many bytes are under way (two workgroups a CU, four or five steps each).
+typedef gs_tile::Shape<256, 256, 2, 4> Big;
+typedef gs_tile::Shape<128, 128, 2, 2> Mid;
+typedef gs_tile::Shape<64, 256, 1, 4> Narrow;
+typedef gs_tile::Shape<64, 32, 2, 1, 6> Thin32;
+typedef gs_tile::Shape<64, 64, 2, 1, 5> Thin64;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.6931471805599453;
 constexpr int kJoinThreads = 256;
-constexpr int64_t kRowsPiece = 65536;          // rows of a piece (a multiple of 64 and of the tile)
-constexpr int64_t kPieceBytes = 512ll << 20;   // ds of one piece, all planes
+constexpr int64_t kPieceBytes = 1ll << 30;     // ds of one piece, all planes
+constexpr int64_t kLeastSide = 4096;           // rows or vocabulary of a piece, at least (a multiple of the tiles')
 constexpr int64_t kStatBytes = 256ll << 20;    // the tiles' pairs of one piece (forward)
-// fp16 has 2^-14 as its least normal number: ds (at most 1 in magnitude after
-// the division by the largest g) is held times 2^15, so that probabilities down to 2^-29 keep all
-// their bits.  bf16 has fp32's exponents and needs no scale.
+// fp16 (and fp32's planes) have 2^-14 as their least normal number: ds (at most 1
+// in magnitude after the division by the largest g) is held times 2^15, so that
+// probabilities down to 2^-29 keep all their bits.  bf16 has fp32's exponents and
+// needs no scale.  Rounding ds to 16 bits adds an error of the size of the
+// results' own rounding to the same type; fp32's three planes keep 22 bits of
+// probabilities down to 2^-51, and an error of 2^-62.
 template <typename T>
 struct Held {
   static constexpr float kScale = 1.0f;
@@ -56,43 +68,98 @@ struct Targets {
 };
 
 // ------------------------------------------------------------------ packing
+// fp32: the largest finite magnitude of a matrix, one value a block (targets.p:
+// of the rows that count only, so that what ignored rows hold does not reach the unit of the others).
+constexpr int kLargestBlocks = 1024;
+__global__ __launch_bounds__(256) void magnitude_kernel(const float* __restrict__ src, int64_t ld, int64_t rows,
+                                                        int dim, Targets targets, float* __restrict__ largest) {
+  __shared__ float lds[4];
+  const int lane = threadIdx.x & 63;
+  const int64_t waves = (int64_t)gridDim.x * 4;
+  float top = 0.0f;
+  constexpr int kRows = 8;  // rows in flight
+  for (int64_t r0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * kRows; r0 < rows; r0 += waves * kRows) {
+    for (int c = lane; c < dim; c += 64) {
+      float v[kRows];
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) v[j] = r0 + j < rows ? fabsf(src[(r0 + j) * ld + c]) : 0.0f;
+#pragma unroll
+      for (int j = 0; j < kRows; ++j)
+        if (v[j] < INFINITY && v[j] > top && (!targets.p || targets.at(r0 + j) != targets.ignore)) top = v[j];
+    }
+  }
+#pragma unroll
+  for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+  if (lane == 0) lds[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) largest[blockIdx.x] = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
+}
+
+// The unit of a matrix from its blocks' magnitudes: the power of two 2^e with
+// largest / 2^e in [2^13, 2^14) (one workgroup of 256 threads).
+__device__ __forceinline__ float unit_of(const float* __restrict__ largest, int n) {
+  __shared__ float lds[4];
+  float top = 0.0f;
+  for (int i = threadIdx.x; i < n; i += 256) top = fmaxf(top, largest[i]);
+#pragma unroll
+  for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
+  if (top == 0.0f) return 1.0f;
+  int e;
+  frexpf(top, &e);
+  return ldexpf(1.0f, max(e - 14, -126));
+}
+
 // A matrix laid out for the tile loads: rows of dp = ceil(dim / 8) * 8 16-bit
-// values, zero past dim; fp32 as three bf16 planes.  Only for fp32 and for
-// rows that the 16-byte loads cannot take (dim or ld not a multiple of 8).
+// values, zero past dim; fp32 as the planes hi and lo of value / unit (the unit
+// goes to *unit).  Only for fp32 and for rows that the 16-byte loads cannot take
+// (dim or ld not a multiple of 8).
 template <typename T>
 __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, int64_t ld, int64_t rows, int dim,
-                                                   int dp, uint16_t* __restrict__ dst, int64_t plane) {
+                                                   int dp, uint16_t* __restrict__ dst, int64_t plane,
+                                                   const float* __restrict__ largest, int largest_n,
+                                                   float* __restrict__ unit) {
+  float scale = 1.0f;
+  if constexpr (sizeof(T) == 4) {
+    const float u = unit_of(largest, largest_n);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *unit = u;
+    scale = 1.0f / u;
+  }
   const int64_t total = rows * (dp / 8);
   for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < total; v += (int64_t)gridDim.x * 256) {
     const int64_t row = v / (dp / 8);
     const int col = (int)(v - row * (dp / 8)) * 8;
     const T* s = src + row * ld + col;
-    uint16_t out[3][8];
+    uint16_t* d = dst + row * dp + col;
+    if constexpr (sizeof(T) == 4) {
+      gs_tile::f16x8 hi, lo;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if constexpr (sizeof(T) == 4) {
-        const float x = col + e < dim ? s[e] : 0.0f;
-        float left = x;
-#pragma unroll
-        for (int p = 0; p < 3; ++p) {
-          // the nearest bf16, or x cut short where that would be infinite; nothing is
-          // left of infinities and NaN
-          __bf16 part = (__bf16)left;
-          if (__builtin_isinf((float)part) && __builtin_isfinite(left))
-            part = __builtin_bit_cast(__bf16, (uint16_t)(__builtin_bit_cast(uint32_t, left) >> 16));
-          out[p][e] = __builtin_bit_cast(uint16_t, part);
-          left = __builtin_isfinite(x) ? left - (float)part : 0.0f;
-        }
-      } else {
-        out[0][e] = col + e < dim ? __builtin_bit_cast(uint16_t, s[e]) : (uint16_t)0;
+      for (int e = 0; e < 8; ++e) {
+        const float x = (col + e < dim ? s[e] : 0.0f) * scale;
+        hi[e] = (_Float16)x;
+        // nothing is left of infinities and NaN
+        lo[e] = fabsf(x) < INFINITY ? (_Float16)((x - (float)hi[e]) * gs_tile::kPlaneStep) : (_Float16)0.0f;
       }
-    }
-    constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
+      *reinterpret_cast<gs_tile::f16x8*>(d) = hi;
+      *reinterpret_cast<gs_tile::f16x8*>(d + plane) = lo;
+    } else {
+      uint16_t out[8];
 #pragma unroll
-    for (int p = 0; p < kPlanes; ++p)
-      *reinterpret_cast<gs_tile::u32x4*>(dst + p * plane + row * dp + col) =
-          *reinterpret_cast<const gs_tile::u32x4*>(out[p]);
+      for (int e = 0; e < 8; ++e) out[e] = col + e < dim ? __builtin_bit_cast(uint16_t, s[e]) : (uint16_t)0;
+      *reinterpret_cast<gs_tile::u32x4*>(d) = *reinterpret_cast<const gs_tile::u32x4*>(out);
+    }
   }
+}
+
+// What the tiles' dot products are multiplied by for base-2 logits: scale2 times
+// the operands' units (fp32), kept a normal number so that minus infinity (what
+// lies past the vocabulary) stays that under a scale that underflows, or is zero: the same flat
+// distribution.
+__device__ __forceinline__ float scale_of(float scale2, const float* units) {
+  if (units) scale2 = scale2 * units[0] * units[1];
+  return copysignf(fmaxf(fabsf(scale2), 1.17549435e-38f), scale2);
 }
 
 // m of element e of accumulator block a, from the lane's first m.
@@ -111,12 +178,12 @@ __device__ __forceinline__ int from_first(int64_t target, int64_t base, int firs
 // The logits of a tile (vocabulary m x rows n), reduced to one pair per row:
 // stats[tile * rows + row] = (max, sum of 2^(s log2 e - max)), max the largest
 // s log2 e rounded to fp32 (the exponents are formed from the unrounded product).
-// The tile that holds a row's target also writes its dot product.  scale2 > 0;
-// flip: the dot products change their signs first (a negative scale).
+// The tile that holds a row's target also writes its logit in the same units.
 template <class S, typename T>
 __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, Operand features, int dim,
-                                                                 int products, float scale2, bool flip,
-                                                                 Targets targets, int tiles_m, int tiles_n,
+                                                                 int products, float logit_scale2,
+                                                                 const float* __restrict__ units, Targets targets,
+                                                                 int tiles_m, int tiles_n,
                                                                  float2* __restrict__ stats,
                                                                  float* __restrict__ label_logit) {
   __shared__ __attribute__((aligned(16))) char lds[S::kLdsBytes];
@@ -125,10 +192,13 @@ __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, 
   Accumulators<S> acc;
   gs_tile::product<S, T, true, true>(acc, table, features, m0, n0, 0, dim, products, nullptr, lds);
 
+  float scale2 = scale_of(logit_scale2, units);
   const int lane = threadIdx.x & 63;
   const int wm = gs_tile::wave_m<S>(), wn = gs_tile::wave_n<S>();
   float2* red = reinterpret_cast<float2*>(lds);  // [kWavesM][BN]
-  if (flip) {
+  // under a negative scale the dot products change their signs first
+  if (scale2 < 0.0f) {
+    scale2 = -scale2;
 #pragma unroll
     for (int a = 0; a < S::kMB; ++a)
 #pragma unroll
@@ -150,7 +220,7 @@ __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, 
             label = acc.c[a][b][e];
             mine = true;
           }
-      if (mine) label_logit[n] = label;
+      if (mine) label_logit[n] = label;  // times scale2, in the join
     }
     if (m0 + S::BM > table.extent) {
 #pragma unroll
@@ -230,7 +300,8 @@ __device__ __forceinline__ void write_total(Sum s, int reduction, float* loss, i
 template <int kLanes>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float2* __restrict__ stats,
                                                             const float* __restrict__ label_logit, int rows,
-                                                            int tiles, int vocab, float scale2, Targets targets,
+                                                            int tiles, int vocab, float logit_scale2,
+                                                            const float* __restrict__ units, Targets targets,
                                                             int reduction, float2* __restrict__ norm,
                                                             float* __restrict__ loss_rows,
                                                             Sum* __restrict__ partial, bool last,
@@ -261,7 +332,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float2* __rest
     if (t != targets.ignore) {
       // in 64 bits, the maximum kept apart: small losses do not drown in the logits' size
       value = t >= 0 && t < vocab
-                  ? (float)(log(sum) + kLn2 * ((double)top - (double)label_logit[row] * (double)scale2))
+                  ? (float)(log(sum) + kLn2 * ((double)top - (double)label_logit[row] * (double)fabsf(scale_of(logit_scale2, units))))
                   : __builtin_nanf("");
       mine = {(double)value, 1};
     }
@@ -308,7 +379,6 @@ __global__ __launch_bounds__(256) void largest_kernel(const float* __restrict__ 
 // the row count.  With a gradient for each row the factors are g_i / G, G the
 // largest, so that ds stays in the 16-bit type's range; alpha, applied to the
 // sums, holds the rest.
-constexpr int kLargestBlocks = 256;
 __global__ __launch_bounds__(256) void factors_kernel(const float* __restrict__ grad, int64_t rows, int vocab,
                                                       Targets targets, int reduction, const int64_t* __restrict__ count,
                                                       float logit_scale, float held_scale,
@@ -319,7 +389,8 @@ __global__ __launch_bounds__(256) void factors_kernel(const float* __restrict__ 
   const int lane = threadIdx.x & 63;
   float G = 1.0f;
   if (reduction == GS_REDUCE_NONE) {
-    float top = (int)threadIdx.x < largest_n ? largest[threadIdx.x] : 0.0f;
+    float top = 0.0f;
+    for (int i = threadIdx.x; i < largest_n; i += 256) top = fmaxf(top, largest[i]);
 #pragma unroll
     for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
     if (lane == 0) lds[threadIdx.x >> 6] = top;
@@ -355,7 +426,8 @@ __device__ __forceinline__ bool row_counts(const uint64_t* counts, int64_t row) 
 // past the end are zeros.
 template <class S, typename T, int kPlanes>
 __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, Operand features, int dim,
-                                                                 int products, float scale2, Targets targets,
+                                                                 int products, float logit_scale2,
+                                                                 const float* __restrict__ units, Targets targets,
                                                                  int64_t m_base, int tiles_m, int tiles_n,
                                                                  const float2* __restrict__ norm,
                                                                  const float* __restrict__ factor,
@@ -367,6 +439,7 @@ __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, 
   const int m0 = tile.m * S::BM, n0 = tile.n * S::BN;
   Accumulators<S> acc;
   gs_tile::product<S, T, true, true>(acc, table, features, m0, n0, 0, dim, products, nullptr, lds);
+  const float scale2 = scale_of(logit_scale2, units);
   const int lane = threadIdx.x & 63;
   const int wm = gs_tile::wave_m<S>(), wn = gs_tile::wave_n<S>();
   const int first = m0 + wm + 4 * (lane >> 5);  // the lane's first m
@@ -395,17 +468,20 @@ __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, 
           if (first + block_m(a, e) >= table.extent) acc.c[a][b][e] = 0.0f;
     }
   }
-  // Through LDS, so that the stores are 16 bytes of whole rows: BN rows of BM
-  // values, 16 bytes apart from a multiple of the banks, which keeps both sides free of conflicts.
+  // Through LDS, so that the stores are 16 bytes of whole rows: for each column
+  // block the waves' rows of BM values, 16 bytes apart from a multiple of the
+  // banks, which keeps both sides free of conflicts.
   constexpr int kPitch = S::BM * 2 + 16;
-  static_assert(S::BN * kPitch <= S::kLdsBytes, "the tile of ds fits where the operands were");
+  constexpr int kRows = 32 * S::kWavesN;
+  static_assert(kRows * kPitch <= S::kLdsBytes, "a column block of ds fits where the operands were");
 #pragma unroll
-  for (int p = 0; p < kPlanes; ++p) {
-    if (p > 0) __syncthreads();
+  for (int b = 0; b < S::kNB; ++b) {
 #pragma unroll
-    for (int b = 0; b < S::kNB; ++b) {
-      const int row = wn + 32 * b + (lane & 31);
-      const uint32_t use = n0 + row < features.extent && row_counts(counts, n0 + row) ? ~0u : 0u;
+    for (int p = 0; p < kPlanes; ++p) {
+      if (p > 0 || b > 0) __syncthreads();
+      const int n = n0 + wn + 32 * b + (lane & 31);
+      const uint32_t use = n < features.extent && row_counts(counts, n) ? ~0u : 0u;
+      char* to = lds + (wn / S::kWaveN * 32 + (lane & 31)) * kPitch + (wm + 4 * (lane >> 5)) * 2;
 #pragma unroll
       for (int a = 0; a < S::kMB; ++a)
 #pragma unroll
@@ -415,21 +491,24 @@ __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, 
           for (int j = 0; j < 4; ++j) {
             const float v = acc.c[a][b][4 * q + j];
             held[j] = (T)v;
-            if (kPlanes > 1) acc.c[a][b][4 * q + j] = v - (float)held[j];
+            if (kPlanes > 1) acc.c[a][b][4 * q + j] = (v - (float)held[j]) * gs_tile::kPlaneStep;
           }
           // a row that does not count holds zeros whatever came out above
           gs_tile::u32x2 bits = __builtin_bit_cast(gs_tile::u32x2, held);
           bits &= use;
-          *reinterpret_cast<gs_tile::u32x2*>(lds + row * kPitch + (wm + 32 * a + 8 * q + 4 * (lane >> 5)) * 2) = bits;
+          *reinterpret_cast<gs_tile::u32x2*>(to + (32 * a + 8 * q) * 2) = bits;
         }
-    }
-    __syncthreads();
-    constexpr int kRowVectors = S::BM / 8;
-    for (int i = threadIdx.x; i < S::BN * kRowVectors; i += S::kThreads) {
-      const int row = i / kRowVectors, v = i % kRowVectors;
-      if (n0 + row >= features.extent) break;
-      *reinterpret_cast<gs_tile::u32x4*>(ds + p * plane + (int64_t)(n0 + row) * ld + m0 + v * 8) =
-          *reinterpret_cast<const gs_tile::u32x4*>(lds + row * kPitch + v * 16);
+      __syncthreads();
+      constexpr int kRowVectors = S::BM / 8;
+#pragma unroll
+      for (int j = 0; j < kRows * kRowVectors / S::kThreads; ++j) {
+        const int i = threadIdx.x + j * S::kThreads;
+        const int slot = i / kRowVectors, v = i % kRowVectors;
+        const int row = n0 + slot / 32 * S::kWaveN + 32 * b + slot % 32;
+        if (row < features.extent)
+          *reinterpret_cast<gs_tile::u32x4*>(ds + p * plane + (int64_t)row * ld + m0 + v * 8) =
+              *reinterpret_cast<const gs_tile::u32x4*>(lds + slot * kPitch + v * 16);
+      }
     }
   }
 }
@@ -438,14 +517,14 @@ __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, 
 // features or of the table), m the D columns.  kTableGrad: dw (both operands in
 // K rows, K the rows of the piece); else dh (ds along K, K the vocabulary).
 // With `part` set the tile goes, in fp32, to plane blockIdx.y of part (added to
-// what is there if `add`); else out = alpha * tile in the result's type.
+// what is there if `add`); else out = alpha * tile in the result's type (unit: x's, fp32).
 // rows_count (dh): rows that do not count are zero.
 template <class S, typename T, typename Out, bool kTableGrad>
 __global__ __launch_bounds__(S::kThreads) void grad_kernel(Operand x, Operand ds, int32_t K, int32_t k_part,
                                                            int products, const uint64_t* __restrict__ counts,
                                                            int tiles_m, int tiles_n, float* __restrict__ part, int64_t part_plane,
                                                            bool add, const float* __restrict__ alpha,
-                                                           Out* __restrict__ out) {
+                                                           const float* __restrict__ unit, Out* __restrict__ out) {
   __shared__ __attribute__((aligned(16))) char lds[S::kLdsBytes];
   const gs_tile::TileAt tile = gs_tile::tile_at(tiles_m, tiles_n);
   const int m0 = tile.m * S::BM, n0 = tile.n * S::BN;
@@ -458,7 +537,7 @@ __global__ __launch_bounds__(S::kThreads) void grad_kernel(Operand x, Operand ds
                                              kTableGrad ? counts : nullptr, lds);
   const int lane = threadIdx.x & 63;
   const int wm = gs_tile::wave_m<S>(), wn = gs_tile::wave_n<S>();
-  const float al = part ? 0.0f : *alpha;
+  const float al = part ? 0.0f : unit ? *alpha * *unit : *alpha;
 #pragma unroll
   for (int b = 0; b < S::kNB; ++b) {
     const int n = n0 + wn + 32 * b + (lane & 31);
@@ -484,12 +563,13 @@ __global__ __launch_bounds__(S::kThreads) void grad_kernel(Operand x, Operand ds
   }
 }
 
-// out = alpha * sum of the planes; counts (dh): rows that do not count are zero.
+// out = alpha (and x's unit) * sum of the planes; counts (dh): rows that do not count are zero.
 template <typename Out>
 __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ part, int planes, int64_t plane,
                                                      int64_t n, int D, const uint64_t* __restrict__ counts,
-                                                     const float* __restrict__ alpha, Out* __restrict__ out) {
-  const float al = *alpha;
+                                                     const float* __restrict__ alpha, const float* __restrict__ unit,
+                                                     Out* __restrict__ out) {
+  const float al = unit ? *alpha * *unit : *alpha;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     float s = 0.0f;
     for (int p = 0; p < planes; ++p) s += part[(int64_t)p * plane + i];
@@ -522,6 +602,8 @@ struct Problem {
   int64_t ld_table;
   int planes() const { return dtype == GS_FP32 ? gs_tile::kSplitPlanes : 1; }
   int products() const { return dtype == GS_FP32 ? gs_tile::kSplitProducts : 1; }
+  int ds_planes() const { return dtype == GS_FP32 ? gs_tile::kWidePlanes : 1; }
+  int ds_products() const { return dtype == GS_FP32 ? gs_tile::kWideProducts : 1; }
   int64_t dp() const { return round_up(dim, 8); }
   bool packs(int64_t ld) const { return dtype == GS_FP32 || dim % 8 || ld % 8 || ld > gs_tile::kMaxLd; }
   size_t element() const { return dtype == GS_FP32 ? 4 : 2; }
@@ -542,55 +624,96 @@ static int check_pointers(const Problem& p) {
   return GS_OK;
 }
 
-static void pack(const Problem& p, const void* src, int64_t ld, int64_t rows, uint16_t* dst, hipStream_t s) {
-  const int64_t vectors = rows * (p.dp() / 8);
-  if (vectors == 0) return;
-  const int blocks = (int)min(ceil_div(vectors, 256), (int64_t)16384);
-  const int64_t plane = rows * p.dp();
-  if (p.dtype == GS_FP32)
-    pack_kernel<<<blocks, 256, 0, s>>>((const float*)src, ld, rows, p.dim, (int)p.dp(), dst, plane);
-  else
-    pack_kernel<<<blocks, 256, 0, s>>>((const _Float16*)src, ld, rows, p.dim, (int)p.dp(), dst, plane);
+// Where a matrix's layout for the tile loads goes, if it needs one.
+struct Layout {
+  uint16_t* space;
+  float* unit;     // fp32
+  float* largest;  // fp32: kLargestBlocks
+  int largest_n;
+};
+
+// fp32: the magnitudes that the layout's unit comes from.
+static void measure(const Problem& p, const void* src, int64_t ld, int64_t rows, Targets targets, Layout& to,
+                    hipStream_t s) {
+  if (p.dtype != GS_FP32) return;
+  to.largest_n = (int)min(ceil_div(rows, 32), (int64_t)kLargestBlocks);
+  magnitude_kernel<<<to.largest_n, 256, 0, s>>>((const float*)src, ld, rows, p.dim, targets, to.largest);
 }
 
-// The operand of `rows` rows from row `first` of a matrix: in place, or packed into `space`.
-static Operand operand(const Problem& p, const void* src, int64_t ld, int64_t first, int64_t rows, uint16_t* space,
+// The operand of `rows` rows from row `first` of a matrix: in place, or laid out.
+static Operand operand(const Problem& p, const void* src, int64_t ld, int64_t first, int64_t rows, const Layout& to,
                        hipStream_t s) {
   const char* at = (const char*)src + first * ld * (int64_t)p.element();
   if (!p.packs(ld)) return {(const uint16_t*)at, ld, 0, (int32_t)rows};
-  pack(p, at, ld, rows, space, s);
-  return {space, p.dp(), rows * p.dp(), (int32_t)rows};
+  const int64_t plane = rows * p.dp();
+  const int blocks = (int)min(ceil_div(plane / 8, 256), (int64_t)8192);
+  if (p.dtype == GS_FP32)
+    pack_kernel<<<blocks, 256, 0, s>>>((const float*)at, ld, rows, p.dim, (int)p.dp(), to.space, plane, to.largest,
+                                       to.largest_n, to.unit);
+  else
+    pack_kernel<<<blocks, 256, 0, s>>>((const _Float16*)at, ld, rows, p.dim, (int)p.dp(), to.space, plane, nullptr, 0,
+                                       nullptr);
+  return {to.space, p.dp(), plane, (int32_t)rows};
 }
 
-// The logits' scale in base 2.  Zero becomes the least normal number: the same
-// flat distribution, and minus infinity (what lies past the vocabulary) stays that.
-static float base2_scale(float logit_scale) {
-  const float scale2 = logit_scale * kLog2e;
-  return scale2 == 0.0f ? 1.17549435e-38f : scale2;
+// Both matrices' layouts; units: the features' and the table's, side by side (fp32; else null).
+struct Layouts {
+  Layout features, table;
+  float* units;
+  Layouts() = default;
+  Layouts(const Problem& p, int64_t rows_piece, Carve& c) {
+    units = c.take<float>(p.dtype == GS_FP32 ? 2 : 0);
+    if (p.dtype != GS_FP32) units = nullptr;
+    features = {c.take<uint16_t>(p.packs(p.ld_features) ? rows_piece * p.dp() * p.planes() : 0), units,
+                c.take<float>(p.dtype == GS_FP32 ? kLargestBlocks : 0), 0};
+    table = {c.take<uint16_t>(p.packs(p.ld_table) ? p.vocab * p.dp() * p.planes() : 0), units ? units + 1 : nullptr,
+             c.take<float>(p.dtype == GS_FP32 ? kLargestBlocks : 0), 0};
+  }
+  void measure(const Problem& p, Targets targets, hipStream_t s) {
+    gs_xent::measure(p, p.features, p.ld_features, p.rows, targets, features, s);
+    gs_xent::measure(p, p.table, p.ld_table, p.vocab, {nullptr, 64, 0}, table, s);
+  }
+};
+
+// Big or Mid tiles for a product of M x N (parts: copies of it side by side):
+// the time of whole rounds of the chip's 256 CUs, one Big workgroup each or two
+// Mid ones, a Mid tile of a quarter of the work taking 1.15 times its share.
+static bool takes_big(int64_t M, int64_t N) {
+  const int64_t big = ceil_div(M, Big::BM) * ceil_div(N, Big::BN), mid = ceil_div(M, Mid::BM) * ceil_div(N, Mid::BN);
+  const int64_t mid_rounds = mid <= 256 ? 1 : 2 * ceil_div(mid, 512);
+  return 400 * ceil_div(big, 256) <= 115 * mid_rounds;
+}
+
+// Calls f with a value of the shape for the tiles of ds.
+template <bool kBig, class F>
+static void with_logits_shape(int64_t vocab, int64_t rows, F f) {
+  if constexpr (kBig)
+    if (takes_big(vocab, rows)) return f(Big{});
+  f(Mid{});
 }
 
 struct ForwardPlan {
+  enum { kThin32, kThin64, kMid, kBig } shape;
   int64_t rows_piece, tiles_m, blocks;
   int lanes;
-  uint16_t *table, *features;
+  Layouts layouts;
   float2* stats;
   float* label;
   Sum* partial;
   size_t bytes;
 
   ForwardPlan(const Problem& p, void* ws) {
-    tiles_m = ceil_div(p.vocab, Tile::BM);
-    rows_piece = kStatBytes / (tiles_m * (int64_t)sizeof(float2)) / Tile::BN * Tile::BN;
-    if (rows_piece < Tile::BN) rows_piece = Tile::BN;
-    if (rows_piece > (1 << 20)) rows_piece = 1 << 20;
-    if (rows_piece > p.rows) rows_piece = p.rows;
+    shape = p.rows <= 32 ? kThin32 : p.rows <= 64 ? kThin64 : takes_big(p.vocab, p.rows) ? kBig : kMid;
+    const int bm = shape == kBig ? Big::BM : shape == kMid ? Mid::BM : Thin32::BM;
+    tiles_m = ceil_div(p.vocab, bm);
+    rows_piece = max((int64_t)256, kStatBytes / (tiles_m * (int64_t)sizeof(float2)) / 256 * 256);
+    rows_piece = min(p.rows, min(rows_piece, (int64_t)1 << 20));
     lanes = p.rows <= 4096 ? 64 : 1;
     blocks = 0;
     for (int64_t r = 0; r < p.rows; r += rows_piece)
       blocks += ceil_div(min(rows_piece, p.rows - r), kJoinThreads / lanes);
     Carve c{(char*)ws};
-    table = c.take<uint16_t>(p.packs(p.ld_table) ? p.vocab * p.dp() * p.planes() : 0);
-    features = c.take<uint16_t>(p.packs(p.ld_features) ? rows_piece * p.dp() * p.planes() : 0);
+    layouts = Layouts(p, rows_piece, c);
     stats = c.take<float2>(tiles_m * rows_piece);
     label = c.take<float>(rows_piece);
     partial = c.take<Sum>(blocks);
@@ -598,32 +721,36 @@ struct ForwardPlan {
   }
 };
 
-template <typename T>
+template <class S, typename T>
 static void launch_logits_fwd(const Problem& p, const ForwardPlan& f, const Operand& table, const Operand& features,
                               float scale2, Targets targets, hipStream_t s) {
-  const int64_t tiles = f.tiles_m * ceil_div(features.extent, Tile::BN);
-  logits_fwd_kernel<Tile, T><<<(unsigned)tiles, Tile::kThreads, 0, s>>>(
-      table, features, (int)p.dp(), p.products(), fabsf(scale2), scale2 < 0.0f, targets, (int)f.tiles_m, (int)ceil_div(features.extent, Tile::BN), f.stats, f.label);
+  const int64_t tiles_n = ceil_div(features.extent, S::BN);
+  logits_fwd_kernel<S, T><<<(unsigned)(f.tiles_m * tiles_n), S::kThreads, 0, s>>>(
+      table, features, (int)p.dp(), p.products(), scale2, f.layouts.units, targets, (int)f.tiles_m, (int)tiles_n,
+      f.stats, f.label);
 }
 
+template <typename T>
 static int forward(const Problem& p, Targets targets, float logit_scale, int reduction, float* loss, float2* norm,
-                   int64_t* count, const ForwardPlan& f, hipStream_t s) {
-  if (p.rows == 0) {
-    total_kernel<<<1, kJoinThreads, 0, s>>>(nullptr, 0, reduction, loss, count);
-    return gs_status_from_hip(hipGetLastError());
-  }
-  const float scale2 = base2_scale(logit_scale);
-  const Operand table = operand(p, p.table, p.ld_table, 0, p.vocab, f.table, s);
+                   int64_t* count, ForwardPlan& f, hipStream_t s) {
+  const float scale2 = logit_scale * kLog2e;
+  f.layouts.measure(p, targets, s);
+  const Operand table = operand(p, p.table, p.ld_table, 0, p.vocab, f.layouts.table, s);
   int64_t block = 0;
   for (int64_t r = 0; r < p.rows; r += f.rows_piece) {
     const int64_t rows = min(f.rows_piece, p.rows - r);
-    const Operand features = operand(p, p.features, p.ld_features, r, rows, f.features, s);
-    if (p.dtype == GS_FP16) launch_logits_fwd<_Float16>(p, f, table, features, scale2, targets.from(r), s);
-    else launch_logits_fwd<__bf16>(p, f, table, features, scale2, targets.from(r), s);
+    const Operand features = operand(p, p.features, p.ld_features, r, rows, f.layouts.features, s);
+    const Targets t = targets.from(r);
+    switch (f.shape) {
+      case ForwardPlan::kThin32: launch_logits_fwd<Thin32, T>(p, f, table, features, scale2, t, s); break;
+      case ForwardPlan::kThin64: launch_logits_fwd<Thin64, T>(p, f, table, features, scale2, t, s); break;
+      case ForwardPlan::kMid: launch_logits_fwd<Mid, T>(p, f, table, features, scale2, t, s); break;
+      case ForwardPlan::kBig: launch_logits_fwd<Big, T>(p, f, table, features, scale2, t, s); break;
+    }
     const int64_t blocks = ceil_div(rows, kJoinThreads / f.lanes);
     auto* join = f.lanes == 64 ? join_kernel<64> : join_kernel<1>;
-    join<<<(unsigned)blocks, kJoinThreads, 0, s>>>(f.stats, f.label, (int)rows, (int)f.tiles_m, p.vocab, fabsf(scale2),
-                                                   targets.from(r), reduction, norm ? norm + r : nullptr,
+    join<<<(unsigned)blocks, kJoinThreads, 0, s>>>(f.stats, f.label, (int)rows, (int)f.tiles_m, p.vocab, scale2,
+                                                   f.layouts.units, t, reduction, norm ? norm + r : nullptr,
                                                    reduction == GS_REDUCE_NONE ? loss + r : nullptr,
                                                    f.partial + block, f.blocks == 1, loss, count);
     block += blocks;
@@ -632,11 +759,31 @@ static int forward(const Problem& p, Targets targets, float logit_scale, int red
   return gs_status_from_hip(hipGetLastError());
 }
 
+// The shape of a gradient's tiles, D columns of m: 64 wide where D fits, else 256
+// unless 128 leaves so much less of the last tile empty that its smaller reuse pays.
+enum class Columns { kNarrow, kMid, kBig };
+static Columns columns_of(int64_t D) {
+  if (D <= Narrow::BM) return Columns::kNarrow;
+  return round_up(D, Big::BM) * 100 <= round_up(D, Mid::BM) * 115 ? Columns::kBig : Columns::kMid;
+}
+
+template <class F>
+static void with_columns(Columns c, F f) {
+  if (c == Columns::kNarrow) f(Narrow{});
+  else if (c == Columns::kMid) f(Mid{});
+  else f(Big{});
+}
+
 // How many parts a gradient's product of (N x D) over K is cut into along K, so
-// that the launch fills the chip; a part has at least four steps.
+// that the launch fills the chip (512 workgroups where two share a CU); a part has at least four steps.
 static int parts_for(int64_t N, int64_t D, int64_t K) {
-  const int64_t tiles = ceil_div(N, Tile::BN) * ceil_div(D, Tile::BM);
-  const int64_t want = tiles >= 384 ? 1 : ceil_div(512, tiles);
+  int64_t want = 1;
+  with_columns(columns_of(D), [&](auto shape) {
+    typedef decltype(shape) S;
+    const int64_t tiles = ceil_div(N, S::BN) * ceil_div(D, S::BM);
+    const int64_t fill = 2 * S::kLdsBytes <= 160 * 1024 ? 512 : 256;
+    want = tiles * 4 >= fill * 3 ? 1 : ceil_div(fill, tiles);
+  });
   return (int)max((int64_t)1, min(want, K / (4 * kBK)));
 }
 
@@ -644,17 +791,24 @@ struct BackwardPlan {
   int64_t rows_piece, cols_piece, ld, row_pieces, col_pieces;
   int parts_h, parts_t;  // parts along K of dh and dw
   bool direct_h, direct_t;  // one part and one piece: no fp32 sums in between
-  uint16_t *table, *features, *ds;
+  Layouts layouts;
+  uint16_t* ds;
   float *factor, *alpha, *largest, *part_h, *part_t;
   uint64_t* counts;
   size_t bytes;
 
   BackwardPlan(const Problem& p, bool want_h, bool want_t, void* ws) {
-    const int64_t row_bytes = 2 * p.planes() * round_up(p.vocab, Tile::BM);
-    rows_piece = min(p.rows, max(kRowsPiece, kPieceBytes / row_bytes / kRowsPiece * kRowsPiece));
-    cols_piece = max((int64_t)Tile::BM, kPieceBytes / (rows_piece * 2 * p.planes()) / Tile::BM * Tile::BM);
-    if (cols_piece > p.vocab) cols_piece = p.vocab;
-    ld = round_up(cols_piece, Tile::BM);
+    // The piece: a part of the longer side against (if it fits) the whole of the
+    // shorter, whose gradient's sums then wait from piece to piece; that one is the smaller.
+    const int64_t most = kPieceBytes / (2 * p.ds_planes());  // elements of ds
+    if (p.rows > p.vocab) {
+      cols_piece = min((int64_t)p.vocab, most / kLeastSide / 256 * 256);
+      rows_piece = min(p.rows, most / round_up(cols_piece, 256) / 256 * 256);
+    } else {
+      rows_piece = min(p.rows, most / kLeastSide / 256 * 256);
+      cols_piece = min((int64_t)p.vocab, most / rows_piece / 256 * 256);
+    }
+    ld = round_up(cols_piece, 256);
     row_pieces = ceil_div(p.rows, rows_piece);
     col_pieces = ceil_div(p.vocab, cols_piece);
     parts_h = want_h ? parts_for(rows_piece, p.dim, cols_piece) : 1;
@@ -662,9 +816,8 @@ struct BackwardPlan {
     direct_h = parts_h == 1 && col_pieces == 1;
     direct_t = parts_t == 1 && row_pieces == 1;
     Carve c{(char*)ws};
-    table = c.take<uint16_t>(p.packs(p.ld_table) ? p.vocab * p.dp() * p.planes() : 0);
-    features = c.take<uint16_t>(p.packs(p.ld_features) ? rows_piece * p.dp() * p.planes() : 0);
-    ds = c.take<uint16_t>(rows_piece * ld * p.planes());
+    layouts = Layouts(p, rows_piece, c);
+    ds = c.take<uint16_t>(rows_piece * ld * p.ds_planes());
     factor = c.take<float>(p.rows);
     counts = c.take<uint64_t>(ceil_div(p.rows, 64));
     alpha = c.take<float>(1);
@@ -680,8 +833,8 @@ static unsigned finish_blocks(int64_t n) { return (unsigned)min(ceil_div(n, 256)
 template <typename T, typename Out, int kPlanes>
 static int backward(const Problem& p, Targets targets, float logit_scale, int reduction, const float2* norm,
                     const int64_t* count, const float* grad_loss, Out* grad_features, Out* grad_table,
-                    const BackwardPlan& b, hipStream_t s) {
-  const float scale2 = base2_scale(logit_scale);
+                    BackwardPlan& b, hipStream_t s) {
+  const float scale2 = logit_scale * kLog2e;
   const int D = p.dim;
   int largest_n = 0;
   if (reduction == GS_REDUCE_NONE) {
@@ -691,11 +844,12 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
   factors_kernel<<<(unsigned)ceil_div(p.rows, 256), 256, 0, s>>>(grad_loss, p.rows, p.vocab, targets, reduction, count,
                                                                  logit_scale, Held<T>::kScale, b.largest, largest_n,
                                                                  b.factor, b.counts, b.alpha);
-  const Operand table = operand(p, p.table, p.ld_table, 0, p.vocab, b.table, s);
-  const int tiles_d = (int)ceil_div(D, Tile::BM);
+  b.layouts.measure(p, targets, s);
+  const float *unit_h = b.layouts.features.unit, *unit_w = b.layouts.table.unit;
+  const Operand table = operand(p, p.table, p.ld_table, 0, p.vocab, b.layouts.table, s);
   for (int64_t r = 0; r < p.rows; r += b.rows_piece) {
-    const int64_t rows = min(b.rows_piece, p.rows - r);
-    const Operand features = operand(p, p.features, p.ld_features, r, rows, b.features, s);
+    const int32_t rows = (int32_t)min(b.rows_piece, p.rows - r);
+    const Operand features = operand(p, p.features, p.ld_features, r, rows, b.layouts.features, s);
     const uint64_t* counts = b.counts + r / 64;
     const int64_t ds_plane = rows * b.ld;
     for (int64_t c = 0; c < p.vocab; c += b.cols_piece) {
@@ -703,42 +857,53 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
       Operand piece = table;  // the piece's rows of the table
       piece.p += c * table.ld;
       piece.extent = cols;
-      const int tiles_v = (int)ceil_div(cols, Tile::BM);
-      logits_bwd_kernel<Tile, T, kPlanes><<<(unsigned)(tiles_v * ceil_div(rows, Tile::BN)), Tile::kThreads, 0, s>>>(
-          piece, features, (int)p.dp(), p.products(), scale2, targets.from(r), c, tiles_v, (int)ceil_div(rows, Tile::BN), norm + r, b.factor + r,
-          counts, b.ds, b.ld, ds_plane);
-      if (grad_features) {
-        const Operand ds = {b.ds, b.ld, ds_plane, (int32_t)rows};
-        Operand x = piece;  // D columns of the piece's rows
-        x.extent = D;
-        const int32_t k_part = (int32_t)round_up(ceil_div(cols, b.parts_h), kBK);
-        grad_kernel<Tile, T, Out, false><<<dim3((unsigned)(tiles_d * ceil_div(rows, Tile::BN)), b.parts_h),
-                                           Tile::kThreads, 0, s>>>(
-            x, ds, cols, k_part, p.products(), counts, tiles_d, (int)ceil_div(rows, Tile::BN), b.direct_h ? nullptr : b.part_h, rows * D, c > 0,
-            b.alpha, grad_features + r * D);
-      }
-      if (grad_table) {
-        const Operand ds = {b.ds, b.ld, ds_plane, cols};
-        Operand x = features;
-        x.extent = D;
-        const int32_t k_part = (int32_t)round_up(ceil_div(rows, b.parts_t), kBK);
-        float* part = b.direct_t ? nullptr : b.part_t + (b.row_pieces > 1 ? c * D : 0);
-        const int64_t part_plane = (b.row_pieces > 1 ? (int64_t)p.vocab : cols) * D;
-        grad_kernel<Tile, T, Out, true><<<dim3((unsigned)(tiles_d * ceil_div(cols, Tile::BN)), b.parts_t),
-                                          Tile::kThreads, 0, s>>>(
-            x, ds, (int32_t)rows, k_part, p.products(), counts, tiles_d, (int)ceil_div(cols, Tile::BN), part, part_plane, r > 0, b.alpha, grad_table + c * D);
-        if (part && b.row_pieces == 1)
-          finish_kernel<<<finish_blocks((int64_t)cols * D), 256, 0, s>>>(part, b.parts_t, part_plane, (int64_t)cols * D,
-                                                                        D, nullptr, b.alpha, grad_table + c * D);
-      }
+      // fp32 always in Mid tiles: the planes of a Big one's ds do not fit its registers
+      with_logits_shape<kPlanes == 1>(cols, rows, [&](auto shape) {
+        typedef decltype(shape) S;
+        const int tiles_m = (int)ceil_div(cols, S::BM), tiles_n = (int)ceil_div(rows, S::BN);
+        logits_bwd_kernel<S, T, kPlanes><<<(unsigned)((int64_t)tiles_m * tiles_n), S::kThreads, 0, s>>>(
+            piece, features, (int)p.dp(), p.products(), scale2, b.layouts.units, targets.from(r), c, tiles_m, tiles_n,
+            norm + r, b.factor + r, counts, b.ds, b.ld, ds_plane);
+      });
+      with_columns(columns_of(D), [&](auto shape) {
+        typedef decltype(shape) S;
+        const int tiles_m = (int)ceil_div(D, S::BM);
+        if (grad_features) {
+          const Operand ds = {b.ds, b.ld, ds_plane, rows};
+          Operand x = piece;  // D columns of the piece's rows
+          x.extent = D;
+          const int tiles_n = (int)ceil_div(rows, S::BN);
+          const int32_t k_part = (int32_t)round_up(ceil_div(cols, b.parts_h), kBK);
+          grad_kernel<S, T, Out, false><<<dim3((unsigned)((int64_t)tiles_m * tiles_n), b.parts_h), S::kThreads, 0, s>>>(
+              x, ds, cols, k_part, p.ds_products(), counts, tiles_m, tiles_n, b.direct_h ? nullptr : b.part_h,
+              (int64_t)rows * D, c > 0, b.alpha, unit_w, grad_features + r * D);
+        }
+        if (grad_table) {
+          const Operand ds = {b.ds, b.ld, ds_plane, cols};
+          Operand x = features;
+          x.extent = D;
+          const int tiles_n = (int)ceil_div(cols, S::BN);
+          const int32_t k_part = (int32_t)round_up(ceil_div(rows, b.parts_t), kBK);
+          float* part = b.direct_t ? nullptr : b.part_t + (b.row_pieces > 1 ? c * D : 0);
+          const int64_t part_plane = (b.row_pieces > 1 ? (int64_t)p.vocab : cols) * D;
+          grad_kernel<S, T, Out, true><<<dim3((unsigned)((int64_t)tiles_m * tiles_n), b.parts_t), S::kThreads, 0, s>>>(
+              x, ds, rows, k_part, p.ds_products(), counts, tiles_m, tiles_n, part, part_plane, r > 0, b.alpha, unit_h,
+              grad_table + c * D);
+          if (part && b.row_pieces == 1)
+            finish_kernel<<<finish_blocks((int64_t)cols * D), 256, 0, s>>>(
+                part, b.parts_t, part_plane, (int64_t)cols * D, D, nullptr, b.alpha, unit_h, grad_table + c * D);
+        }
+      });
     }
     if (grad_features && !b.direct_h)
-      finish_kernel<<<finish_blocks(rows * D), 256, 0, s>>>(b.part_h, b.parts_h, rows * D, rows * D, D, counts, b.alpha,
-                                                            grad_features + r * D);
+      finish_kernel<<<finish_blocks((int64_t)rows * D), 256, 0, s>>>(b.part_h, b.parts_h, (int64_t)rows * D,
+                                                                    (int64_t)rows * D, D, counts, b.alpha, unit_w,
+                                                                    grad_features + r * D);
   }
   if (grad_table && b.row_pieces > 1)
     finish_kernel<<<finish_blocks((int64_t)p.vocab * D), 256, 0, s>>>(b.part_t, b.parts_t, (int64_t)p.vocab * D,
-                                                                     (int64_t)p.vocab * D, D, nullptr, b.alpha, grad_table);
+                                                                     (int64_t)p.vocab * D, D, nullptr, b.alpha, unit_h,
+                                                                     grad_table);
   return gs_status_from_hip(hipGetLastError());
 }
 
@@ -776,10 +941,15 @@ extern "C" int gs_xent_fwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dty
   if ((status = gs_xent::check_pointers(p)) != GS_OK) return status;
   if (rows > 0 && ((uintptr_t)workspace & 255)) return GS_ERR_MISALIGNED;
   if (rows > 0 && (!workspace || workspace_bytes < gs_xent::ForwardPlan(p, nullptr).bytes)) return GS_ERR_SCRATCH_TOO_SMALL;
-  if (rows == 0) workspace = nullptr;
-  const gs_xent::ForwardPlan f(p, workspace);
-  return gs_xent::forward(p, {targets, target_bits, ignore_index}, logit_scale, reduction, loss, (float2*)norm, count, f,
-                          (hipStream_t)stream);
+  hipStream_t s = (hipStream_t)stream;
+  if (rows == 0) {
+    gs_xent::total_kernel<<<1, gs_xent::kJoinThreads, 0, s>>>(nullptr, 0, reduction, loss, count);
+    return gs_status_from_hip(hipGetLastError());
+  }
+  gs_xent::ForwardPlan f(p, workspace);
+  const gs_xent::Targets t = {targets, target_bits, ignore_index};
+  auto* run = dtype == GS_BF16 ? gs_xent::forward<__bf16> : gs_xent::forward<_Float16>;  // fp32: planes of fp16
+  return run(p, t, logit_scale, reduction, loss, (float2*)norm, count, f, s);
 }
 
 extern "C" size_t gs_xent_bwd_workspace_bytes(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype,
@@ -814,10 +984,10 @@ extern "C" int gs_xent_bwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dty
   const bool want_h = grad_features != nullptr, want_t = grad_table != nullptr;
   if (!workspace || workspace_bytes < gs_xent::BackwardPlan(p, want_h, want_t, nullptr).bytes)
     return GS_ERR_SCRATCH_TOO_SMALL;
-  const gs_xent::BackwardPlan b(p, want_h, want_t, workspace);
+  gs_xent::BackwardPlan b(p, want_h, want_t, workspace);
   const gs_xent::Targets t = {targets, target_bits, ignore_index};
   if (dtype == GS_FP32)
-    return gs_xent::backward<__bf16, float, 3>(p, t, logit_scale, reduction, (const float2*)norm, count, grad_loss,
+    return gs_xent::backward<_Float16, float, gs_tile::kWidePlanes>(p, t, logit_scale, reduction, (const float2*)norm, count, grad_loss,
                                                (float*)grad_features, (float*)grad_table, b, s);
   if (dtype == GS_BF16)
     return gs_xent::backward<__bf16, __bf16, 1>(p, t, logit_scale, reduction, (const float2*)norm, count, grad_loss,
