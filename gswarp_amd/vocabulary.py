@@ -19,6 +19,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib, _workspace
+from ._pipeline import _device_guard, _stream
 
 _DTYPES = {torch.float32: _lib.GS_FP32, torch.bfloat16: _lib.GS_BF16, torch.float16: _lib.GS_FP16}
 _INDEX_BITS = {torch.int32: 32, torch.int64: 64}
@@ -28,14 +29,17 @@ _MAX_DIM = 2**21 - 8
 
 
 def _check_table(table, name: str) -> None:
+    if isinstance(table, torch.Tensor) and table.is_cuda and table.dtype in _DTYPES and table.ndim == 2:
+        vocab, dim = table.shape
+        if 0 < vocab <= _INT32_MAX and 0 < dim <= _MAX_DIM:
+            return
     if not isinstance(table, torch.Tensor) or not table.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     if table.dtype not in _DTYPES:
         raise ValueError(f"{name} must have dtype float32, bfloat16 or float16, got {table.dtype}")
     if table.ndim != 2 or table.shape[0] == 0 or table.shape[1] == 0:
         raise ValueError(f"{name} must have shape (vocabulary, dim), got {tuple(table.shape)}")
-    if table.shape[0] > _INT32_MAX or table.shape[1] > _MAX_DIM:
-        raise ValueError(f"{name} must have at most 2**31 - 1 rows of at most 2**21 - 8 values")
+    raise ValueError(f"{name} must have at most 2**31 - 1 rows of at most 2**21 - 8 values")
 
 
 def _check_indices(indices, name: str, device: torch.device) -> None:
@@ -58,17 +62,18 @@ def _check_factor(value, name: str) -> float:
 
 def _rows(t: torch.Tensor, alignment: int = 1) -> torch.Tensor:
     """The matrix, or a copy of it, with contiguous rows that do not overlap, on `alignment` bytes."""
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    if t.is_contiguous():
+        if t.data_ptr() % alignment == 0:
+            return t
+    elif (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
         t = t.contiguous()
     return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % alignment else t
 
 
 def _row_stride(t: torch.Tensor) -> int:
+    if t.is_contiguous():
+        return t.shape[1]
     return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
-
-
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
 
 
 def _workspace_of(nbytes: int, device: torch.device) -> torch.Tensor:
@@ -82,14 +87,13 @@ def _aligned(space: torch.Tensor) -> int:
 # ---------------------------------------------------------------- lookup
 
 def _embed_forward(tokens, table, scale):
-    device = table.device
+    device, (vocab, dim) = table.device, table.shape
     lib = _lib.load()
     tokens, rows = tokens.contiguous(), _rows(table)
-    out = torch.empty((*tokens.shape, table.shape[1]), dtype=table.dtype, device=device)
-    with torch.cuda.device(device), _workspace.device_lock(device):
-        lib.call("gs_embed_fwd", tokens.numel(), table.shape[0], table.shape[1], _DTYPES[table.dtype],
-                 tokens.data_ptr(), _INDEX_BITS[tokens.dtype], rows.data_ptr(), _row_stride(rows), scale,
-                 out.data_ptr(), _stream(device))
+    out = torch.empty((*tokens.shape, dim), dtype=table.dtype, device=device)
+    with _device_guard(device), _workspace.device_lock(device):
+        lib.call("gs_embed_fwd", tokens.numel(), vocab, dim, _DTYPES[table.dtype], tokens.data_ptr(),
+                 _INDEX_BITS[tokens.dtype], rows.data_ptr(), _row_stride(rows), scale, out.data_ptr(), _stream(device))
     return out
 
 
@@ -110,7 +114,7 @@ class EmbedTokens(torch.autograd.Function):
         tokens, grad_out = tokens.contiguous(), grad_out.contiguous()
         grad = torch.empty((vocab, dim), dtype=dtype, device=device)
         n, code = tokens.numel(), _DTYPES[dtype]
-        with torch.cuda.device(device), _workspace.device_lock(device):
+        with _device_guard(device), _workspace.device_lock(device):
             nbytes = lib.gs_embed_bwd_workspace_bytes(n, vocab, dim, code)
             space = _workspace_of(nbytes, device)
             lib.call("gs_embed_bwd", n, vocab, dim, code, tokens.data_ptr(), _INDEX_BITS[tokens.dtype],
@@ -147,7 +151,7 @@ def _entropy_forward(features, table, targets, ignore_index, reduction, logit_sc
     code, reduce = _DTYPES[table.dtype], _REDUCTIONS[reduction]
     loss = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=device)
     norm = torch.empty((n, 2), dtype=torch.float32, device=device) if keep else None
-    with torch.cuda.device(device), _workspace.device_lock(device):
+    with _device_guard(device), _workspace.device_lock(device):
         nbytes = lib.gs_xent_fwd_workspace_bytes(n, vocab, dim, code, _row_stride(features), _row_stride(table))
         # the count of rows sits in front of the workspace
         space = _workspace_of(nbytes + 256 if not keep else nbytes, device)
@@ -181,7 +185,7 @@ class LinearCrossEntropy(torch.autograd.Function):
         ldf, ldt = _row_stride(features), _row_stride(table)
         grad_features = torch.empty((n, dim), dtype=table.dtype, device=device) if want_features else None
         grad_table = torch.empty((vocab, dim), dtype=table.dtype, device=device) if want_table else None
-        with torch.cuda.device(device), _workspace.device_lock(device):
+        with _device_guard(device), _workspace.device_lock(device):
             nbytes = lib.gs_xent_bwd_workspace_bytes(n, vocab, dim, code, ldf, ldt, want_features, want_table)
             space = _workspace_of(nbytes, device)
             lib.call("gs_xent_bwd", n, vocab, dim, code, features.data_ptr(), ldf, table.data_ptr(), ldt,
