@@ -93,9 +93,10 @@ struct Pack<_Float16> {
 //
 // LDS layouts (bytes), 16-byte chunks permuted so that no read of a wave meets a
 // bank twice:
-//   K contiguous: row i at i * 128, its chunk c at (c ^ ((i >> 1) & 7)) * 16:
-//     the 16 rows that one phase of a 16-byte read takes lie in 16 different
-//     chunks of the 256 bytes of the banks;
+//   K contiguous: row i at i * 128, its chunk c at (c ^ spread(i)) * 16: the 16
+//     rows that one phase of a 16-byte read takes lie in 16 different chunks of
+//     the 256 bytes of the banks, and so do four rows of 64 bytes, which a
+//     transposing read takes;
 //   K rows: K row k at k * 2 BT, its 32-byte chunk c at (c ^ turn(k)) * 32: the
 //     four K rows that the transposing load takes per 16 lanes lie apart.
 template <bool kAlongK, int BT, int kWaves>
@@ -106,6 +107,7 @@ struct Stage {
   static constexpr int kLoadRows = 64 / kRowVectors;            // rows of the layout that an instruction fills
   static_assert(kLoads * kWaves * 1024 == kBytes, "every wave issues the same loads");
 
+  static __device__ __forceinline__ int spread(int i) { return ((i >> 2) & 3) | ((i << 1) & 4); }
   static __device__ __forceinline__ int turn(int k) { return BT >= 128 ? 2 * (k & 3) : 2 * ((k >> 1) & 1); }
 
   // Byte offsets of the lane's chunk from the step's first element, for
@@ -119,7 +121,7 @@ struct Stage {
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
       const int r = p * kLoadRows + row;
-      if (kAlongK) chunk[p] = at ^ ((r >> 1) & 7);
+      if (kAlongK) chunk[p] = at ^ spread(r);
       else chunk[p] = (((at >> 1) ^ turn(r)) << 1) | (at & 1);
       offset[p] = (uint32_t)row * (uint32_t)o.ld * 2u + chunk[p] * 16u;
       if (!kAlongK && i0 + chunk[p] * 8 >= o.extent) offset[p] = kOutOfRange;
@@ -128,7 +130,7 @@ struct Stage {
 
   // Starts the loads of the K step at k0 of plane `plane` into lds; K and the
   // operand's extent bound what is read, and everything outside is zero.
-  // row_mask (K rows only): K row k0 + k counts as zero where bit k is clear.
+  // row_mask: row r of the layout (of the tile, or K row k0 + r) counts as zero where bit r is clear.
   __device__ __forceinline__ void load(const Operand& o, int plane, int i0, int32_t k0, int32_t K, uint64_t row_mask,
                                        char* __restrict__ lds) const {
     typedef __attribute__((address_space(3))) void lds_void;
@@ -154,12 +156,29 @@ struct Stage {
     for (int j = 0; j < kLoads; ++j) {
       const int number = wave * kLoads + j;
       uint32_t at = off[number & 1] + (uint32_t)(number * kLoadRows) * ld2;
-      if (!kAlongK && row_mask != ~0ull) {
+      if (row_mask != ~0ull) {
         const int k = number * kLoadRows + (threadIdx.x & 63) / kRowVectors;
         if (!((row_mask >> k) & 1)) at = kOutOfRange;
       }
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(lds + number * 1024), 16, at, 0, 0, 0);
     }
+  }
+
+  // The other way round (K contiguous, BT rows x 64 columns): operand of 32
+  // columns from i and the 16 rows from r0 as K, in their order, or (kHalves) as
+  // accumulators hold them: rows 0-3 and 8-11 in the lower half of the wave, 4-7 and 12-15 in the upper.
+  template <typename T, bool kHalves>
+  static __device__ __forceinline__ typename Pack<T>::v8 across(const char* __restrict__ lds, int i, int r0) {
+    const int lane = threadIdx.x & 63;
+    const int j = lane & 15, group = lane >> 4;
+    const int c = i + 16 * (group & 1) + 4 * (j & 3);
+    const int lo_row = r0 + (kHalves ? 4 : 8) * (group >> 1) + (j >> 2), hi_row = lo_row + (kHalves ? 8 : 4);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_s16x4*)(lds + lo_row * 128 + (((c >> 3) ^ spread(lo_row)) << 4) + (c & 4) * 2));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_s16x4*)(lds + hi_row * 128 + (((c >> 3) ^ spread(hi_row)) << 4) + (c & 4) * 2));
+    const s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(typename Pack<T>::v8, both);
   }
 
   // Matrix-core operand of 32 rows from i (a multiple of 32) and K columns
@@ -170,7 +189,7 @@ struct Stage {
     if (kAlongK) {
       const int row = i + (lane & 31);
       const int c = 2 * ks + (lane >> 5);
-      return *reinterpret_cast<const typename Pack<T>::v8*>(lds + row * 128 + ((c ^ ((row >> 1) & 7)) << 4));
+      return *reinterpret_cast<const typename Pack<T>::v8*>(lds + row * 128 + ((c ^ spread(row)) << 4));
     } else {
       // The transposing load: in each group of 16 lanes, lane j gives the
       // address of 4 values of K row j / 4 and gets the 4 K rows of column j.

@@ -1,0 +1,40 @@
+// What the cross entropy's kernels share: the targets, the logits' scale, and
+// what the backward keeps of a row.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace gs_xent {
+
+struct Targets {
+  const void* p;
+  int bits;
+  int64_t ignore;
+  __device__ __forceinline__ int64_t at(int64_t i) const {
+    return bits == 64 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
+  }
+  __host__ __device__ Targets from(int64_t row) const {
+    return {(const char*)p + row * (bits / 8), bits, ignore};
+  }
+};
+
+// What the dot products of laid-out rows are multiplied by for base-2 logits:
+// scale2 times the operands' units (fp32; else null), kept a normal number so
+// that minus infinity (what lies past the vocabulary) stays that under a scale
+// that underflows, or is zero: the same flat distribution.
+__device__ __forceinline__ float scale_of(float scale2, const float* units) {
+  if (units) scale2 = scale2 * units[0] * units[1];
+  return copysignf(fmaxf(fabsf(scale2), 1.17549435e-38f), scale2);
+}
+
+// What the backward needs of a row, f the factor of its loss's gradient (held
+// scale included): ds = share 2^(s log2 e - top) for every column but the label's, label there.
+struct __attribute__((aligned(16))) RowInfo {
+  float top;    // max s log2 e
+  float share;  // f / sum
+  float label;  // f (p_t - 1), from the label's logit in fp32
+  int target;   // -1: none in the vocabulary, or the row does not count
+};
+
+}  // namespace gs_xent

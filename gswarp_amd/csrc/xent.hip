@@ -13,7 +13,9 @@
 // piece into its parts of the gradients.  Nothing of rows x vocabulary exists
 // beyond one piece.
 #include "gs_capi.h"
+#include "gs_resident.h"
 #include "gs_tile.h"
+#include "gs_xent.h"
 
 #include <type_traits>
 
@@ -55,38 +57,41 @@ struct Held<_Float16> {
   static constexpr float kScale = 32768.0f;
 };
 
-struct Targets {
-  const void* p;
-  int bits;
-  int64_t ignore;
-  __device__ __forceinline__ int64_t at(int64_t i) const {
-    return bits == 64 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
-  }
-  __host__ __device__ Targets from(int64_t row) const {
-    return {(const char*)p + row * (bits / 8), bits, ignore};
-  }
-};
-
 // ------------------------------------------------------------------ packing
 // fp32: the largest finite magnitude of a matrix, one value a block (targets.p:
-// of the rows that count only, so that what ignored rows hold does not reach the unit of the others).
+// of the rows that count only, so that what ignored rows hold does not reach the
+// unit of the others).  flat: the rows are contiguous, 16-byte aligned and a multiple of 4 long in all.
 constexpr int kLargestBlocks = 1024;
 __global__ __launch_bounds__(256) void magnitude_kernel(const float* __restrict__ src, int64_t ld, int64_t rows,
-                                                        int dim, Targets targets, float* __restrict__ largest) {
+                                                        int dim, bool flat, Targets targets,
+                                                        float* __restrict__ largest) {
   __shared__ float lds[4];
   const int lane = threadIdx.x & 63;
-  const int64_t waves = (int64_t)gridDim.x * 4;
   float top = 0.0f;
-  constexpr int kRows = 8;  // rows in flight
-  for (int64_t r0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * kRows; r0 < rows; r0 += waves * kRows) {
-    for (int c = lane; c < dim; c += 64) {
-      float v[kRows];
+  auto see = [&](float v, int64_t row) {
+    if (v < INFINITY && v > top && (!targets.p || targets.at(row) != targets.ignore)) top = v;
+  };
+  if (flat) {
+    const int64_t n = rows * dim / 4, stride = (int64_t)gridDim.x * 256;
+    constexpr int kItems = 4;  // vectors in flight
+    for (int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x; i0 < n; i0 += stride * kItems) {
+      float4 v[kItems];
 #pragma unroll
-      for (int j = 0; j < kRows; ++j) v[j] = r0 + j < rows ? fabsf(src[(r0 + j) * ld + c]) : 0.0f;
+      for (int j = 0; j < kItems; ++j)
+        v[j] = i0 + j * stride < n ? reinterpret_cast<const float4*>(src)[i0 + j * stride] : make_float4(0, 0, 0, 0);
 #pragma unroll
-      for (int j = 0; j < kRows; ++j)
-        if (v[j] < INFINITY && v[j] > top && (!targets.p || targets.at(r0 + j) != targets.ignore)) top = v[j];
+      for (int j = 0; j < kItems; ++j) {
+        const float x[4] = {fabsf(v[j].x), fabsf(v[j].y), fabsf(v[j].z), fabsf(v[j].w)};
+        // few vectors hold a new maximum, so few look their rows up
+        if (x[0] > top || x[1] > top || x[2] > top || x[3] > top)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) see(x[e], ((i0 + j * stride) * 4 + e) / dim);
+      }
     }
+  } else {
+    const int64_t waves = (int64_t)gridDim.x * 4;
+    for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += waves)
+      for (int c = lane; c < dim; c += 64) see(fabsf(src[row * ld + c]), row);
   }
 #pragma unroll
   for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
@@ -95,38 +100,33 @@ __global__ __launch_bounds__(256) void magnitude_kernel(const float* __restrict_
   if (threadIdx.x == 0) largest[blockIdx.x] = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
 }
 
-// The unit of a matrix from its blocks' magnitudes: the power of two 2^e with
-// largest / 2^e in [2^13, 2^14) (one workgroup of 256 threads).
-__device__ __forceinline__ float unit_of(const float* __restrict__ largest, int n) {
+// units[b] for matrix b: the power of two 2^e that brings its largest magnitude
+// (the maximum of largest[b kLargestBlocks ..]) to [2^13, 2^14).
+__global__ __launch_bounds__(256) void units_kernel(const float* __restrict__ largest, int features_n, int table_n,
+                                                    float* __restrict__ units) {
   __shared__ float lds[4];
+  const int n = blockIdx.x == 0 ? features_n : table_n;
   float top = 0.0f;
-  for (int i = threadIdx.x; i < n; i += 256) top = fmaxf(top, largest[i]);
+  for (int i = threadIdx.x; i < n; i += 256) top = fmaxf(top, largest[blockIdx.x * kLargestBlocks + i]);
 #pragma unroll
   for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = top;
   __syncthreads();
+  if (threadIdx.x > 0) return;
   top = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
-  if (top == 0.0f) return 1.0f;
-  int e;
-  frexpf(top, &e);
-  return ldexpf(1.0f, max(e - 14, -126));
+  int e = 14;
+  if (top > 0.0f) frexpf(top, &e);
+  units[blockIdx.x] = ldexpf(1.0f, max(e - 14, -126));
 }
 
 // A matrix laid out for the tile loads: rows of dp = ceil(dim / 8) * 8 16-bit
-// values, zero past dim; fp32 as the planes hi and lo of value / unit (the unit
-// goes to *unit).  Only for fp32 and for rows that the 16-byte loads cannot take
-// (dim or ld not a multiple of 8).
+// values, zero past dim; fp32 as the planes hi and lo of value / unit.  Only for
+// fp32 and for rows that the 16-byte loads cannot take (dim or ld not a multiple of 8).
 template <typename T>
 __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, int64_t ld, int64_t rows, int dim,
                                                    int dp, uint16_t* __restrict__ dst, int64_t plane,
-                                                   const float* __restrict__ largest, int largest_n,
-                                                   float* __restrict__ unit) {
-  float scale = 1.0f;
-  if constexpr (sizeof(T) == 4) {
-    const float u = unit_of(largest, largest_n);
-    if (blockIdx.x == 0 && threadIdx.x == 0) *unit = u;
-    scale = 1.0f / u;
-  }
+                                                   const float* __restrict__ unit) {
+  const float scale = unit ? 1.0f / *unit : 1.0f;
   const int64_t total = rows * (dp / 8);
   for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < total; v += (int64_t)gridDim.x * 256) {
     const int64_t row = v / (dp / 8);
@@ -153,15 +153,6 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, in
   }
 }
 
-// What the tiles' dot products are multiplied by for base-2 logits: scale2 times
-// the operands' units (fp32), kept a normal number so that minus infinity (what
-// lies past the vocabulary) stays that under a scale that underflows, or is zero: the same flat
-// distribution.
-__device__ __forceinline__ float scale_of(float scale2, const float* units) {
-  if (units) scale2 = scale2 * units[0] * units[1];
-  return copysignf(fmaxf(fabsf(scale2), 1.17549435e-38f), scale2);
-}
-
 // m of element e of accumulator block a, from the lane's first m.
 __device__ __forceinline__ constexpr int block_m(int a, int e) { return 32 * a + 8 * (e >> 2) + (e & 3); }
 
@@ -178,14 +169,14 @@ __device__ __forceinline__ int from_first(int64_t target, int64_t base, int firs
 // The logits of a tile (vocabulary m x rows n), reduced to one pair per row:
 // stats[tile * rows + row] = (max, sum of 2^(s log2 e - max)), max the largest
 // s log2 e rounded to fp32 (the exponents are formed from the unrounded product).
-// The tile that holds a row's target also writes its logit in the same units.
+// The tile that holds a row's target also writes its dot product.
 template <class S, typename T>
 __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, Operand features, int dim,
                                                                  int products, float logit_scale2,
                                                                  const float* __restrict__ units, Targets targets,
                                                                  int tiles_m, int tiles_n,
                                                                  float2* __restrict__ stats,
-                                                                 float* __restrict__ label_logit) {
+                                                                 float* __restrict__ label_dot) {
   __shared__ __attribute__((aligned(16))) char lds[S::kLdsBytes];
   const gs_tile::TileAt tile = gs_tile::tile_at(tiles_m, tiles_n);
   const int m0 = tile.m * S::BM, n0 = tile.n * S::BN;
@@ -193,11 +184,12 @@ __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, 
   gs_tile::product<S, T, true, true>(acc, table, features, m0, n0, 0, dim, products, nullptr, lds);
 
   float scale2 = scale_of(logit_scale2, units);
+  const bool flip = scale2 < 0.0f;
   const int lane = threadIdx.x & 63;
   const int wm = gs_tile::wave_m<S>(), wn = gs_tile::wave_n<S>();
   float2* red = reinterpret_cast<float2*>(lds);  // [kWavesM][BN]
   // under a negative scale the dot products change their signs first
-  if (scale2 < 0.0f) {
+  if (flip) {
     scale2 = -scale2;
 #pragma unroll
     for (int a = 0; a < S::kMB; ++a)
@@ -220,7 +212,7 @@ __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, 
             label = acc.c[a][b][e];
             mine = true;
           }
-      if (mine) label_logit[n] = label;  // times scale2, in the join
+      if (mine) label_dot[n] = flip ? -label : label;
     }
     if (m0 + S::BM > table.extent) {
 #pragma unroll
@@ -294,15 +286,15 @@ __device__ __forceinline__ void write_total(Sum s, int reduction, float* loss, i
 }
 
 // Joins the tiles' pairs of each row (kLanes lanes a row, in a fixed order):
-// norm = (maximum, 1 / sum), from which the backward forms the probabilities
+// norm = (maximum, 1 / sum, the label's dot product), from which the backward forms the probabilities
 // 2^(s log2 e - maximum) / sum to fp32's relative precision, and the loss; ignored rows give 0, targets outside the
 // vocabulary NaN.  The block's sum goes to partial[block], or, when there is one block in all, to the result.
 template <int kLanes>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float2* __restrict__ stats,
-                                                            const float* __restrict__ label_logit, int rows,
+                                                            const float* __restrict__ label_dot, int rows,
                                                             int tiles, int vocab, float logit_scale2,
                                                             const float* __restrict__ units, Targets targets,
-                                                            int reduction, float2* __restrict__ norm,
+                                                            int reduction, float4* __restrict__ norm,
                                                             float* __restrict__ loss_rows,
                                                             Sum* __restrict__ partial, bool last,
                                                             float* __restrict__ loss, int64_t* __restrict__ count) {
@@ -332,11 +324,11 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float2* __rest
     if (t != targets.ignore) {
       // in 64 bits, the maximum kept apart: small losses do not drown in the logits' size
       value = t >= 0 && t < vocab
-                  ? (float)(log(sum) + kLn2 * ((double)top - (double)label_logit[row] * (double)fabsf(scale_of(logit_scale2, units))))
+                  ? (float)(log(sum) + kLn2 * ((double)top - (double)label_dot[row] * (double)scale_of(logit_scale2, units)))
                   : __builtin_nanf("");
       mine = {(double)value, 1};
     }
-    if (norm) norm[row] = make_float2(top, (float)(1.0 / sum));
+    if (norm) norm[row] = make_float4(top, (float)(1.0 / sum), label_dot[row], 0.0f);
     if (loss_rows) loss_rows[row] = value;
   }
   const Sum s = block_sum(mine, lds);
@@ -375,16 +367,16 @@ __global__ __launch_bounds__(256) void largest_kernel(const float* __restrict__ 
   if (threadIdx.x == 0) largest[blockIdx.x] = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
 }
 
-// Per row: the factor that ds takes in the piece's products, and one bit: does
-// the row count.  With a gradient for each row the factors are g_i / G, G the
-// largest, so that ds stays in the 16-bit type's range; alpha, applied to the
-// sums, holds the rest.
-__global__ __launch_bounds__(256) void factors_kernel(const float* __restrict__ grad, int64_t rows, int vocab,
-                                                      Targets targets, int reduction, const int64_t* __restrict__ count,
-                                                      float logit_scale, float held_scale,
-                                                      const float* __restrict__ largest, int largest_n,
-                                                      float* __restrict__ factor, uint64_t* __restrict__ counts,
-                                                      float* __restrict__ alpha) {
+// Per row: its RowInfo, and one bit: does the row count.  With a gradient for
+// each row the factors are g_i / G, G the largest, so that ds stays in the 16-bit
+// type's range; alpha, applied to the sums, holds the rest.
+__global__ __launch_bounds__(256) void rows_kernel(const float* __restrict__ grad, int64_t rows, int vocab,
+                                                   Targets targets, int reduction, const int64_t* __restrict__ count,
+                                                   const float4* __restrict__ norm, float logit_scale,
+                                                   float logit_scale2, const float* __restrict__ units,
+                                                   float held_scale, const float* __restrict__ largest, int largest_n,
+                                                   RowInfo* __restrict__ info, uint64_t* __restrict__ counts,
+                                                   float* __restrict__ label_dot, float* __restrict__ alpha) {
   __shared__ float lds[4];
   const int lane = threadIdx.x & 63;
   float G = 1.0f;
@@ -402,10 +394,20 @@ __global__ __launch_bounds__(256) void factors_kernel(const float* __restrict__ 
   bool use = false;
   if (row < rows) {
     const int64_t t = targets.at(row);
+    const float4 z = norm[row];
     use = t != targets.ignore;
-    float f = reduction == GS_REDUCE_NONE ? grad[row] / G : 1.0f;
-    if (use && (t < 0 || t >= vocab)) f = __builtin_nanf("");
-    factor[row] = use ? f * held_scale : 0.0f;
+    RowInfo r = {0.0f, 0.0f, 0.0f, -1};
+    if (use) {
+      const bool in = t >= 0 && t < vocab;
+      const float f = (reduction == GS_REDUCE_NONE ? grad[row] / G : 1.0f) * (in ? held_scale : __builtin_nanf(""));
+      r.top = z.x;
+      r.share = f * z.y;
+      const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(z.z, scale_of(logit_scale2, units), -z.x));
+      r.label = __builtin_fmaf(e, r.share, -f);
+      r.target = in ? (int)t : -1;
+    }
+    info[row] = r;
+    label_dot[row] = z.z;
   }
   const uint64_t bits = __ballot(use);
   if (lane == 0 && row < rows) counts[row / 64] = bits;
@@ -427,10 +429,9 @@ __device__ __forceinline__ bool row_counts(const uint64_t* counts, int64_t row) 
 template <class S, typename T, int kPlanes>
 __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, Operand features, int dim,
                                                                  int products, float logit_scale2,
-                                                                 const float* __restrict__ units, Targets targets,
-                                                                 int64_t m_base, int tiles_m, int tiles_n,
-                                                                 const float2* __restrict__ norm,
-                                                                 const float* __restrict__ factor,
+                                                                 const float* __restrict__ units, int32_t m_base,
+                                                                 int tiles_m, int tiles_n,
+                                                                 const RowInfo* __restrict__ info,
                                                                  const uint64_t* __restrict__ counts,
                                                                  uint16_t* __restrict__ ds, int64_t ld,
                                                                  int64_t plane) {
@@ -446,19 +447,18 @@ __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, 
 #pragma unroll
   for (int b = 0; b < S::kNB; ++b) {
     const int n = min(n0 + wn + 32 * b + (lane & 31), features.extent - 1);
-    const int label_at = from_first(targets.at(n), m_base, first, S::kWaveM, table.extent);
-    const float2 z = norm[n];
-    const float f = factor[n], share = f * z.y;
+    const RowInfo r = info[n];
+    const int label_at = from_first(r.target, m_base, first, S::kWaveM, table.extent);
 #pragma unroll
     for (int a = 0; a < S::kMB; ++a)
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        acc.c[a][b][e] = share * __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[a][b][e], scale2, -z.x));
+        acc.c[a][b][e] = r.share * __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[a][b][e], scale2, -r.top));
     if (__any(label_at >= 0)) {
 #pragma unroll
       for (int a = 0; a < S::kMB; ++a)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc.c[a][b][e] -= label_at == block_m(a, e) ? f : 0.0f;
+        for (int e = 0; e < 16; ++e) acc.c[a][b][e] = label_at == block_m(a, e) ? r.label : acc.c[a][b][e];
     }
     if (m0 + S::BM > table.extent) {
 #pragma unroll
@@ -624,56 +624,95 @@ static int check_pointers(const Problem& p) {
   return GS_OK;
 }
 
-// Where a matrix's layout for the tile loads goes, if it needs one.
-struct Layout {
-  uint16_t* space;
-  float* unit;     // fp32
-  float* largest;  // fp32: kLargestBlocks
-  int largest_n;
-};
-
-// fp32: the magnitudes that the layout's unit comes from.
-static void measure(const Problem& p, const void* src, int64_t ld, int64_t rows, Targets targets, Layout& to,
-                    hipStream_t s) {
-  if (p.dtype != GS_FP32) return;
-  to.largest_n = (int)min(ceil_div(rows, 32), (int64_t)kLargestBlocks);
-  magnitude_kernel<<<to.largest_n, 256, 0, s>>>((const float*)src, ld, rows, p.dim, targets, to.largest);
-}
-
-// The operand of `rows` rows from row `first` of a matrix: in place, or laid out.
-static Operand operand(const Problem& p, const void* src, int64_t ld, int64_t first, int64_t rows, const Layout& to,
-                       hipStream_t s) {
+// The operand of `rows` rows from row `first` of a matrix: in place, or laid out in space.
+static Operand operand(const Problem& p, const void* src, int64_t ld, int64_t first, int64_t rows, uint16_t* space,
+                       const float* unit, hipStream_t s) {
   const char* at = (const char*)src + first * ld * (int64_t)p.element();
   if (!p.packs(ld)) return {(const uint16_t*)at, ld, 0, (int32_t)rows};
   const int64_t plane = rows * p.dp();
   const int blocks = (int)min(ceil_div(plane / 8, 256), (int64_t)8192);
   if (p.dtype == GS_FP32)
-    pack_kernel<<<blocks, 256, 0, s>>>((const float*)at, ld, rows, p.dim, (int)p.dp(), to.space, plane, to.largest,
-                                       to.largest_n, to.unit);
+    pack_kernel<<<blocks, 256, 0, s>>>((const float*)at, ld, rows, p.dim, (int)p.dp(), space, plane, unit);
   else
-    pack_kernel<<<blocks, 256, 0, s>>>((const _Float16*)at, ld, rows, p.dim, (int)p.dp(), to.space, plane, nullptr, 0,
-                                       nullptr);
-  return {to.space, p.dp(), plane, (int32_t)rows};
+    pack_kernel<<<blocks, 256, 0, s>>>((const _Float16*)at, ld, rows, p.dim, (int)p.dp(), space, plane, nullptr);
+  return {space, p.dp(), plane, (int32_t)rows};
 }
 
-// Both matrices' layouts; units: the features' and the table's, side by side (fp32; else null).
+// Both matrices' layouts for the tile loads, where they need one, and (fp32, else null) their units.
 struct Layouts {
-  Layout features, table;
-  float* units;
+  uint16_t *features_space, *table_space;
+  float *units, *largest;
   Layouts() = default;
   Layouts(const Problem& p, int64_t rows_piece, Carve& c) {
-    units = c.take<float>(p.dtype == GS_FP32 ? 2 : 0);
-    if (p.dtype != GS_FP32) units = nullptr;
-    features = {c.take<uint16_t>(p.packs(p.ld_features) ? rows_piece * p.dp() * p.planes() : 0), units,
-                c.take<float>(p.dtype == GS_FP32 ? kLargestBlocks : 0), 0};
-    table = {c.take<uint16_t>(p.packs(p.ld_table) ? p.vocab * p.dp() * p.planes() : 0), units ? units + 1 : nullptr,
-             c.take<float>(p.dtype == GS_FP32 ? kLargestBlocks : 0), 0};
+    const bool fp32 = p.dtype == GS_FP32;
+    features_space = c.take<uint16_t>(p.packs(p.ld_features) ? rows_piece * p.dp() * p.planes() : 0);
+    table_space = c.take<uint16_t>(p.packs(p.ld_table) ? p.vocab * p.dp() * p.planes() : 0);
+    units = c.take<float>(fp32 ? 2 : 0);
+    largest = c.take<float>(fp32 ? 2 * kLargestBlocks : 0);
+    if (!fp32) units = nullptr;
   }
-  void measure(const Problem& p, Targets targets, hipStream_t s) {
-    gs_xent::measure(p, p.features, p.ld_features, p.rows, targets, features, s);
-    gs_xent::measure(p, p.table, p.ld_table, p.vocab, {nullptr, 64, 0}, table, s);
+  const float* features_unit() const { return units; }
+  const float* table_unit() const { return units ? units + 1 : nullptr; }
+  // fp32: the units, from the matrices' magnitudes
+  void measure(const Problem& p, Targets targets, hipStream_t s) const {
+    if (!units) return;
+    auto one = [&](const void* src, int64_t ld, int64_t rows, Targets t, float* to) {
+      const bool flat = ld == p.dim && rows * p.dim % 4 == 0 && (uintptr_t)src % 16 == 0;
+      const int blocks = (int)min(ceil_div(rows * p.dim, 4096), (int64_t)kLargestBlocks);
+      magnitude_kernel<<<blocks, 256, 0, s>>>((const float*)src, ld, rows, p.dim, flat, t, to);
+      return blocks;
+    };
+    const int features_n = one(p.features, p.ld_features, p.rows, targets, largest);
+    const int table_n = one(p.table, p.ld_table, p.vocab, {nullptr, 64, 0}, largest + kLargestBlocks);
+    units_kernel<<<2, 256, 0, s>>>(largest, features_n, table_n, units);
+  }
+  Operand features(const Problem& p, int64_t first, int64_t rows, hipStream_t s) const {
+    return operand(p, p.features, p.ld_features, first, rows, features_space, features_unit(), s);
+  }
+  Operand table(const Problem& p, hipStream_t s) const {
+    return operand(p, p.table, p.ld_table, 0, p.vocab, table_space, table_unit(), s);
   }
 };
+
+// Short rows: the kernels that hold one operand in registers (gs_resident.h).
+static bool resident(const Problem& p) { return p.dp() <= (p.dtype == GS_FP32 ? 64 : 128); }
+
+// Parts along the streamed operand for `slots` workgroups at a time: whole rounds
+// of the chip, each a part's tiles and about six tiles' time to begin and end;
+// and what it costs to write and add the parts' fp32 sums (sum_bytes a part) at
+// a tile's microsecond.
+static int resident_parts(int64_t held, int64_t stream, int64_t slots, double sum_bytes) {
+  const int64_t blocks = ceil_div(held, gs_resident::kHeldRows), tiles = ceil_div(stream, gs_resident::kTileRows);
+  const int64_t most = min(max((int64_t)1, tiles / 4), max((int64_t)4, 2 * ceil_div(slots, blocks)));
+  int64_t best = 1;
+  double least = 1e300;
+  for (int64_t n = 1; n <= most; ++n) {
+    const double cost = (double)(ceil_div(blocks * n, slots) * (ceil_div(tiles, n) + 6)) +
+                        (n > 1 ? (double)n * sum_bytes / 2.0e6 : 0.0);
+    if (cost < least) {
+      least = cost;
+      best = n;
+    }
+  }
+  return (int)best;
+}
+
+static int32_t part_rows(int64_t stream, int64_t parts) {
+  return (int32_t)round_up(ceil_div(stream, parts), gs_resident::kTileRows);
+}
+
+template <typename T, int kKind>
+static void launch_resident(const Problem& p, const gs_resident::Args& a, int parts, hipStream_t s) {
+  const dim3 grid((unsigned)ceil_div(a.held.extent, gs_resident::kHeldRows), (unsigned)parts);
+  if constexpr (std::is_same<T, _Float16>::value) {
+    if (p.dtype == GS_FP32) {
+      gs_resident::resident_kernel<T, 1, gs_tile::kSplitPlanes, kKind><<<grid, gs_resident::kThreads, 0, s>>>(a);
+      return;
+    }
+  }
+  if (a.dim <= 64) gs_resident::resident_kernel<T, 1, 1, kKind><<<grid, gs_resident::kThreads, 0, s>>>(a);
+  else gs_resident::resident_kernel<T, 2, 1, kKind><<<grid, gs_resident::kThreads, 0, s>>>(a);
+}
 
 // Big or Mid tiles for a product of M x N (parts: copies of it side by side):
 // the time of whole rounds of the chip's 256 CUs, one Big workgroup each or two
@@ -693,7 +732,7 @@ static void with_logits_shape(int64_t vocab, int64_t rows, F f) {
 }
 
 struct ForwardPlan {
-  enum { kThin32, kThin64, kMid, kBig } shape;
+  enum { kThin32, kThin64, kResident, kMid, kBig } shape;
   int64_t rows_piece, tiles_m, blocks;
   int lanes;
   Layouts layouts;
@@ -703,9 +742,11 @@ struct ForwardPlan {
   size_t bytes;
 
   ForwardPlan(const Problem& p, void* ws) {
-    shape = p.rows <= 32 ? kThin32 : p.rows <= 64 ? kThin64 : takes_big(p.vocab, p.rows) ? kBig : kMid;
+    shape = p.rows <= 32 ? kThin32 : p.rows <= 64 ? kThin64 : resident(p) ? kResident
+            : takes_big(p.vocab, p.rows) ? kBig : kMid;
     const int bm = shape == kBig ? Big::BM : shape == kMid ? Mid::BM : Thin32::BM;
-    tiles_m = ceil_div(p.vocab, bm);
+    // (two of its workgroups share a CU)
+    tiles_m = shape == kResident ? resident_parts(p.rows, p.vocab, 512, 0.0) : ceil_div(p.vocab, bm);
     rows_piece = max((int64_t)256, kStatBytes / (tiles_m * (int64_t)sizeof(float2)) / 256 * 256);
     rows_piece = min(p.rows, min(rows_piece, (int64_t)1 << 20));
     lanes = p.rows <= 4096 ? 64 : 1;
@@ -731,19 +772,33 @@ static void launch_logits_fwd(const Problem& p, const ForwardPlan& f, const Oper
 }
 
 template <typename T>
-static int forward(const Problem& p, Targets targets, float logit_scale, int reduction, float* loss, float2* norm,
+static int forward(const Problem& p, Targets targets, float logit_scale, int reduction, float* loss, float4* norm,
                    int64_t* count, ForwardPlan& f, hipStream_t s) {
   const float scale2 = logit_scale * kLog2e;
   f.layouts.measure(p, targets, s);
-  const Operand table = operand(p, p.table, p.ld_table, 0, p.vocab, f.layouts.table, s);
+  const Operand table = f.layouts.table(p, s);
   int64_t block = 0;
   for (int64_t r = 0; r < p.rows; r += f.rows_piece) {
     const int64_t rows = min(f.rows_piece, p.rows - r);
-    const Operand features = operand(p, p.features, p.ld_features, r, rows, f.layouts.features, s);
+    const Operand features = f.layouts.features(p, r, rows, s);
     const Targets t = targets.from(r);
     switch (f.shape) {
       case ForwardPlan::kThin32: launch_logits_fwd<Thin32, T>(p, f, table, features, scale2, t, s); break;
       case ForwardPlan::kThin64: launch_logits_fwd<Thin64, T>(p, f, table, features, scale2, t, s); break;
+      case ForwardPlan::kResident: {
+        gs_resident::Args a = {};
+        a.held = features;
+        a.stream = table;
+        a.part = part_rows(p.vocab, f.tiles_m);
+        a.dim = (int32_t)p.dp();
+        a.logit_scale2 = scale2;
+        a.units = f.layouts.units;
+        a.targets = t;
+        a.stats = f.stats;
+        a.label_dot = f.label;
+        launch_resident<T, gs_resident::kForward>(p, a, (int)f.tiles_m, s);
+        break;
+      }
       case ForwardPlan::kMid: launch_logits_fwd<Mid, T>(p, f, table, features, scale2, t, s); break;
       case ForwardPlan::kBig: launch_logits_fwd<Big, T>(p, f, table, features, scale2, t, s); break;
     }
@@ -793,11 +848,21 @@ struct BackwardPlan {
   bool direct_h, direct_t;  // one part and one piece: no fp32 sums in between
   Layouts layouts;
   uint16_t* ds;
-  float *factor, *alpha, *largest, *part_h, *part_t;
+  RowInfo* info;
+  float *label_dot, *alpha, *largest, *part_h, *part_t;
   uint64_t* counts;
   size_t bytes;
 
   BackwardPlan(const Problem& p, bool want_h, bool want_t, void* ws) {
+    if (resident(p)) {  // one piece of everything, and no ds
+      rows_piece = p.rows;
+      cols_piece = p.vocab;
+      ld = 0;
+      parts_h = want_h ? resident_parts(p.rows, p.vocab, 256, 4.0 * p.rows * p.dim) : 1;
+      parts_t = want_t ? resident_parts(p.vocab, p.rows, 256, 4.0 * p.vocab * p.dim) : 1;
+      carve(p, want_h, want_t, ws);
+      return;
+    }
     // The piece: a part of the longer side against (if it fits) the whole of the
     // shorter, whose gradient's sums then wait from piece to piece; that one is the smaller.
     const int64_t most = kPieceBytes / (2 * p.ds_planes());  // elements of ds
@@ -809,16 +874,21 @@ struct BackwardPlan {
       cols_piece = min((int64_t)p.vocab, most / rows_piece / 256 * 256);
     }
     ld = round_up(cols_piece, 256);
-    row_pieces = ceil_div(p.rows, rows_piece);
-    col_pieces = ceil_div(p.vocab, cols_piece);
     parts_h = want_h ? parts_for(rows_piece, p.dim, cols_piece) : 1;
     parts_t = want_t ? parts_for(cols_piece, p.dim, rows_piece) : 1;
+    carve(p, want_h, want_t, ws);
+  }
+
+  void carve(const Problem& p, bool want_h, bool want_t, void* ws) {
+    row_pieces = ceil_div(p.rows, rows_piece);
+    col_pieces = ceil_div(p.vocab, cols_piece);
     direct_h = parts_h == 1 && col_pieces == 1;
     direct_t = parts_t == 1 && row_pieces == 1;
     Carve c{(char*)ws};
     layouts = Layouts(p, rows_piece, c);
     ds = c.take<uint16_t>(rows_piece * ld * p.ds_planes());
-    factor = c.take<float>(p.rows);
+    info = c.take<RowInfo>(p.rows);
+    label_dot = c.take<float>(p.rows);
     counts = c.take<uint64_t>(ceil_div(p.rows, 64));
     alpha = c.take<float>(1);
     largest = c.take<float>(kLargestBlocks);
@@ -831,7 +901,7 @@ struct BackwardPlan {
 static unsigned finish_blocks(int64_t n) { return (unsigned)min(ceil_div(n, 256), (int64_t)8192); }
 
 template <typename T, typename Out, int kPlanes>
-static int backward(const Problem& p, Targets targets, float logit_scale, int reduction, const float2* norm,
+static int backward(const Problem& p, Targets targets, float logit_scale, int reduction, const float4* norm,
                     const int64_t* count, const float* grad_loss, Out* grad_features, Out* grad_table,
                     BackwardPlan& b, hipStream_t s) {
   const float scale2 = logit_scale * kLog2e;
@@ -841,15 +911,46 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
     largest_n = (int)min(ceil_div(p.rows, 256), (int64_t)kLargestBlocks);
     largest_kernel<<<largest_n, 256, 0, s>>>(grad_loss, p.rows, targets, b.largest);
   }
-  factors_kernel<<<(unsigned)ceil_div(p.rows, 256), 256, 0, s>>>(grad_loss, p.rows, p.vocab, targets, reduction, count,
-                                                                 logit_scale, Held<T>::kScale, b.largest, largest_n,
-                                                                 b.factor, b.counts, b.alpha);
   b.layouts.measure(p, targets, s);
-  const float *unit_h = b.layouts.features.unit, *unit_w = b.layouts.table.unit;
-  const Operand table = operand(p, p.table, p.ld_table, 0, p.vocab, b.layouts.table, s);
+  const float *unit_h = b.layouts.features_unit(), *unit_w = b.layouts.table_unit();
+  rows_kernel<<<(unsigned)ceil_div(p.rows, 256), 256, 0, s>>>(grad_loss, p.rows, p.vocab, targets, reduction, count, norm,
+                                                              logit_scale, scale2, b.layouts.units, Held<T>::kScale,
+                                                              b.largest, largest_n, b.info, b.counts, b.label_dot, b.alpha);
+  const Operand table = b.layouts.table(p, s);
+  if (resident(p)) {
+    const Operand features = b.layouts.features(p, 0, p.rows, s);
+    gs_resident::Args a = {};
+    a.dim = (int32_t)p.dp();
+    a.logit_scale2 = scale2;
+    a.units = b.layouts.units;
+    a.label_dot = b.label_dot;
+    a.info = b.info;
+    a.counts = b.counts;
+    a.alpha = b.alpha;
+    a.D = D;
+    auto run = [&](auto kind, const Operand& held, const Operand& stream, int parts, float* sums, const float* unit,
+                   Out* out) {
+      a.held = held;
+      a.stream = stream;
+      a.part = part_rows(stream.extent, parts);
+      a.part_sums = parts > 1 ? sums : nullptr;
+      a.part_plane = (int64_t)held.extent * D;
+      a.unit = unit;
+      a.out = out;
+      launch_resident<T, decltype(kind)::value>(p, a, parts, s);
+      if (parts > 1)
+        finish_kernel<<<finish_blocks(a.part_plane), 256, 0, s>>>(sums, parts, a.part_plane, a.part_plane, D, nullptr,
+                                                                 b.alpha, unit, out);
+    };
+    if (grad_features)
+      run(std::integral_constant<int, gs_resident::kFeatures>{}, features, table, b.parts_h, b.part_h, unit_w, grad_features);
+    if (grad_table)
+      run(std::integral_constant<int, gs_resident::kTable>{}, table, features, b.parts_t, b.part_t, unit_h, grad_table);
+    return gs_status_from_hip(hipGetLastError());
+  }
   for (int64_t r = 0; r < p.rows; r += b.rows_piece) {
     const int32_t rows = (int32_t)min(b.rows_piece, p.rows - r);
-    const Operand features = operand(p, p.features, p.ld_features, r, rows, b.layouts.features, s);
+    const Operand features = b.layouts.features(p, r, rows, s);
     const uint64_t* counts = b.counts + r / 64;
     const int64_t ds_plane = rows * b.ld;
     for (int64_t c = 0; c < p.vocab; c += b.cols_piece) {
@@ -862,8 +963,8 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
         typedef decltype(shape) S;
         const int tiles_m = (int)ceil_div(cols, S::BM), tiles_n = (int)ceil_div(rows, S::BN);
         logits_bwd_kernel<S, T, kPlanes><<<(unsigned)((int64_t)tiles_m * tiles_n), S::kThreads, 0, s>>>(
-            piece, features, (int)p.dp(), p.products(), scale2, b.layouts.units, targets.from(r), c, tiles_m, tiles_n,
-            norm + r, b.factor + r, counts, b.ds, b.ld, ds_plane);
+            piece, features, (int)p.dp(), p.products(), scale2, b.layouts.units, (int32_t)c, tiles_m, tiles_n,
+            b.info + r, counts, b.ds, b.ld, ds_plane);
       });
       with_columns(columns_of(D), [&](auto shape) {
         typedef decltype(shape) S;
@@ -949,7 +1050,7 @@ extern "C" int gs_xent_fwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dty
   gs_xent::ForwardPlan f(p, workspace);
   const gs_xent::Targets t = {targets, target_bits, ignore_index};
   auto* run = dtype == GS_BF16 ? gs_xent::forward<__bf16> : gs_xent::forward<_Float16>;  // fp32: planes of fp16
-  return run(p, t, logit_scale, reduction, loss, (float2*)norm, count, f, s);
+  return run(p, t, logit_scale, reduction, loss, (float4*)norm, count, f, s);
 }
 
 extern "C" size_t gs_xent_bwd_workspace_bytes(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype,
@@ -987,11 +1088,11 @@ extern "C" int gs_xent_bwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dty
   gs_xent::BackwardPlan b(p, want_h, want_t, workspace);
   const gs_xent::Targets t = {targets, target_bits, ignore_index};
   if (dtype == GS_FP32)
-    return gs_xent::backward<_Float16, float, gs_tile::kWidePlanes>(p, t, logit_scale, reduction, (const float2*)norm, count, grad_loss,
+    return gs_xent::backward<_Float16, float, gs_tile::kWidePlanes>(p, t, logit_scale, reduction, (const float4*)norm, count, grad_loss,
                                                (float*)grad_features, (float*)grad_table, b, s);
   if (dtype == GS_BF16)
-    return gs_xent::backward<__bf16, __bf16, 1>(p, t, logit_scale, reduction, (const float2*)norm, count, grad_loss,
+    return gs_xent::backward<__bf16, __bf16, 1>(p, t, logit_scale, reduction, (const float4*)norm, count, grad_loss,
                                                 (__bf16*)grad_features, (__bf16*)grad_table, b, s);
-  return gs_xent::backward<_Float16, _Float16, 1>(p, t, logit_scale, reduction, (const float2*)norm, count, grad_loss,
+  return gs_xent::backward<_Float16, _Float16, 1>(p, t, logit_scale, reduction, (const float4*)norm, count, grad_loss,
                                                   (_Float16*)grad_features, (_Float16*)grad_table, b, s);
 }

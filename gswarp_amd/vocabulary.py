@@ -150,7 +150,7 @@ def _entropy_forward(features, table, targets, ignore_index, reduction, logit_sc
     lib = _lib.load()
     code, reduce = _DTYPES[table.dtype], _REDUCTIONS[reduction]
     loss = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=device)
-    norm = torch.empty((n, 2), dtype=torch.float32, device=device) if keep else None
+    norm = torch.empty((n, 4), dtype=torch.float32, device=device) if keep else None
     with _device_guard(device), _workspace.device_lock(device):
         nbytes = lib.gs_xent_fwd_workspace_bytes(n, vocab, dim, code, _row_stride(features), _row_stride(table))
         # the count of rows sits in front of the workspace

@@ -604,9 +604,9 @@ int gs_embed_bwd(int64_t n, int32_t vocab, int32_t dim, int32_t dtype, const voi
  * s_{i, targets_i}.  Rows whose target is ignore_index give 0 and do not
  * count, whatever they hold; any other target outside [0, vocab) gives NaN.
  * loss: `rows` fp32 for GS_REDUCE_NONE, else one (the sum, or the mean over
- * the rows that count; over none, NaN).  norm (2 fp32 a row, 8-byte aligned;
- * NULL if no backward follows) receives max_j s_ij / ln 2 and 1 / sum_j
- * exp(s_ij - max), count the number of rows that count; gs_xent_bwd takes both.  features and table must be 16-byte
+ * the rows that count; over none, NaN).  norm (4 fp32 a row, 16-byte aligned;
+ * NULL if no backward follows) receives what gs_xent_bwd needs of the row's
+ * softmax, count the number of rows that count.  features and table must be 16-byte
  * aligned unless they are fp32 or have a dim or row distance that is not a
  * multiple of 8 (those are laid out in the workspace first).  workspace:
  * gs_xent_fwd_workspace_bytes bytes on 256, of any content.
