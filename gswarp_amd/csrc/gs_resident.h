@@ -1,5 +1,5 @@
-// The cross entropy's products for short rows (up to 128 values of 16 bits, 64 of
-// fp32): one operand's rows stay in registers, the other's stream through LDS in
+// The cross entropy's products for short rows (up to 128 values of 16 bits or 64
+// of fp32, and twice that where only the loss is wanted): one operand's rows stay in registers, the other's stream through LDS in
 // tiles of 64 rows, and the logits of a tile never leave the registers of the
 // wave that formed them.
 //
@@ -17,8 +17,8 @@
 // What the products bring per element is little, so the vector instructions
 // count: an element takes an fma, an exponential and a multiplication.  The label
 // is kept out of that: its logit is formed once per row (kForward), kFeatures
-// adds (v_t - what p_t was rounded to) w_t at the end, and kTable writes v_t over p_t
-// on its way through LDS, v_t = f (p_t - 1) formed once per row in fp32.
+// looks for it only in the tiles that hold one of a wave's labels, and kTable
+// writes f (p_t - 1), formed once per row in fp32, over p_t on its way through LDS.
 #pragma once
 
 #include "gs_tile.h"
@@ -34,7 +34,9 @@ using gs_tile::mfma;
 using gs_tile::Operand;
 using gs_tile::Pack;
 using gs_xent::RowInfo;
+using gs_xent::kLn2f;
 using gs_xent::scale_of;
+using gs_xent::settled;
 
 enum Kind { kForward, kFeatures, kTable };
 
@@ -49,8 +51,8 @@ struct Args {
   int32_t dim;   // of the operands, padded to 8
   float logit_scale2;
   const float* units;
-  float* label_dot;  // the rows' labels' dot products: written by kForward, read by kFeatures
-  // kForward: stats[part * rows + row]
+  // kForward: stats[part * rows + row], and the rows' labels' dot products, upright
+  float* label_dot;
   gs_xent::Targets targets;
   float2* stats;
   // kFeatures, kTable
@@ -127,15 +129,8 @@ __device__ __forceinline__ void planes_of(const f32x16& s, int from, typename Pa
     }
 }
 
-// What a value becomes in the planes.
-template <typename T, int kPlanes>
-__device__ __forceinline__ float rounded(float v) {
-  if (kPlanes > 1) return v;
-  return (float)(T)v;
-}
-
 template <typename T, int KB, int PL, int kKind>
-__global__ __launch_bounds__(kThreads, kKind == kForward ? 4 : 2) void resident_kernel(Args a) {
+__global__ __launch_bounds__(kThreads, kKind == kForward && KB * PL <= 2 ? 4 : 2) void resident_kernel(Args a) {
   typedef gs_tile::Stage<true, kTileRows, kWaves> Stage;
   typedef typename Pack<T>::v8 v8;
   constexpr int kTile = PL * KB * Stage::kBytes;
@@ -144,6 +139,10 @@ __global__ __launch_bounds__(kThreads, kKind == kForward ? 4 : 2) void resident_
   constexpr int kDsPlanes = PL > 1 ? gs_tile::kWidePlanes : 1;
   constexpr int kSums = kKind == kForward ? 1 : PL > 1 ? 3 : 1;  // sums of one step down each
   constexpr int kDBlocks = kKind == kForward ? 1 : 2 * KB;
+  // kFeatures forms the logits of a tile while those of the one before go through
+  // the exponentials and the second product (133k x 1203 x 100 fp16: 136 -> 125 us);
+  // the others gain nothing from it, or lack the registers.
+  constexpr int kLag = kKind == kFeatures && PL == 1 ? 1 : 0;
   __shared__ __attribute__((aligned(16))) char lds[kStages * (kTile + kInfo) + kTurn];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
@@ -166,7 +165,7 @@ __global__ __launch_bounds__(kThreads, kKind == kForward ? 4 : 2) void resident_
       f32x16 s;
       logits<T, KB, PL>(s, [&](int p, int k) { return at_label.v[p][k]; }, [&](int p, int k) { return held.v[p][k]; });
       const float d = diagonal(s);
-      if (held_in && half == 0) a.label_dot[held_row] = d;
+      if (held_in && half == 0) a.label_dot[held_row] = scale2 < 0.0f ? -d : d;
     }
   } else if (kKind == kFeatures) {
     counts = held_in && ((a.counts[held_row >> 6] >> (held_row & 63)) & 1);
@@ -213,13 +212,13 @@ __global__ __launch_bounds__(kThreads, kKind == kForward ? 4 : 2) void resident_
     }
     ++loaded;
   };
-  // a block past dim (dim 65 .. 128 has two, dim up to 64 one) is loaded too: as zeros
-  constexpr int kLoads = PL * KB * Stage::kLoads + (kKind == kTable ? 1 : 0), kAhead = kStages - 1;
+  // (a block past dim is loaded too: as zeros)
+  constexpr int kLoads = PL * KB * Stage::kLoads + (kKind == kTable ? 1 : 0), kAhead = kStages - 1 - kLag;
 #pragma unroll
   for (int t = 0; t < kAhead; ++t)
     if (t < tiles) load();
 
-  float top = -INFINITY, sum = 0.0f;
+  float x = -INFINITY, sum = 0.0f;  // kForward, see settled()
   f32x16 acc[kSums][kDBlocks];
   if (kKind != kForward) {
 #pragma unroll
@@ -228,9 +227,9 @@ __global__ __launch_bounds__(kThreads, kKind == kForward ? 4 : 2) void resident_
       for (int d = 0; d < kDBlocks; ++d) acc[i][d] = f32x16{};
   }
 
-  // one tile, held in LDS at `tile`
-  auto work = [&](const char* __restrict__ tile, const char* __restrict__ infos, int first) {
-    f32x16 s[2];
+  auto at = [&](int t) { return (const char*)lds + (t % kStages) * (kTile + kInfo); };
+  // the logits of tile t
+  auto form = [&](f32x16* s, const char* __restrict__ tile) {
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       auto streamed = [&](int p, int k) {
@@ -241,6 +240,9 @@ __global__ __launch_bounds__(kThreads, kKind == kForward ? 4 : 2) void resident_
       if (kKind == kTable) logits<T, KB, PL>(s[b], own, streamed);
       else logits<T, KB, PL>(s[b], streamed, own);
     }
+  };
+  // and what becomes of them
+  auto use = [&](f32x16* s, const char* __restrict__ tile, const char* __restrict__ infos, int first) {
     if constexpr (kKind == kForward) {
       if (scale2 < 0.0f) {
         s[0] = -s[0];
@@ -259,20 +261,32 @@ __global__ __launch_bounds__(kThreads, kKind == kForward ? 4 : 2) void resident_
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int e = 0; e < 16; ++e) raw = fmaxf(raw, s[b][e]);
-      const float now = fmaxf(top, raw * scale), ref = now == -INFINITY ? 0.0f : now;
-      float part[4] = {sum * __builtin_amdgcn_exp2f(top - ref), 0.0f, 0.0f, 0.0f};
+      const float now = fmaxf(x, raw), top = now == -INFINITY ? 0.0f : now * scale;
+      float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) part[e & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], scale, -ref));
-      sum = (part[0] + part[1]) + (part[2] + part[3]);
-      top = now;
+        for (int e = 0; e < 16; ++e) part[e & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], scale, -top));
+      const float all = (part[0] + part[1]) + (part[2] + part[3]);
+      if (now > x) {  // the largest so far is among these
+        sum = sum * __builtin_amdgcn_exp2f((x - now) * scale) + settled(now, scale, all);
+        x = now;
+      } else {
+        sum += all * (1.0f - (now == -INFINITY ? 0.0f : __builtin_fmaf(now, scale, -top)) * kLn2f);
+      }
     } else if constexpr (kKind == kFeatures) {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           s[b][e] = row.share * __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], scale2, -row.top));
+      const int label_at = row.target - first - 4 * half;  // from the lane's first of the tile's rows
+      if (__any(label_at >= 0 && label_at < kTileRows)) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[b][e] = label_at == 32 * b + block_m(e) ? row.label : s[b][e];
+      }
       if (first + kTileRows > end) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -360,32 +374,53 @@ __global__ __launch_bounds__(kThreads, kKind == kForward ? 4 : 2) void resident_
     }
   };
 
-  for (int t = 0; t < tiles; ++t) {
+  auto arrive = [&](int t) {
     if (t + kAhead <= tiles) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kAhead - 1) * kLoads) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     if (loaded < tiles) load();
-    const char* tile = lds + (t % kStages) * (kTile + kInfo);
-    work(tile, tile + kTile + wave * 1024, begin + t * kTileRows);
+  };
+  auto finish = [&](f32x16* s, int t) { use(s, at(t), at(t) + kTile + wave * 1024, begin + t * kTileRows); };
+  f32x16 s0[2], s1[2];
+  if constexpr (kLag == 0) {
+    for (int t = 0; t < tiles; ++t) {
+      arrive(t);
+      form(s0, at(t));
+      finish(s0, t);
+    }
+  } else {
+    int t = 1;
+    if (tiles > 0) {
+      arrive(0);
+      form(s0, at(0));
+    }
+    for (; t + 1 < tiles; t += 2) {
+      arrive(t);
+      form(s1, at(t));
+      finish(s0, t - 1);
+      arrive(t + 1);
+      form(s0, at(t + 1));
+      finish(s1, t);
+    }
+    if (t < tiles) {
+      arrive(t);
+      form(s1, at(t));
+      finish(s0, t - 1);
+      finish(s1, t);
+    } else if (tiles > 0) {
+      finish(s0, t - 1);
+    }
   }
 
   if constexpr (kKind == kForward) {
     // the two halves of the wave hold the same rows
-    const float otop = __shfl_xor(top, 32), osum = __shfl_xor(sum, 32);
-    const float all = fmaxf(top, otop), ref = all == -INFINITY ? 0.0f : all;
-    sum = sum * __builtin_amdgcn_exp2f(top - ref) + osum * __builtin_amdgcn_exp2f(otop - ref);
+    const float ox = __shfl_xor(x, 32), osum = __shfl_xor(sum, 32), all = fmaxf(x, ox), scale = fabsf(scale2);
+    sum = sum * (x == all ? 1.0f : __builtin_amdgcn_exp2f((x - all) * scale)) +
+          osum * (ox == all ? 1.0f : __builtin_amdgcn_exp2f((ox - all) * scale));
     if (held_in && half == 0) a.stats[(int64_t)blockIdx.y * a.held.extent + held_row] = make_float2(all, sum);
   } else {
     if (!held_in) return;
-    float fix = 0.0f;
-    const uint16_t* w = nullptr;
-    if (kKind == kFeatures && blockIdx.y == 0 && row.target >= 0) {
-      // what the label's term lacks: the products took p_t as it was rounded
-      const float p_t = row.share * __builtin_amdgcn_exp2f(__builtin_fmaf(a.label_dot[held_row], scale2, -row.top));
-      fix = row.label - rounded<T, kDsPlanes>(p_t);
-      w = a.stream.p + (int64_t)row.target * a.stream.ld;
-    }
     const float al = a.part_sums ? 1.0f : a.unit ? *a.alpha * *a.unit : *a.alpha;
 #pragma unroll
     for (int d = 0; d < kDBlocks; ++d)
@@ -398,16 +433,6 @@ __global__ __launch_bounds__(kThreads, kKind == kForward ? 4 : 2) void resident_
           v[j] = acc[0][d][4 * q + j];
           if constexpr (PL > 1)
             v[j] += (acc[1][d][4 * q + j] + acc[2][d][4 * q + j] * (1.0f / kPlaneStep)) * (1.0f / kPlaneStep);
-        }
-        if (w && first < a.dim) {
-          const typename Pack<T>::v4 x = *reinterpret_cast<const typename Pack<T>::v4*>(w + first);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = __builtin_fmaf(fix, (float)x[j], v[j]);
-          if constexpr (PL > 1) {
-            const typename Pack<T>::v4 y = *reinterpret_cast<const typename Pack<T>::v4*>(w + a.stream.plane + first);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = __builtin_fmaf(fix * (1.0f / kPlaneStep), (float)y[j], v[j]);
-          }
         }
         const int64_t at = (int64_t)held_row * a.D + first;
 #pragma unroll

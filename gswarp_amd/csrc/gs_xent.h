@@ -28,12 +28,25 @@ __device__ __forceinline__ float scale_of(float scale2, const float* units) {
   return copysignf(fmaxf(fabsf(scale2), 1.17549435e-38f), scale2);
 }
 
+// A row's maximum and sum are kept as the largest dot product itself, x (turned
+// upright: times the sign of the scale), and the sum of 2^((x_j - x) scale), in
+// which the largest is exactly 1: a label that is all but certain then has a
+// loss, and p - 1, as small as fp32 can tell, not as small as the rounding of the logits' size.
+// Its terms are formed with one fma as 2^(x_j scale - top), top = x scale rounded;
+// this takes the sum of a set that holds x itself from there.
+constexpr float kLn2f = 0.6931471805599453f;
+__device__ __forceinline__ float settled(float x, float scale, float sum) {
+  const float top = x * scale, off = __builtin_fmaf(x, scale, -top);
+  const float rest = sum - __builtin_amdgcn_exp2f(off);  // all but x
+  return 1.0f + __builtin_fmaf(rest, -off * kLn2f, rest);
+}
+
 // What the backward needs of a row, f the factor of its loss's gradient (held
 // scale included): ds = share 2^(s log2 e - top) for every column but the label's, label there.
 struct __attribute__((aligned(16))) RowInfo {
-  float top;    // max s log2 e
-  float share;  // f / sum
-  float label;  // f (p_t - 1), from the label's logit in fp32
+  float top;    // x scale, rounded
+  float share;  // f / sum, and 2^(top - x scale)
+  float label;  // f (p_t - 1)
   int target;   // -1: none in the vocabulary, or the row does not count
 };
 

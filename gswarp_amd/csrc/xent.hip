@@ -60,42 +60,46 @@ struct Held<_Float16> {
 // ------------------------------------------------------------------ packing
 // fp32: the largest finite magnitude of a matrix, one value a block (targets.p:
 // of the rows that count only, so that what ignored rows hold does not reach the
-// unit of the others).  flat: the rows are contiguous, 16-byte aligned and a multiple of 4 long in all.
+// unit of the others).  A group of `lanes` lanes reads a row, V values a lane at a time.
 constexpr int kLargestBlocks = 1024;
+template <int V>
 __global__ __launch_bounds__(256) void magnitude_kernel(const float* __restrict__ src, int64_t ld, int64_t rows,
-                                                        int dim, bool flat, Targets targets,
+                                                        int dim, int lanes, Targets targets,
                                                         float* __restrict__ largest) {
   __shared__ float lds[4];
-  const int lane = threadIdx.x & 63;
-  float top = 0.0f;
-  auto see = [&](float v, int64_t row) {
-    if (v < INFINITY && v > top && (!targets.p || targets.at(row) != targets.ignore)) top = v;
+  struct __attribute__((aligned(4 * V))) Vec {
+    float v[V];
   };
-  if (flat) {
-    const int64_t n = rows * dim / 4, stride = (int64_t)gridDim.x * 256;
-    constexpr int kItems = 4;  // vectors in flight
-    for (int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x; i0 < n; i0 += stride * kItems) {
-      float4 v[kItems];
+  constexpr int kRows = 8;  // rows in flight
+  const int lane = threadIdx.x % lanes;
+  const int64_t groups = (int64_t)gridDim.x * (256 / lanes);
+  float top = 0.0f;
+  for (int64_t r0 = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes; r0 < rows; r0 += groups * kRows) {
+    bool use[kRows];
 #pragma unroll
-      for (int j = 0; j < kItems; ++j)
-        v[j] = i0 + j * stride < n ? reinterpret_cast<const float4*>(src)[i0 + j * stride] : make_float4(0, 0, 0, 0);
-#pragma unroll
-      for (int j = 0; j < kItems; ++j) {
-        const float x[4] = {fabsf(v[j].x), fabsf(v[j].y), fabsf(v[j].z), fabsf(v[j].w)};
-        // few vectors hold a new maximum, so few look their rows up
-        if (x[0] > top || x[1] > top || x[2] > top || x[3] > top)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) see(x[e], ((i0 + j * stride) * 4 + e) / dim);
-      }
+    for (int j = 0; j < kRows; ++j) {
+      const int64_t row = r0 + j * groups;
+      use[j] = row < rows && (!targets.p || targets.at(row) != targets.ignore);
     }
-  } else {
-    const int64_t waves = (int64_t)gridDim.x * 4;
-    for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += waves)
-      for (int c = lane; c < dim; c += 64) see(fabsf(src[row * ld + c]), row);
+    for (int c = lane * V; c < dim; c += lanes * V) {
+      Vec v[kRows];
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        const int64_t row = min(r0 + j * groups, rows - 1);
+        v[j] = *reinterpret_cast<const Vec*>(src + row * ld + c);
+      }
+#pragma unroll
+      for (int j = 0; j < kRows; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float x = fabsf(v[j].v[e]);
+          if (use[j] && x < INFINITY) top = fmaxf(top, x);
+        }
+    }
   }
 #pragma unroll
   for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-  if (lane == 0) lds[threadIdx.x >> 6] = top;
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = top;
   __syncthreads();
   if (threadIdx.x == 0) largest[blockIdx.x] = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
 }
@@ -165,11 +169,20 @@ __device__ __forceinline__ int from_first(int64_t target, int64_t base, int firs
   return d >= 0 && d < wave_m ? d : -1;
 }
 
+// (x, sum) of a set from its largest and the sum that the fma formed; of nothing, (-inf, 0).
+__device__ __forceinline__ float2 pair_of(float x, float scale, float sum) {
+  return make_float2(x, x == -INFINITY ? 0.0f : settled(x, scale, sum));
+}
+
+// What a sum under x weighs under x_all >= x.
+__device__ __forceinline__ float weight(float x, float x_all, float scale) {
+  return x == x_all ? 1.0f : __builtin_amdgcn_exp2f((x - x_all) * scale);
+}
+
 // ------------------------------------------------------------------ forward
 // The logits of a tile (vocabulary m x rows n), reduced to one pair per row:
-// stats[tile * rows + row] = (max, sum of 2^(s log2 e - max)), max the largest
-// s log2 e rounded to fp32 (the exponents are formed from the unrounded product).
-// The tile that holds a row's target also writes its dot product.
+// stats[tile * rows + row] = (x, sum), see settled().  The tile that holds a row's
+// target also writes its dot product, upright.
 template <class S, typename T>
 __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, Operand features, int dim,
                                                                  int products, float logit_scale2,
@@ -184,12 +197,11 @@ __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, 
   gs_tile::product<S, T, true, true>(acc, table, features, m0, n0, 0, dim, products, nullptr, lds);
 
   float scale2 = scale_of(logit_scale2, units);
-  const bool flip = scale2 < 0.0f;
   const int lane = threadIdx.x & 63;
   const int wm = gs_tile::wave_m<S>(), wn = gs_tile::wave_n<S>();
   float2* red = reinterpret_cast<float2*>(lds);  // [kWavesM][BN]
   // under a negative scale the dot products change their signs first
-  if (flip) {
+  if (scale2 < 0.0f) {
     scale2 = -scale2;
 #pragma unroll
     for (int a = 0; a < S::kMB; ++a)
@@ -212,7 +224,7 @@ __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, 
             label = acc.c[a][b][e];
             mine = true;
           }
-      if (mine) label_dot[n] = flip ? -label : label;
+      if (mine) label_dot[n] = label;
     }
     if (m0 + S::BM > table.extent) {
 #pragma unroll
@@ -238,7 +250,7 @@ __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, 
         sum[e & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[a][b][e], scale2, -ref));
     float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     all += __shfl_xor(all, 32);
-    if (lane < 32) red[(wm / S::kWaveM) * S::BN + wn + 32 * b + lane] = make_float2(top, all);
+    if (lane < 32) red[(wm / S::kWaveM) * S::BN + wn + 32 * b + lane] = pair_of(raw, scale2, all);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < S::BN; i += S::kThreads) {
@@ -247,9 +259,9 @@ __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, 
 #pragma unroll
     for (int w = 1; w < S::kWavesM; ++w) {
       const float2 o = red[w * S::BN + i];
-      const float top = fmaxf(r.x, o.x), ref = top == -INFINITY ? 0.0f : top;
-      r.y = r.y * __builtin_amdgcn_exp2f(r.x - ref) + o.y * __builtin_amdgcn_exp2f(o.x - ref);
-      r.x = top;
+      const float x = fmaxf(r.x, o.x);
+      r.y = r.y * weight(r.x, x, scale2) + o.y * weight(o.x, x, scale2);
+      r.x = x;
     }
     stats[(int64_t)tile.m * features.extent + n0 + i] = r;
   }
@@ -286,9 +298,9 @@ __device__ __forceinline__ void write_total(Sum s, int reduction, float* loss, i
 }
 
 // Joins the tiles' pairs of each row (kLanes lanes a row, in a fixed order):
-// norm = (maximum, 1 / sum, the label's dot product), from which the backward forms the probabilities
-// 2^(s log2 e - maximum) / sum to fp32's relative precision, and the loss; ignored rows give 0, targets outside the
-// vocabulary NaN.  The block's sum goes to partial[block], or, when there is one block in all, to the result.
+// norm = (x, 1 / sum, the label's dot product) for the backward, and the loss;
+// ignored rows give 0, targets outside the vocabulary NaN.  With a reduction the
+// block's sum goes to partial[block], or, when there is one block in all, to the result.
 template <int kLanes>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float2* __restrict__ stats,
                                                             const float* __restrict__ label_dot, int rows,
@@ -302,12 +314,13 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float2* __rest
   const int sub = threadIdx.x % kLanes;
   const int64_t row = (int64_t)blockIdx.x * (kJoinThreads / kLanes) + threadIdx.x / kLanes;
   // the sum in 64 bits: tiles far below a row's maximum count, however many they are
-  float top = -INFINITY;
+  const float scale = fabsf(scale_of(logit_scale2, units));
+  float x = -INFINITY;
   double sum = 0.0;
-  auto add = [&](float otop, double osum) {
-    const float m = fmaxf(top, otop), ref = m == -INFINITY ? 0.0f : m;
-    sum = sum * (double)__builtin_amdgcn_exp2f(top - ref) + osum * (double)__builtin_amdgcn_exp2f(otop - ref);
-    top = m;
+  auto add = [&](float ox, double osum) {
+    const float all = fmaxf(x, ox);
+    sum = sum * (double)weight(x, all, scale) + osum * (double)weight(ox, all, scale);
+    x = all;
   };
   if (row < rows) {
     for (int t = sub; t < tiles; t += kLanes) {
@@ -316,21 +329,20 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float2* __rest
     }
   }
 #pragma unroll
-  for (int off = kLanes / 2; off; off >>= 1) add(__shfl_xor(top, off), __shfl_xor(sum, off));
+  for (int off = kLanes / 2; off; off >>= 1) add(__shfl_xor(x, off), __shfl_xor(sum, off));
   Sum mine = {0.0, 0};
   if (row < rows && sub == 0) {
     const int64_t t = targets.at(row);
     float value = 0.0f;
     if (t != targets.ignore) {
-      // in 64 bits, the maximum kept apart: small losses do not drown in the logits' size
-      value = t >= 0 && t < vocab
-                  ? (float)(log(sum) + kLn2 * ((double)top - (double)label_dot[row] * (double)scale_of(logit_scale2, units)))
-                  : __builtin_nanf("");
+      value = t >= 0 && t < vocab ? (float)(log(sum) + kLn2 * (double)scale * ((double)x - (double)label_dot[row]))
+                                  : __builtin_nanf("");
       mine = {(double)value, 1};
     }
-    if (norm) norm[row] = make_float4(top, (float)(1.0 / sum), label_dot[row], 0.0f);
+    if (norm) norm[row] = make_float4(x, (float)(1.0 / sum), label_dot[row], 0.0f);
     if (loss_rows) loss_rows[row] = value;
   }
+  if (reduction == GS_REDUCE_NONE) return;
   const Sum s = block_sum(mine, lds);
   if (threadIdx.x == 0) {
     if (last) write_total(s, reduction, loss, count);
@@ -376,7 +388,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const float* __restrict__ gra
                                                    float logit_scale2, const float* __restrict__ units,
                                                    float held_scale, const float* __restrict__ largest, int largest_n,
                                                    RowInfo* __restrict__ info, uint64_t* __restrict__ counts,
-                                                   float* __restrict__ label_dot, float* __restrict__ alpha) {
+                                                   float* __restrict__ alpha) {
   __shared__ float lds[4];
   const int lane = threadIdx.x & 63;
   float G = 1.0f;
@@ -400,14 +412,14 @@ __global__ __launch_bounds__(256) void rows_kernel(const float* __restrict__ gra
     if (use) {
       const bool in = t >= 0 && t < vocab;
       const float f = (reduction == GS_REDUCE_NONE ? grad[row] / G : 1.0f) * (in ? held_scale : __builtin_nanf(""));
-      r.top = z.x;
-      r.share = f * z.y;
-      const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(z.z, scale_of(logit_scale2, units), -z.x));
-      r.label = __builtin_fmaf(e, r.share, -f);
+      const float scale = fabsf(scale_of(logit_scale2, units));
+      r.top = z.x * scale;
+      const float off = __builtin_fmaf(z.x, scale, -r.top);
+      r.share = f * z.y * (1.0f - off * kLn2f);
+      r.label = (weight(z.z, z.x, scale) * z.y - 1.0f) * f;
       r.target = in ? (int)t : -1;
     }
     info[row] = r;
-    label_dot[row] = z.z;
   }
   const uint64_t bits = __ballot(use);
   if (lane == 0 && row < rows) counts[row / 64] = bits;
@@ -657,9 +669,12 @@ struct Layouts {
   void measure(const Problem& p, Targets targets, hipStream_t s) const {
     if (!units) return;
     auto one = [&](const void* src, int64_t ld, int64_t rows, Targets t, float* to) {
-      const bool flat = ld == p.dim && rows * p.dim % 4 == 0 && (uintptr_t)src % 16 == 0;
-      const int blocks = (int)min(ceil_div(rows * p.dim, 4096), (int64_t)kLargestBlocks);
-      magnitude_kernel<<<blocks, 256, 0, s>>>((const float*)src, ld, rows, p.dim, flat, t, to);
+      const int V = p.dim % 4 == 0 && ld % 4 == 0 && (uintptr_t)src % 16 == 0 ? 4 : 1;
+      int lanes = 1;
+      while (lanes < 64 && lanes * V < p.dim) lanes *= 2;
+      const int blocks = (int)min(ceil_div(rows, 8 * (256 / lanes)), (int64_t)kLargestBlocks);
+      auto* kernel = V == 4 ? magnitude_kernel<4> : magnitude_kernel<1>;
+      kernel<<<blocks, 256, 0, s>>>((const float*)src, ld, rows, p.dim, lanes, t, to);
       return blocks;
     };
     const int features_n = one(p.features, p.ld_features, p.rows, targets, largest);
@@ -675,7 +690,11 @@ struct Layouts {
 };
 
 // Short rows: the kernels that hold one operand in registers (gs_resident.h).
+// The forward alone needs fewer of them, and goes twice as far.
 static bool resident(const Problem& p) { return p.dp() <= (p.dtype == GS_FP32 ? 64 : 128); }
+static bool resident_forward(const Problem& p) { return p.dp() <= (p.dtype == GS_FP32 ? 128 : 256); }
+// Two workgroups of a forward on rows of one or two 128-byte blocks (counting planes) share a CU, else one has it.
+static int resident_forward_slots(const Problem& p) { return ceil_div(p.dp(), 64) * p.planes() <= 2 ? 512 : 256; }
 
 // Parts along the streamed operand for `slots` workgroups at a time: whole rounds
 // of the chip, each a part's tiles and about six tiles' time to begin and end;
@@ -704,14 +723,19 @@ static int32_t part_rows(int64_t stream, int64_t parts) {
 template <typename T, int kKind>
 static void launch_resident(const Problem& p, const gs_resident::Args& a, int parts, hipStream_t s) {
   const dim3 grid((unsigned)ceil_div(a.held.extent, gs_resident::kHeldRows), (unsigned)parts);
+  auto launch = [&](auto* kernel) { kernel<<<grid, gs_resident::kThreads, 0, s>>>(a); };
+  constexpr bool kForward = kKind == gs_resident::kForward;
   if constexpr (std::is_same<T, _Float16>::value) {
     if (p.dtype == GS_FP32) {
-      gs_resident::resident_kernel<T, 1, gs_tile::kSplitPlanes, kKind><<<grid, gs_resident::kThreads, 0, s>>>(a);
-      return;
+      if constexpr (kForward)
+        if (a.dim > 64) return launch(gs_resident::resident_kernel<T, 2, gs_tile::kSplitPlanes, kKind>);
+      return launch(gs_resident::resident_kernel<T, 1, gs_tile::kSplitPlanes, kKind>);
     }
   }
-  if (a.dim <= 64) gs_resident::resident_kernel<T, 1, 1, kKind><<<grid, gs_resident::kThreads, 0, s>>>(a);
-  else gs_resident::resident_kernel<T, 2, 1, kKind><<<grid, gs_resident::kThreads, 0, s>>>(a);
+  if constexpr (kForward)
+    if (a.dim > 128) return launch(gs_resident::resident_kernel<T, 4, 1, kKind>);
+  if (a.dim <= 64) launch(gs_resident::resident_kernel<T, 1, 1, kKind>);
+  else launch(gs_resident::resident_kernel<T, 2, 1, kKind>);
 }
 
 // Big or Mid tiles for a product of M x N (parts: copies of it side by side):
@@ -742,11 +766,10 @@ struct ForwardPlan {
   size_t bytes;
 
   ForwardPlan(const Problem& p, void* ws) {
-    shape = p.rows <= 32 ? kThin32 : p.rows <= 64 ? kThin64 : resident(p) ? kResident
+    shape = p.rows <= 32 ? kThin32 : p.rows <= 64 ? kThin64 : resident_forward(p) ? kResident
             : takes_big(p.vocab, p.rows) ? kBig : kMid;
     const int bm = shape == kBig ? Big::BM : shape == kMid ? Mid::BM : Thin32::BM;
-    // (two of its workgroups share a CU)
-    tiles_m = shape == kResident ? resident_parts(p.rows, p.vocab, 512, 0.0) : ceil_div(p.vocab, bm);
+    tiles_m = shape == kResident ? resident_parts(p.rows, p.vocab, resident_forward_slots(p), 0.0) : ceil_div(p.vocab, bm);
     rows_piece = max((int64_t)256, kStatBytes / (tiles_m * (int64_t)sizeof(float2)) / 256 * 256);
     rows_piece = min(p.rows, min(rows_piece, (int64_t)1 << 20));
     lanes = p.rows <= 4096 ? 64 : 1;
@@ -810,7 +833,7 @@ static int forward(const Problem& p, Targets targets, float logit_scale, int red
                                                    f.partial + block, f.blocks == 1, loss, count);
     block += blocks;
   }
-  if (f.blocks > 1) total_kernel<<<1, kJoinThreads, 0, s>>>(f.partial, f.blocks, reduction, loss, count);
+  if (f.blocks > 1 && reduction != GS_REDUCE_NONE) total_kernel<<<1, kJoinThreads, 0, s>>>(f.partial, f.blocks, reduction, loss, count);
   return gs_status_from_hip(hipGetLastError());
 }
 
@@ -849,7 +872,7 @@ struct BackwardPlan {
   Layouts layouts;
   uint16_t* ds;
   RowInfo* info;
-  float *label_dot, *alpha, *largest, *part_h, *part_t;
+  float *alpha, *largest, *part_h, *part_t;
   uint64_t* counts;
   size_t bytes;
 
@@ -888,7 +911,6 @@ struct BackwardPlan {
     layouts = Layouts(p, rows_piece, c);
     ds = c.take<uint16_t>(rows_piece * ld * p.ds_planes());
     info = c.take<RowInfo>(p.rows);
-    label_dot = c.take<float>(p.rows);
     counts = c.take<uint64_t>(ceil_div(p.rows, 64));
     alpha = c.take<float>(1);
     largest = c.take<float>(kLargestBlocks);
@@ -915,7 +937,7 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
   const float *unit_h = b.layouts.features_unit(), *unit_w = b.layouts.table_unit();
   rows_kernel<<<(unsigned)ceil_div(p.rows, 256), 256, 0, s>>>(grad_loss, p.rows, p.vocab, targets, reduction, count, norm,
                                                               logit_scale, scale2, b.layouts.units, Held<T>::kScale,
-                                                              b.largest, largest_n, b.info, b.counts, b.label_dot, b.alpha);
+                                                              b.largest, largest_n, b.info, b.counts, b.alpha);
   const Operand table = b.layouts.table(p, s);
   if (resident(p)) {
     const Operand features = b.layouts.features(p, 0, p.rows, s);
@@ -923,7 +945,6 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
     a.dim = (int32_t)p.dp();
     a.logit_scale2 = scale2;
     a.units = b.layouts.units;
-    a.label_dot = b.label_dot;
     a.info = b.info;
     a.counts = b.counts;
     a.alpha = b.alpha;
@@ -1044,6 +1065,7 @@ extern "C" int gs_xent_fwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dty
   if (rows > 0 && (!workspace || workspace_bytes < gs_xent::ForwardPlan(p, nullptr).bytes)) return GS_ERR_SCRATCH_TOO_SMALL;
   hipStream_t s = (hipStream_t)stream;
   if (rows == 0) {
+    if (reduction == GS_REDUCE_NONE) return GS_OK;
     gs_xent::total_kernel<<<1, gs_xent::kJoinThreads, 0, s>>>(nullptr, 0, reduction, loss, count);
     return gs_status_from_hip(hipGetLastError());
   }

@@ -606,7 +606,7 @@ int gs_embed_bwd(int64_t n, int32_t vocab, int32_t dim, int32_t dtype, const voi
  * loss: `rows` fp32 for GS_REDUCE_NONE, else one (the sum, or the mean over
  * the rows that count; over none, NaN).  norm (4 fp32 a row, 16-byte aligned;
  * NULL if no backward follows) receives what gs_xent_bwd needs of the row's
- * softmax, count the number of rows that count.  features and table must be 16-byte
+ * softmax; count, but for GS_REDUCE_NONE, the number of rows that count, which gs_xent_bwd takes too.  features and table must be 16-byte
  * aligned unless they are fp32 or have a dim or row distance that is not a
  * multiple of 8 (those are laid out in the workspace first).  workspace:
  * gs_xent_fwd_workspace_bytes bytes on 256, of any content.

@@ -193,6 +193,44 @@ def test_entropy_scales(device, dtype, logit_scale):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,dim", [(200, 1, 16), (200, 2, 16), (300, 3, 128), (100, 65, 24), (90, 67, 256),
+                                            (70, 66, 192), (600, 700, 64), (513, 1025, 60), (66, 5, 130), (1, 900, 64)])
+def test_entropy_few_classes_and_short_rows(device, dtype, rows, vocab, dim):
+    print(f"entropy {dtype} rows={rows} vocab={vocab} dim={dim}", flush=True)
+    features, table, targets, gen = _problem(device, dtype, rows, vocab, dim, ignored=0.1 if rows > 1 else 0.0)
+    for reduction, logit_scale in (("mean", 1.0), ("none", -1.5)):
+        up = torch.rand(rows, generator=gen).to(device) if reduction == "none" else torch.tensor(1.0, device=device)
+        _compare(features, table, targets, up, reduction=reduction, logit_scale=logit_scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,dim", [(3, 100, 64), (200, 100, 64), (200, 300, 128), (200, 300, 320)])
+def test_entropy_of_certain_labels(device, dtype, rows, vocab, dim):
+    """Labels of all but probability 1 (everything else together below 2^-26): the largest of a
+    row counts as exactly 1, so a loss and a gradient may be lost, but nothing larger takes their place."""
+    gen = _gen(rows + dim)
+    table = (torch.randn(vocab, dim, generator=gen) / math.sqrt(dim)).to(device, dtype)
+    targets = torch.randint(0, vocab, (rows,), generator=gen).to(device)
+    h = 60.0 * table[targets].float() / table[targets].float().square().sum(1, keepdim=True)
+    features = h.to(dtype).requires_grad_(True)
+    leaf = table.clone().requires_grad_(True)
+    loss = vocabulary.linear_cross_entropy(features, leaf, targets, reduction="none", logit_scale=1.3)
+    s = 1.3 * (features.detach().double() @ table.double().T)
+    rest = torch.softmax(s, 1)
+    rest[torch.arange(rows, device=device), targets] = 0.0
+    rest = rest.sum(1)
+    assert float(rest.max()) < 2.0 ** -26
+    exact = torch.log1p(rest)
+    assert bool((loss >= 0).all()) and bool(((loss.double() - exact).abs() <= exact * 1.01).all())
+    grads = torch.autograd.grad(loss, (features, leaf), torch.ones_like(loss))
+    # each row's ds has 1-norm 2 rest
+    bound = 1.3 * 2 * rest.unsqueeze(1) * table.double().abs().amax() * 1.01 + ref.TINY[dtype]
+    assert bool((grads[0].double().abs() <= bound).all())
+    bound = 1.3 * 2 * rest.sum() * features.detach().double().abs().amax() * 1.01 + ref.TINY[dtype]
+    assert bool((grads[1].double().abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_entropy_ignored_rows_hold_anything(device, dtype):
     """NaN, infinities and the type's largest values in rows that do not count."""
     features, table, targets, gen = _problem(device, dtype, 333, 150, 72, ignored=0.4)
