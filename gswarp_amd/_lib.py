@@ -103,6 +103,7 @@ SIGNATURES = {
     "gs_embed_bwd_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
     "gs_embed_bwd": (
         ctypes.c_int, [_i64, _i32, _i32, _i32, _vp, _i32, _vp, _f32, _i64, _vp, _vp, _sz, _vp]),
+    "gs_xent_state_bytes": (_sz, [_i64, _i32, _i32, _i32, _i64, _i64]),
     "gs_xent_fwd_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i64, _i64]),
     "gs_xent_fwd": (
         ctypes.c_int,

@@ -58,36 +58,50 @@ struct Held<_Float16> {
 };
 
 // ------------------------------------------------------------------ packing
-// fp32: the largest finite magnitude of a matrix, one value a block (targets.p:
-// of the rows that count only, so that what ignored rows hold does not reach the
-// unit of the others).  A group of `lanes` lanes reads a row, V values a lane at a time.
+// A matrix and where its layout for the tile loads goes: rows of dp = ceil(dim /
+// 8) * 8 16-bit values, zero past dim, from dst (null: it is read in place);
+// fp32 as the planes hi and lo of value / unit, `plane` apart.  Only for fp32 and
+// for rows that the 16-byte loads cannot take (dim or ld not a multiple of 8).
+struct Matrix {
+  const void* src;
+  int64_t ld, rows;
+  uint16_t* dst;
+  int64_t plane;
+};
+
+// fp32: the largest finite magnitudes of the features (of the rows that count
+// only, so that what ignored rows hold does not reach the unit of the others) and
+// of the table, one value a block, the features' blocks first.  A group of
+// `lanes` lanes reads a row, V values a lane at a time.
 constexpr int kLargestBlocks = 1024;
 template <int V>
-__global__ __launch_bounds__(256) void magnitude_kernel(const float* __restrict__ src, int64_t ld, int64_t rows,
-                                                        int dim, int lanes, Targets targets,
-                                                        float* __restrict__ largest) {
+__global__ __launch_bounds__(256) void magnitude_kernel(Matrix features, int features_blocks, Matrix table, int dim,
+                                                        int lanes, Targets targets, float* __restrict__ largest) {
   __shared__ float lds[4];
   struct __attribute__((aligned(4 * V))) Vec {
     float v[V];
   };
   constexpr int kRows = 8;  // rows in flight
+  const bool of_table = (int)blockIdx.x >= features_blocks;
+  const Matrix m = of_table ? table : features;
+  const float* src = (const float*)m.src;
+  const int block = of_table ? blockIdx.x - features_blocks : blockIdx.x;
+  const int blocks = of_table ? gridDim.x - features_blocks : features_blocks;
   const int lane = threadIdx.x % lanes;
-  const int64_t groups = (int64_t)gridDim.x * (256 / lanes);
+  const int64_t groups = (int64_t)blocks * (256 / lanes);
   float top = 0.0f;
-  for (int64_t r0 = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes; r0 < rows; r0 += groups * kRows) {
+  for (int64_t r0 = (int64_t)block * (256 / lanes) + threadIdx.x / lanes; r0 < m.rows; r0 += groups * kRows) {
     bool use[kRows];
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
       const int64_t row = r0 + j * groups;
-      use[j] = row < rows && (!targets.p || targets.at(row) != targets.ignore);
+      use[j] = row < m.rows && (of_table || targets.at(row) != targets.ignore);
     }
     for (int c = lane * V; c < dim; c += lanes * V) {
       Vec v[kRows];
 #pragma unroll
-      for (int j = 0; j < kRows; ++j) {
-        const int64_t row = min(r0 + j * groups, rows - 1);
-        v[j] = *reinterpret_cast<const Vec*>(src + row * ld + c);
-      }
+      for (int j = 0; j < kRows; ++j)
+        v[j] = *reinterpret_cast<const Vec*>(src + min(r0 + j * groups, m.rows - 1) * m.ld + c);
 #pragma unroll
       for (int j = 0; j < kRows; ++j)
 #pragma unroll
@@ -104,39 +118,46 @@ __global__ __launch_bounds__(256) void magnitude_kernel(const float* __restrict_
   if (threadIdx.x == 0) largest[blockIdx.x] = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
 }
 
-// units[b] for matrix b: the power of two 2^e that brings its largest magnitude
-// (the maximum of largest[b kLargestBlocks ..]) to [2^13, 2^14).
-__global__ __launch_bounds__(256) void units_kernel(const float* __restrict__ largest, int features_n, int table_n,
-                                                    float* __restrict__ units) {
+// The unit of a matrix from its blocks' magnitudes: the power of two 2^e that
+// brings the largest to [2^13, 2^14).
+__device__ __forceinline__ float unit_of(const float* __restrict__ largest, int n) {
   __shared__ float lds[4];
-  const int n = blockIdx.x == 0 ? features_n : table_n;
   float top = 0.0f;
-  for (int i = threadIdx.x; i < n; i += 256) top = fmaxf(top, largest[blockIdx.x * kLargestBlocks + i]);
+  for (int i = threadIdx.x; i < n; i += 256) top = fmaxf(top, largest[i]);
 #pragma unroll
   for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = top;
   __syncthreads();
-  if (threadIdx.x > 0) return;
   top = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
   int e = 14;
   if (top > 0.0f) frexpf(top, &e);
-  units[blockIdx.x] = ldexpf(1.0f, max(e - 14, -126));
+  return ldexpf(1.0f, max(e - 14, -126));
 }
 
-// A matrix laid out for the tile loads: rows of dp = ceil(dim / 8) * 8 16-bit
-// values, zero past dim; fp32 as the planes hi and lo of value / unit.  Only for
-// fp32 and for rows that the 16-byte loads cannot take (dim or ld not a multiple of 8).
+// Lays two matrices out, the first's blocks first; fp32: their units, from
+// largest (the first's magnitudes, then the second's), go to units[0] and units[1].
 template <typename T>
-__global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, int64_t ld, int64_t rows, int dim,
-                                                   int dp, uint16_t* __restrict__ dst, int64_t plane,
-                                                   const float* __restrict__ unit) {
-  const float scale = unit ? 1.0f / *unit : 1.0f;
-  const int64_t total = rows * (dp / 8);
-  for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < total; v += (int64_t)gridDim.x * 256) {
-    const int64_t row = v / (dp / 8);
-    const int col = (int)(v - row * (dp / 8)) * 8;
-    const T* s = src + row * ld + col;
-    uint16_t* d = dst + row * dp + col;
+__global__ __launch_bounds__(256) void layout_kernel(Matrix first, int first_blocks, Matrix second, int dim, int dp,
+                                                     const float* __restrict__ largest, int first_n, int second_n,
+                                                     float* __restrict__ units) {
+  const bool other = (int)blockIdx.x >= first_blocks;
+  const Matrix m = other ? second : first;
+  const int block = other ? blockIdx.x - first_blocks : blockIdx.x;
+  const int blocks = other ? gridDim.x - first_blocks : first_blocks;
+  float scale = 1.0f;
+  if constexpr (sizeof(T) == 4) {
+    const float unit = unit_of(largest + (other ? first_n : 0), other ? second_n : first_n);
+    if (block == 0 && threadIdx.x == 0) units[other] = unit;
+    scale = 1.0f / unit;
+  }
+  const T* src = (const T*)m.src;
+  const uint32_t vectors = dp / 8;
+  const int64_t total = m.rows * vectors;
+  for (int64_t v = (int64_t)block * 256 + threadIdx.x; v < total; v += (int64_t)blocks * 256) {
+    const int64_t row = v / vectors;
+    const int col = (int)(v - row * vectors) * 8;
+    const T* s = src + row * m.ld + col;
+    uint16_t* d = m.dst + row * dp + col;
     if constexpr (sizeof(T) == 4) {
       gs_tile::f16x8 hi, lo;
 #pragma unroll
@@ -147,7 +168,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, in
         lo[e] = fabsf(x) < INFINITY ? (_Float16)((x - (float)hi[e]) * gs_tile::kPlaneStep) : (_Float16)0.0f;
       }
       *reinterpret_cast<gs_tile::f16x8*>(d) = hi;
-      *reinterpret_cast<gs_tile::f16x8*>(d + plane) = lo;
+      *reinterpret_cast<gs_tile::f16x8*>(d + m.plane) = lo;
     } else {
       uint16_t out[8];
 #pragma unroll
@@ -575,17 +596,31 @@ __global__ __launch_bounds__(S::kThreads) void grad_kernel(Operand x, Operand ds
   }
 }
 
-// out = alpha (and x's unit) * sum of the planes; counts (dh): rows that do not count are zero.
-template <typename Out>
+// out = alpha (and x's unit) * sum of the planes; counts (dh): rows that do not
+// count are zero.  kGroups threads share an element's planes, their sums joined in
+// order.
+template <int kGroups, typename Out>
 __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ part, int planes, int64_t plane,
                                                      int64_t n, int D, const uint64_t* __restrict__ counts,
                                                      const float* __restrict__ alpha, const float* __restrict__ unit,
                                                      Out* __restrict__ out) {
+  constexpr int kElements = 256 / kGroups;
+  __shared__ float lds[256];
   const float al = unit ? *alpha * *unit : *alpha;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+  const int element = threadIdx.x % kElements, group = threadIdx.x / kElements;
+  for (int64_t i0 = (int64_t)blockIdx.x * kElements; i0 < n; i0 += (int64_t)gridDim.x * kElements) {
+    const int64_t i = i0 + element;
     float s = 0.0f;
-    for (int p = 0; p < planes; ++p) s += part[(int64_t)p * plane + i];
-    out[i] = (Out)(!counts || row_counts(counts, i / D) ? s * al : 0.0f);
+    if (i < n)
+      for (int p = group; p < planes; p += kGroups) s += part[(int64_t)p * plane + i];
+    if (kGroups > 1) {
+      __syncthreads();
+      lds[threadIdx.x] = s;
+      __syncthreads();
+      if (group > 0) continue;
+      for (int g = 1; g < kGroups; ++g) s += lds[g * kElements + element];
+    }
+    if (i < n) out[i] = (Out)(!counts || row_counts(counts, i / D) ? s * al : 0.0f);
   }
 }
 
@@ -636,56 +671,75 @@ static int check_pointers(const Problem& p) {
   return GS_OK;
 }
 
-// The operand of `rows` rows from row `first` of a matrix: in place, or laid out in space.
-static Operand operand(const Problem& p, const void* src, int64_t ld, int64_t first, int64_t rows, uint16_t* space,
-                       const float* unit, hipStream_t s) {
-  const char* at = (const char*)src + first * ld * (int64_t)p.element();
-  if (!p.packs(ld)) return {(const uint16_t*)at, ld, 0, (int32_t)rows};
-  const int64_t plane = rows * p.dp();
-  const int blocks = (int)min(ceil_div(plane / 8, 256), (int64_t)8192);
-  if (p.dtype == GS_FP32)
-    pack_kernel<<<blocks, 256, 0, s>>>((const float*)at, ld, rows, p.dim, (int)p.dp(), space, plane, unit);
-  else
-    pack_kernel<<<blocks, 256, 0, s>>>((const _Float16*)at, ld, rows, p.dim, (int)p.dp(), space, plane, nullptr);
-  return {space, p.dp(), plane, (int32_t)rows};
-}
-
-// Both matrices' layouts for the tile loads, where they need one, and (fp32, else null) their units.
+// Both matrices as the kernels read them: in place, or laid out (struct Matrix).
+// The layouts of a forward whose backward may follow are of all rows and go to its
+// state, where the backward finds them; else the features are laid out a piece
+// of the rows at a time, in the workspace.
 struct Layouts {
   uint16_t *features_space, *table_space;
   float *units, *largest;
+  int64_t rows;  // that features_space holds
+  int features_n, table_n;
+
   Layouts() = default;
-  Layouts(const Problem& p, int64_t rows_piece, Carve& c) {
+  Layouts(const Problem& p, int64_t rows_held, Carve& c) : rows(rows_held), features_n(0), table_n(0) {
     const bool fp32 = p.dtype == GS_FP32;
-    features_space = c.take<uint16_t>(p.packs(p.ld_features) ? rows_piece * p.dp() * p.planes() : 0);
+    features_space = c.take<uint16_t>(p.packs(p.ld_features) ? rows * p.dp() * p.planes() : 0);
     table_space = c.take<uint16_t>(p.packs(p.ld_table) ? p.vocab * p.dp() * p.planes() : 0);
     units = c.take<float>(fp32 ? 2 : 0);
-    largest = c.take<float>(fp32 ? 2 * kLargestBlocks : 0);
     if (!fp32) units = nullptr;
   }
   const float* features_unit() const { return units; }
   const float* table_unit() const { return units ? units + 1 : nullptr; }
-  // fp32: the units, from the matrices' magnitudes
-  void measure(const Problem& p, Targets targets, hipStream_t s) const {
-    if (!units) return;
-    auto one = [&](const void* src, int64_t ld, int64_t rows, Targets t, float* to) {
-      const int V = p.dim % 4 == 0 && ld % 4 == 0 && (uintptr_t)src % 16 == 0 ? 4 : 1;
+
+  // Lays out the table and, where all rows are held, the features.
+  void prepare(const Problem& p, Targets targets, hipStream_t s) {
+    const Matrix f = {p.features, p.ld_features, p.rows, features_space, rows * p.dp()};
+    const Matrix t = {p.table, p.ld_table, p.vocab, table_space, p.vocab * p.dp()};
+    if (units) {
+      auto fits = [](const Matrix& m) { return m.ld % 4 == 0 && (uintptr_t)m.src % 16 == 0; };
+      const int V = p.dim % 4 == 0 && fits(f) && fits(t) ? 4 : 1;
       int lanes = 1;
       while (lanes < 64 && lanes * V < p.dim) lanes *= 2;
-      const int blocks = (int)min(ceil_div(rows, 8 * (256 / lanes)), (int64_t)kLargestBlocks);
+      auto blocks = [&](int64_t n) { return (int)min(ceil_div(n, 8 * (256 / lanes)), (int64_t)kLargestBlocks); };
+      features_n = blocks(p.rows);
+      table_n = blocks(p.vocab);
       auto* kernel = V == 4 ? magnitude_kernel<4> : magnitude_kernel<1>;
-      kernel<<<blocks, 256, 0, s>>>((const float*)src, ld, rows, p.dim, lanes, t, to);
-      return blocks;
-    };
-    const int features_n = one(p.features, p.ld_features, p.rows, targets, largest);
-    const int table_n = one(p.table, p.ld_table, p.vocab, {nullptr, 64, 0}, largest + kLargestBlocks);
-    units_kernel<<<2, 256, 0, s>>>(largest, features_n, table_n, units);
+      kernel<<<features_n + table_n, 256, 0, s>>>(f, features_n, t, p.dim, lanes, targets, largest);
+    }
+    lay_out(p, rows == p.rows && p.packs(p.ld_features) ? f : Matrix{}, p.packs(p.ld_table) ? t : Matrix{}, s);
   }
-  Operand features(const Problem& p, int64_t first, int64_t rows, hipStream_t s) const {
-    return operand(p, p.features, p.ld_features, first, rows, features_space, features_unit(), s);
+  void lay_out(const Problem& p, const Matrix& f, const Matrix& t, hipStream_t s) const {
+    auto blocks = [&](const Matrix& m) { return (int)min(ceil_div(m.rows * (p.dp() / 8), 256), (int64_t)4096); };
+    const int fn = blocks(f), tn = blocks(t);
+    if (fn + tn == 0) return;
+    auto* kernel = p.dtype == GS_FP32 ? layout_kernel<float> : layout_kernel<_Float16>;
+    kernel<<<fn + tn, 256, 0, s>>>(f, fn, t, p.dim, (int)p.dp(), largest, features_n, table_n, units);
   }
-  Operand table(const Problem& p, hipStream_t s) const {
-    return operand(p, p.table, p.ld_table, 0, p.vocab, table_space, table_unit(), s);
+  Operand features(const Problem& p, int64_t first, int64_t n, hipStream_t s) const {
+    const char* at = (const char*)p.features + first * p.ld_features * (int64_t)p.element();
+    if (!p.packs(p.ld_features)) return {(const uint16_t*)at, p.ld_features, 0, (int32_t)n};
+    const int64_t plane = rows * p.dp();
+    if (rows == p.rows) return {features_space + first * p.dp(), p.dp(), plane, (int32_t)n};
+    lay_out(p, {at, p.ld_features, n, features_space, plane}, Matrix{}, s);
+    return {features_space, p.dp(), plane, (int32_t)n};
+  }
+  Operand table(const Problem& p) const {
+    if (!p.packs(p.ld_table)) return {(const uint16_t*)p.table, p.ld_table, 0, p.vocab};
+    return {table_space, p.dp(), p.vocab * p.dp(), p.vocab};
+  }
+};
+
+// What a forward leaves for its backward.
+struct State {
+  float4* norm;  // see join_kernel
+  Layouts layouts;
+  size_t bytes;
+  State(const Problem& p, void* at) {
+    Carve c{(char*)at};
+    norm = c.take<float4>(p.rows);
+    layouts = Layouts(p, p.rows, c);
+    bytes = c.at;
   }
 };
 
@@ -765,7 +819,8 @@ struct ForwardPlan {
   Sum* partial;
   size_t bytes;
 
-  ForwardPlan(const Problem& p, void* ws) {
+  // kept: the layouts lie in a state
+  ForwardPlan(const Problem& p, bool kept, void* ws) {
     shape = p.rows <= 32 ? kThin32 : p.rows <= 64 ? kThin64 : resident_forward(p) ? kResident
             : takes_big(p.vocab, p.rows) ? kBig : kMid;
     const int bm = shape == kBig ? Big::BM : shape == kMid ? Mid::BM : Thin32::BM;
@@ -777,7 +832,8 @@ struct ForwardPlan {
     for (int64_t r = 0; r < p.rows; r += rows_piece)
       blocks += ceil_div(min(rows_piece, p.rows - r), kJoinThreads / lanes);
     Carve c{(char*)ws};
-    layouts = Layouts(p, rows_piece, c);
+    if (!kept) layouts = Layouts(p, rows_piece, c);
+    layouts.largest = c.take<float>(p.dtype == GS_FP32 ? 2 * kLargestBlocks : 0);
     stats = c.take<float2>(tiles_m * rows_piece);
     label = c.take<float>(rows_piece);
     partial = c.take<Sum>(blocks);
@@ -798,8 +854,8 @@ template <typename T>
 static int forward(const Problem& p, Targets targets, float logit_scale, int reduction, float* loss, float4* norm,
                    int64_t* count, ForwardPlan& f, hipStream_t s) {
   const float scale2 = logit_scale * kLog2e;
-  f.layouts.measure(p, targets, s);
-  const Operand table = f.layouts.table(p, s);
+  f.layouts.prepare(p, targets, s);
+  const Operand table = f.layouts.table(p);
   int64_t block = 0;
   for (int64_t r = 0; r < p.rows; r += f.rows_piece) {
     const int64_t rows = min(f.rows_piece, p.rows - r);
@@ -869,7 +925,6 @@ struct BackwardPlan {
   int64_t rows_piece, cols_piece, ld, row_pieces, col_pieces;
   int parts_h, parts_t;  // parts along K of dh and dw
   bool direct_h, direct_t;  // one part and one piece: no fp32 sums in between
-  Layouts layouts;
   uint16_t* ds;
   RowInfo* info;
   float *alpha, *largest, *part_h, *part_t;
@@ -908,7 +963,6 @@ struct BackwardPlan {
     direct_h = parts_h == 1 && col_pieces == 1;
     direct_t = parts_t == 1 && row_pieces == 1;
     Carve c{(char*)ws};
-    layouts = Layouts(p, rows_piece, c);
     ds = c.take<uint16_t>(rows_piece * ld * p.ds_planes());
     info = c.take<RowInfo>(p.rows);
     counts = c.take<uint64_t>(ceil_div(p.rows, 64));
@@ -922,8 +976,16 @@ struct BackwardPlan {
 
 static unsigned finish_blocks(int64_t n) { return (unsigned)min(ceil_div(n, 256), (int64_t)8192); }
 
+template <typename Out>
+static void finish(const float* part, int planes, int64_t plane, int64_t n, int D, const uint64_t* counts,
+                   const float* alpha, const float* unit, Out* out, hipStream_t s) {
+  // many planes of few elements (a small table's) do not fill the chip by their elements alone
+  if (planes >= 16) finish_kernel<8><<<finish_blocks(n * 8), 256, 0, s>>>(part, planes, plane, n, D, counts, alpha, unit, out);
+  else finish_kernel<1><<<finish_blocks(n), 256, 0, s>>>(part, planes, plane, n, D, counts, alpha, unit, out);
+}
+
 template <typename T, typename Out, int kPlanes>
-static int backward(const Problem& p, Targets targets, float logit_scale, int reduction, const float4* norm,
+static int backward(const Problem& p, Targets targets, float logit_scale, int reduction, const State& state,
                     const int64_t* count, const float* grad_loss, Out* grad_features, Out* grad_table,
                     BackwardPlan& b, hipStream_t s) {
   const float scale2 = logit_scale * kLog2e;
@@ -933,18 +995,18 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
     largest_n = (int)min(ceil_div(p.rows, 256), (int64_t)kLargestBlocks);
     largest_kernel<<<largest_n, 256, 0, s>>>(grad_loss, p.rows, targets, b.largest);
   }
-  b.layouts.measure(p, targets, s);
-  const float *unit_h = b.layouts.features_unit(), *unit_w = b.layouts.table_unit();
-  rows_kernel<<<(unsigned)ceil_div(p.rows, 256), 256, 0, s>>>(grad_loss, p.rows, p.vocab, targets, reduction, count, norm,
-                                                              logit_scale, scale2, b.layouts.units, Held<T>::kScale,
+  const Layouts& layouts = state.layouts;
+  const float *unit_h = layouts.features_unit(), *unit_w = layouts.table_unit();
+  rows_kernel<<<(unsigned)ceil_div(p.rows, 256), 256, 0, s>>>(grad_loss, p.rows, p.vocab, targets, reduction, count, state.norm,
+                                                              logit_scale, scale2, layouts.units, Held<T>::kScale,
                                                               b.largest, largest_n, b.info, b.counts, b.alpha);
-  const Operand table = b.layouts.table(p, s);
+  const Operand table = layouts.table(p);
   if (resident(p)) {
-    const Operand features = b.layouts.features(p, 0, p.rows, s);
+    const Operand features = layouts.features(p, 0, p.rows, s);
     gs_resident::Args a = {};
     a.dim = (int32_t)p.dp();
     a.logit_scale2 = scale2;
-    a.units = b.layouts.units;
+    a.units = layouts.units;
     a.info = b.info;
     a.counts = b.counts;
     a.alpha = b.alpha;
@@ -960,8 +1022,7 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
       a.out = out;
       launch_resident<T, decltype(kind)::value>(p, a, parts, s);
       if (parts > 1)
-        finish_kernel<<<finish_blocks(a.part_plane), 256, 0, s>>>(sums, parts, a.part_plane, a.part_plane, D, nullptr,
-                                                                 b.alpha, unit, out);
+        finish(sums, parts, a.part_plane, a.part_plane, D, nullptr, b.alpha, unit, out, s);
     };
     if (grad_features)
       run(std::integral_constant<int, gs_resident::kFeatures>{}, features, table, b.parts_h, b.part_h, unit_w, grad_features);
@@ -971,7 +1032,7 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
   }
   for (int64_t r = 0; r < p.rows; r += b.rows_piece) {
     const int32_t rows = (int32_t)min(b.rows_piece, p.rows - r);
-    const Operand features = b.layouts.features(p, r, rows, s);
+    const Operand features = layouts.features(p, r, rows, s);
     const uint64_t* counts = b.counts + r / 64;
     const int64_t ds_plane = rows * b.ld;
     for (int64_t c = 0; c < p.vocab; c += b.cols_piece) {
@@ -984,7 +1045,7 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
         typedef decltype(shape) S;
         const int tiles_m = (int)ceil_div(cols, S::BM), tiles_n = (int)ceil_div(rows, S::BN);
         logits_bwd_kernel<S, T, kPlanes><<<(unsigned)((int64_t)tiles_m * tiles_n), S::kThreads, 0, s>>>(
-            piece, features, (int)p.dp(), p.products(), scale2, b.layouts.units, (int32_t)c, tiles_m, tiles_n,
+            piece, features, (int)p.dp(), p.products(), scale2, layouts.units, (int32_t)c, tiles_m, tiles_n,
             b.info + r, counts, b.ds, b.ld, ds_plane);
       });
       with_columns(columns_of(D), [&](auto shape) {
@@ -1012,20 +1073,15 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
               x, ds, rows, k_part, p.ds_products(), counts, tiles_m, tiles_n, part, part_plane, r > 0, b.alpha, unit_h,
               grad_table + c * D);
           if (part && b.row_pieces == 1)
-            finish_kernel<<<finish_blocks((int64_t)cols * D), 256, 0, s>>>(
-                part, b.parts_t, part_plane, (int64_t)cols * D, D, nullptr, b.alpha, unit_h, grad_table + c * D);
+            finish(part, b.parts_t, part_plane, (int64_t)cols * D, D, nullptr, b.alpha, unit_h, grad_table + c * D, s);
         }
       });
     }
     if (grad_features && !b.direct_h)
-      finish_kernel<<<finish_blocks((int64_t)rows * D), 256, 0, s>>>(b.part_h, b.parts_h, (int64_t)rows * D,
-                                                                    (int64_t)rows * D, D, counts, b.alpha, unit_w,
-                                                                    grad_features + r * D);
+      finish(b.part_h, b.parts_h, (int64_t)rows * D, (int64_t)rows * D, D, counts, b.alpha, unit_w, grad_features + r * D, s);
   }
   if (grad_table && b.row_pieces > 1)
-    finish_kernel<<<finish_blocks((int64_t)p.vocab * D), 256, 0, s>>>(b.part_t, b.parts_t, (int64_t)p.vocab * D,
-                                                                     (int64_t)p.vocab * D, D, nullptr, b.alpha, unit_h,
-                                                                     grad_table);
+    finish(b.part_t, b.parts_t, (int64_t)p.vocab * D, (int64_t)p.vocab * D, D, nullptr, b.alpha, unit_h, grad_table, s);
   return gs_status_from_hip(hipGetLastError());
 }
 
@@ -1043,17 +1099,24 @@ static bool options_valid(int32_t target_bits, float logit_scale, int32_t reduct
 
 using gs_xent::Problem;
 
+extern "C" size_t gs_xent_state_bytes(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, int64_t ld_features,
+                                      int64_t ld_table) {
+  const Problem p = {rows, vocab, dim, dtype, nullptr, ld_features, nullptr, ld_table};
+  if (gs_xent::check(p) != GS_OK || rows == 0) return 0;
+  return gs_xent::State(p, nullptr).bytes;
+}
+
 extern "C" size_t gs_xent_fwd_workspace_bytes(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype,
                                               int64_t ld_features, int64_t ld_table) {
   const Problem p = {rows, vocab, dim, dtype, nullptr, ld_features, nullptr, ld_table};
   if (gs_xent::check(p) != GS_OK || rows == 0) return 0;
-  return gs_xent::ForwardPlan(p, nullptr).bytes;
+  return gs_xent::ForwardPlan(p, false, nullptr).bytes;
 }
 
 extern "C" int gs_xent_fwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void* features,
                            int64_t ld_features, const void* table, int64_t ld_table, const void* targets,
                            int32_t target_bits, int64_t ignore_index, float logit_scale, int32_t reduction, float* loss,
-                           float* norm, int64_t* count, void* workspace, size_t workspace_bytes, void* stream) {
+                           void* state, int64_t* count, void* workspace, size_t workspace_bytes, void* stream) {
   const Problem p = {rows, vocab, dim, dtype, features, ld_features, table, ld_table};
   int status = gs_xent::check(p);
   if (status != GS_OK) return status;
@@ -1061,18 +1124,27 @@ extern "C" int gs_xent_fwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dty
       (!loss && (rows > 0 || reduction != GS_REDUCE_NONE)))
     return GS_ERR_INVALID_ARGUMENT;
   if ((status = gs_xent::check_pointers(p)) != GS_OK) return status;
-  if (rows > 0 && ((uintptr_t)workspace & 255)) return GS_ERR_MISALIGNED;
-  if (rows > 0 && (!workspace || workspace_bytes < gs_xent::ForwardPlan(p, nullptr).bytes)) return GS_ERR_SCRATCH_TOO_SMALL;
   hipStream_t s = (hipStream_t)stream;
   if (rows == 0) {
     if (reduction == GS_REDUCE_NONE) return GS_OK;
     gs_xent::total_kernel<<<1, gs_xent::kJoinThreads, 0, s>>>(nullptr, 0, reduction, loss, count);
     return gs_status_from_hip(hipGetLastError());
   }
-  gs_xent::ForwardPlan f(p, workspace);
+  if (((uintptr_t)workspace & 255) || ((uintptr_t)state & 255)) return GS_ERR_MISALIGNED;
+  if (!workspace || workspace_bytes < gs_xent::ForwardPlan(p, state != nullptr, nullptr).bytes)
+    return GS_ERR_SCRATCH_TOO_SMALL;
+  gs_xent::ForwardPlan f(p, state != nullptr, workspace);
+  float4* norm = nullptr;
+  if (state) {
+    const gs_xent::State kept(p, state);
+    float* largest = f.layouts.largest;
+    f.layouts = kept.layouts;
+    f.layouts.largest = largest;
+    norm = kept.norm;
+  }
   const gs_xent::Targets t = {targets, target_bits, ignore_index};
   auto* run = dtype == GS_BF16 ? gs_xent::forward<__bf16> : gs_xent::forward<_Float16>;  // fp32: planes of fp16
-  return run(p, t, logit_scale, reduction, loss, (float4*)norm, count, f, s);
+  return run(p, t, logit_scale, reduction, loss, norm, count, f, s);
 }
 
 extern "C" size_t gs_xent_bwd_workspace_bytes(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype,
@@ -1086,7 +1158,7 @@ extern "C" size_t gs_xent_bwd_workspace_bytes(int64_t rows, int32_t vocab, int32
 extern "C" int gs_xent_bwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void* features,
                            int64_t ld_features, const void* table, int64_t ld_table, const void* targets,
                            int32_t target_bits, int64_t ignore_index, float logit_scale, int32_t reduction,
-                           const float* norm, const int64_t* count, const float* grad_loss, void* grad_features,
+                           const void* state, const int64_t* count, const float* grad_loss, void* grad_features,
                            void* grad_table, void* workspace, size_t workspace_bytes, void* stream) {
   const Problem p = {rows, vocab, dim, dtype, features, ld_features, table, ld_table};
   int status = gs_xent::check(p);
@@ -1101,20 +1173,21 @@ extern "C" int gs_xent_bwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dty
     }
     return gs_status_from_hip(hipGetLastError());
   }
-  if (!targets || !norm || !grad_loss || !count) return GS_ERR_INVALID_ARGUMENT;
+  if (!targets || !state || !grad_loss || !count) return GS_ERR_INVALID_ARGUMENT;
   if ((status = gs_xent::check_pointers(p)) != GS_OK) return status;
-  if ((uintptr_t)workspace & 255) return GS_ERR_MISALIGNED;
+  if (((uintptr_t)workspace & 255) || ((uintptr_t)state & 255)) return GS_ERR_MISALIGNED;
   const bool want_h = grad_features != nullptr, want_t = grad_table != nullptr;
   if (!workspace || workspace_bytes < gs_xent::BackwardPlan(p, want_h, want_t, nullptr).bytes)
     return GS_ERR_SCRATCH_TOO_SMALL;
   gs_xent::BackwardPlan b(p, want_h, want_t, workspace);
+  const gs_xent::State kept(p, const_cast<void*>(state));
   const gs_xent::Targets t = {targets, target_bits, ignore_index};
   if (dtype == GS_FP32)
-    return gs_xent::backward<_Float16, float, gs_tile::kWidePlanes>(p, t, logit_scale, reduction, (const float4*)norm, count, grad_loss,
-                                               (float*)grad_features, (float*)grad_table, b, s);
+    return gs_xent::backward<_Float16, float, gs_tile::kWidePlanes>(p, t, logit_scale, reduction, kept, count, grad_loss,
+                                                                    (float*)grad_features, (float*)grad_table, b, s);
   if (dtype == GS_BF16)
-    return gs_xent::backward<__bf16, __bf16, 1>(p, t, logit_scale, reduction, (const float4*)norm, count, grad_loss,
+    return gs_xent::backward<__bf16, __bf16, 1>(p, t, logit_scale, reduction, kept, count, grad_loss,
                                                 (__bf16*)grad_features, (__bf16*)grad_table, b, s);
-  return gs_xent::backward<_Float16, _Float16, 1>(p, t, logit_scale, reduction, (const float4*)norm, count, grad_loss,
+  return gs_xent::backward<_Float16, _Float16, 1>(p, t, logit_scale, reduction, kept, count, grad_loss,
                                                   (_Float16*)grad_features, (_Float16*)grad_table, b, s);
 }

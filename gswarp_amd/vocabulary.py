@@ -145,53 +145,54 @@ def embed_tokens(tokens: torch.Tensor, table: torch.Tensor, *, scale: float = 1.
 # ---------------------------------------------------------------- cross entropy
 
 def _entropy_forward(features, table, targets, ignore_index, reduction, logit_scale, keep: bool):
-    """(loss, norm or None, count) for 2-D features and 1-D targets."""
+    """(loss, what the backward needs or None) for 2-D features and 1-D targets."""
     device, n, (vocab, dim) = table.device, features.shape[0], table.shape
     lib = _lib.load()
-    code, reduce = _DTYPES[table.dtype], _REDUCTIONS[reduction]
+    code, ldf, ldt = _DTYPES[table.dtype], _row_stride(features), _row_stride(table)
     loss = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=device)
-    norm = torch.empty((n, 4), dtype=torch.float32, device=device) if keep else None
     with _device_guard(device), _workspace.device_lock(device):
-        nbytes = lib.gs_xent_fwd_workspace_bytes(n, vocab, dim, code, _row_stride(features), _row_stride(table))
-        # the count of rows sits in front of the workspace
-        space = _workspace_of(nbytes + 256 if not keep else nbytes, device)
-        count = torch.empty((1,), dtype=torch.int64, device=device) if keep else None
-        base = _aligned(space)
-        lib.call("gs_xent_fwd", n, vocab, dim, code, features.data_ptr(), _row_stride(features), table.data_ptr(),
-                 _row_stride(table), targets.data_ptr(), _INDEX_BITS[targets.dtype], ignore_index, logit_scale, reduce,
-                 loss.data_ptr(), _lib.ptr(norm), count.data_ptr() if keep else base, base if keep else base + 256,
-                 nbytes, _stream(device))
-    return loss, norm, count
+        # the count of rows sits in front of the workspace, or of the state
+        nbytes = lib.gs_xent_fwd_workspace_bytes(n, vocab, dim, code, ldf, ldt)
+        space = _workspace_of(256 + nbytes, device)
+        state = None
+        count = _aligned(space)
+        if keep:
+            state = _workspace_of(256 + lib.gs_xent_state_bytes(n, vocab, dim, code, ldf, ldt), device)
+            count = _aligned(state)
+        lib.call("gs_xent_fwd", n, vocab, dim, code, features.data_ptr(), ldf, table.data_ptr(), ldt,
+                 targets.data_ptr(), _INDEX_BITS[targets.dtype], ignore_index, logit_scale, _REDUCTIONS[reduction],
+                 loss.data_ptr(), count + 256 if keep else None, count, _aligned(space) + 256, nbytes, _stream(device))
+    return loss, state
 
 
 class LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, features, table, targets, ignore_index, reduction, logit_scale):
-        loss, norm, count = _entropy_forward(features, table, targets, ignore_index, reduction, logit_scale, True)
-        ctx.save_for_backward(features, table, targets, norm, count)
+        loss, state = _entropy_forward(features, table, targets, ignore_index, reduction, logit_scale, True)
+        ctx.save_for_backward(features, table, targets, state)
         ctx.options = (ignore_index, reduction, logit_scale)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
-        features, table, targets, norm, count = ctx.saved_tensors
+        features, table, targets, state = ctx.saved_tensors
         ignore_index, reduction, logit_scale = ctx.options
         want_features, want_table = ctx.needs_input_grad[:2]
         device, n, (vocab, dim) = table.device, features.shape[0], table.shape
         lib = _lib.load()
-        code = _DTYPES[table.dtype]
+        code, ldf, ldt = _DTYPES[table.dtype], _row_stride(features), _row_stride(table)
         grad_loss = grad_loss.contiguous()
-        ldf, ldt = _row_stride(features), _row_stride(table)
         grad_features = torch.empty((n, dim), dtype=table.dtype, device=device) if want_features else None
         grad_table = torch.empty((vocab, dim), dtype=table.dtype, device=device) if want_table else None
         with _device_guard(device), _workspace.device_lock(device):
             nbytes = lib.gs_xent_bwd_workspace_bytes(n, vocab, dim, code, ldf, ldt, want_features, want_table)
             space = _workspace_of(nbytes, device)
+            count = _aligned(state)
             lib.call("gs_xent_bwd", n, vocab, dim, code, features.data_ptr(), ldf, table.data_ptr(), ldt,
                      targets.data_ptr(), _INDEX_BITS[targets.dtype], ignore_index, logit_scale, _REDUCTIONS[reduction],
-                     norm.data_ptr(), count.data_ptr(), grad_loss.data_ptr(), _lib.ptr(grad_features),
-                     _lib.ptr(grad_table), _aligned(space), nbytes, _stream(device))
+                     count + 256, count, grad_loss.data_ptr(), _lib.ptr(grad_features), _lib.ptr(grad_table),
+                     _aligned(space), nbytes, _stream(device))
         return grad_features, grad_table, None, None, None, None
 
 

@@ -604,18 +604,21 @@ int gs_embed_bwd(int64_t n, int32_t vocab, int32_t dim, int32_t dtype, const voi
  * s_{i, targets_i}.  Rows whose target is ignore_index give 0 and do not
  * count, whatever they hold; any other target outside [0, vocab) gives NaN.
  * loss: `rows` fp32 for GS_REDUCE_NONE, else one (the sum, or the mean over
- * the rows that count; over none, NaN).  norm (4 fp32 a row, 16-byte aligned;
- * NULL if no backward follows) receives what gs_xent_bwd needs of the row's
- * softmax; count, but for GS_REDUCE_NONE, the number of rows that count, which gs_xent_bwd takes too.  features and table must be 16-byte
- * aligned unless they are fp32 or have a dim or row distance that is not a
- * multiple of 8 (those are laid out in the workspace first).  workspace:
+ * the rows that count; over none, NaN).  state (gs_xent_state_bytes bytes on
+ * 256; NULL if no backward follows) receives what gs_xent_bwd needs: the rows'
+ * softmax and, for the inputs named next, their layouts; count, but for
+ * GS_REDUCE_NONE, the number of rows that count, which gs_xent_bwd takes too.
+ * features and table must be 16-byte aligned unless they are fp32 or have a dim
+ * or row distance that is not a multiple of 8 (those are laid out first).  workspace:
  * gs_xent_fwd_workspace_bytes bytes on 256, of any content.
  */
+size_t gs_xent_state_bytes(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, int64_t ld_features,
+                           int64_t ld_table);
 size_t gs_xent_fwd_workspace_bytes(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, int64_t ld_features,
                                    int64_t ld_table);
 int gs_xent_fwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void* features, int64_t ld_features,
                 const void* table, int64_t ld_table, const void* targets, int32_t target_bits, int64_t ignore_index,
-                float logit_scale, int32_t reduction, float* loss, float* norm, int64_t* count, void* workspace,
+                float logit_scale, int32_t reduction, float* loss, void* state, int64_t* count, void* workspace,
                 size_t workspace_bytes, void* stream);
 
 /*
@@ -629,7 +632,7 @@ size_t gs_xent_bwd_workspace_bytes(int64_t rows, int32_t vocab, int32_t dim, int
                                    int64_t ld_table, int32_t want_features, int32_t want_table);
 int gs_xent_bwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void* features, int64_t ld_features,
                 const void* table, int64_t ld_table, const void* targets, int32_t target_bits, int64_t ignore_index,
-                float logit_scale, int32_t reduction, const float* norm, const int64_t* count, const float* grad_loss,
+                float logit_scale, int32_t reduction, const void* state, const int64_t* count, const float* grad_loss,
                 void* grad_features, void* grad_table, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
