@@ -13,6 +13,7 @@ back, and results do not change from run to run.
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -26,6 +27,7 @@ _INDEX_BITS = {torch.int32: 32, torch.int64: 64}
 _REDUCTIONS = {"none": _lib.GS_REDUCE_NONE, "sum": _lib.GS_REDUCE_SUM, "mean": _lib.GS_REDUCE_MEAN}
 _INT32_MAX = 2**31 - 1
 _MAX_DIM = 2**21 - 8
+_FP32_MAX = torch.finfo(torch.float32).max
 
 
 def _check_table(table, name: str) -> None:
@@ -43,19 +45,21 @@ def _check_table(table, name: str) -> None:
 
 
 def _check_indices(indices, name: str, device: torch.device) -> None:
+    if (isinstance(indices, torch.Tensor) and indices.dtype in _INDEX_BITS and indices.device == device
+            and indices.numel() <= _INT32_MAX):
+        return
     if not isinstance(indices, torch.Tensor):
         raise ValueError(f"{name} must be a torch.Tensor")
     if indices.device != device:
         raise ValueError(f"{name} must be on {device}, got {indices.device}")
     if indices.dtype not in _INDEX_BITS:
         raise ValueError(f"{name} must have dtype int32 or int64, got {indices.dtype}")
-    if indices.numel() > _INT32_MAX:
-        raise ValueError(f"{name} must have at most 2**31 - 1 elements")
+    raise ValueError(f"{name} must have at most 2**31 - 1 elements")
 
 
 def _check_factor(value, name: str) -> float:
     value = float(value)
-    if not math.isfinite(value) or abs(value) > torch.finfo(torch.float32).max:
+    if not -_FP32_MAX <= value <= _FP32_MAX:
         raise ValueError(f"{name} must be finite in float32")
     return value
 
@@ -77,11 +81,30 @@ def _row_stride(t: torch.Tensor) -> int:
 
 
 def _workspace_of(nbytes: int, device: torch.device) -> torch.Tensor:
-    return torch.empty((int(nbytes) + 255,), dtype=torch.uint8, device=device)
+    return torch.empty(nbytes + 255, dtype=torch.uint8, device=device)
 
 
 def _aligned(space: torch.Tensor) -> int:
     return (space.data_ptr() + 255) & ~255
+
+
+# Workspace sizes are functions of the sizes alone; a training loop asks for the same ones again.
+@functools.lru_cache(maxsize=256)
+def _embed_bwd_bytes(n, vocab, dim, code) -> int:
+    return _lib.load().gs_embed_bwd_workspace_bytes(n, vocab, dim, code)
+
+
+@functools.lru_cache(maxsize=256)
+def _entropy_fwd_bytes(n, vocab, dim, code, ldf, ldt) -> tuple[int, int]:
+    """(workspace, state)"""
+    lib = _lib.load()
+    return (lib.gs_xent_fwd_workspace_bytes(n, vocab, dim, code, ldf, ldt),
+            lib.gs_xent_state_bytes(n, vocab, dim, code, ldf, ldt))
+
+
+@functools.lru_cache(maxsize=256)
+def _entropy_bwd_bytes(n, vocab, dim, code, ldf, ldt, want_features, want_table) -> int:
+    return _lib.load().gs_xent_bwd_workspace_bytes(n, vocab, dim, code, ldf, ldt, want_features, want_table)
 
 
 # ---------------------------------------------------------------- lookup
@@ -114,9 +137,9 @@ class EmbedTokens(torch.autograd.Function):
         tokens, grad_out = tokens.contiguous(), grad_out.contiguous()
         grad = torch.empty((vocab, dim), dtype=dtype, device=device)
         n, code = tokens.numel(), _DTYPES[dtype]
+        nbytes = _embed_bwd_bytes(n, vocab, dim, code)
+        space = _workspace_of(nbytes, device)
         with _device_guard(device), _workspace.device_lock(device):
-            nbytes = lib.gs_embed_bwd_workspace_bytes(n, vocab, dim, code)
-            space = _workspace_of(nbytes, device)
             lib.call("gs_embed_bwd", n, vocab, dim, code, tokens.data_ptr(), _INDEX_BITS[tokens.dtype],
                      grad_out.data_ptr(), ctx.scale, -1 if ctx.padding_idx is None else ctx.padding_idx,
                      grad.data_ptr(), _aligned(space), nbytes, _stream(device))
@@ -150,15 +173,12 @@ def _entropy_forward(features, table, targets, ignore_index, reduction, logit_sc
     lib = _lib.load()
     code, ldf, ldt = _DTYPES[table.dtype], _row_stride(features), _row_stride(table)
     loss = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=device)
+    # the count of rows sits in front of the workspace, or of the state
+    nbytes, state_bytes = _entropy_fwd_bytes(n, vocab, dim, code, ldf, ldt)
+    space = _workspace_of(256 + nbytes, device)
+    state = _workspace_of(256 + state_bytes, device) if keep else None
+    count = _aligned(state if keep else space)
     with _device_guard(device), _workspace.device_lock(device):
-        # the count of rows sits in front of the workspace, or of the state
-        nbytes = lib.gs_xent_fwd_workspace_bytes(n, vocab, dim, code, ldf, ldt)
-        space = _workspace_of(256 + nbytes, device)
-        state = None
-        count = _aligned(space)
-        if keep:
-            state = _workspace_of(256 + lib.gs_xent_state_bytes(n, vocab, dim, code, ldf, ldt), device)
-            count = _aligned(state)
         lib.call("gs_xent_fwd", n, vocab, dim, code, features.data_ptr(), ldf, table.data_ptr(), ldt,
                  targets.data_ptr(), _INDEX_BITS[targets.dtype], ignore_index, logit_scale, _REDUCTIONS[reduction],
                  loss.data_ptr(), count + 256 if keep else None, count, _aligned(space) + 256, nbytes, _stream(device))
@@ -185,10 +205,10 @@ class LinearCrossEntropy(torch.autograd.Function):
         grad_loss = grad_loss.contiguous()
         grad_features = torch.empty((n, dim), dtype=table.dtype, device=device) if want_features else None
         grad_table = torch.empty((vocab, dim), dtype=table.dtype, device=device) if want_table else None
+        nbytes = _entropy_bwd_bytes(n, vocab, dim, code, ldf, ldt, want_features, want_table)
+        space = _workspace_of(nbytes, device)
+        count = _aligned(state)
         with _device_guard(device), _workspace.device_lock(device):
-            nbytes = lib.gs_xent_bwd_workspace_bytes(n, vocab, dim, code, ldf, ldt, want_features, want_table)
-            space = _workspace_of(nbytes, device)
-            count = _aligned(state)
             lib.call("gs_xent_bwd", n, vocab, dim, code, features.data_ptr(), ldf, table.data_ptr(), ldt,
                      targets.data_ptr(), _INDEX_BITS[targets.dtype], ignore_index, logit_scale, _REDUCTIONS[reduction],
                      count + 256, count, grad_loss.data_ptr(), _lib.ptr(grad_features), _lib.ptr(grad_table),
@@ -226,12 +246,13 @@ def linear_cross_entropy(features: torch.Tensor, table: torch.Tensor, targets: t
     logit_scale = _check_factor(logit_scale, "logit_scale")
     shape = targets.shape
     features = features if features.ndim == 2 else features.reshape(-1, dim)
-    features, table, targets = _rows(features, 16), _rows(table, 16), targets.reshape(-1).contiguous()
+    features, table = _rows(features, 16), _rows(table, 16)
+    targets = (targets if len(shape) == 1 else targets.reshape(-1)).contiguous()
     if torch.is_grad_enabled() and (features.requires_grad or table.requires_grad):
         loss = LinearCrossEntropy.apply(features, table, targets, ignore_index, reduction, logit_scale)
     else:
         loss = _entropy_forward(features, table, targets, ignore_index, reduction, logit_scale, False)[0]
-    return loss.reshape(shape) if reduction == "none" and loss.shape != shape else loss
+    return loss.reshape(shape) if reduction == "none" and len(shape) != 1 else loss
 
 
 class Vocabulary(nn.Module):
