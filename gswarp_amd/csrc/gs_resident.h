@@ -58,9 +58,10 @@ struct Args {
   // kFeatures, kTable
   const RowInfo* info;
   const uint64_t* counts;
-  float* part_sums;  // fp32, part_plane apart; null: out = alpha * unit * sum
+  float* part_sums;  // fp32, part_plane apart; null: the gradients go to out
   int64_t part_plane;
-  const float *alpha, *unit;
+  const double* alpha;
+  const float* unit;
   int32_t D;
   void* out;
 };
@@ -421,7 +422,7 @@ __global__ __launch_bounds__(kThreads, kKind == kForward && KB * PL <= 2 ? 4 : 2
     if (held_in && half == 0) a.stats[(int64_t)blockIdx.y * a.held.extent + held_row] = make_float2(all, sum);
   } else {
     if (!held_in) return;
-    const float al = a.part_sums ? 1.0f : a.unit ? *a.alpha * *a.unit : *a.alpha;
+    const float factor = a.part_sums ? 0.0f : gs_xent::factor_of(a.alpha, a.unit);
 #pragma unroll
     for (int d = 0; d < kDBlocks; ++d)
 #pragma unroll
@@ -436,7 +437,8 @@ __global__ __launch_bounds__(kThreads, kKind == kForward && KB * PL <= 2 ? 4 : 2
         }
         const int64_t at = (int64_t)held_row * a.D + first;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = counts ? v[j] * al : 0.0f;
+        for (int j = 0; j < 4; ++j)
+          v[j] = !counts ? 0.0f : a.part_sums ? v[j] : gs_xent::gradient_of<T>(v[j], factor);
         if (a.part_sums) {
           float* to = a.part_sums + (int64_t)blockIdx.y * a.part_plane + at;
           if (a.D % 4 == 0 && first < a.D) *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);

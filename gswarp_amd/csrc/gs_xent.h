@@ -50,4 +50,30 @@ struct __attribute__((aligned(16))) RowInfo {
   int target;   // -1: none in the vocabulary, or the row does not count
 };
 
+// fp16 (and fp32's planes) have 2^-14 as their least normal number: ds (at most 1
+// in magnitude after the division by the largest g) is held times 2^15, so that
+// probabilities down to 2^-29 keep all their bits.  bf16 has fp32's exponents and
+// needs no scale.  Rounding ds to 16 bits adds an error of the size of the
+// results' own rounding to the same type; fp32's three planes keep 22 bits of
+// probabilities down to 2^-51, and an error of 2^-62.
+template <typename T>
+struct Held {
+  static constexpr float kScale = 1.0f;
+};
+template <>
+struct Held<_Float16> {
+  static constexpr float kScale = 32768.0f;
+};
+
+// A gradient from its sum of held ds: alpha is the gradient's factor without the
+// held scale, unit the other operand's (fp32; else null).  The power of two
+// first, and the factors' product in 64 bits: none of them leaves fp32's range unless the gradient does.
+template <typename T>
+__device__ __forceinline__ float gradient_of(float sum, float factor) {
+  return sum * (1.0f / Held<T>::kScale) * factor;
+}
+__device__ __forceinline__ float factor_of(const double* alpha, const float* unit) {
+  return (float)(unit ? *alpha * (double)*unit : *alpha);
+}
+
 }  // namespace gs_xent

@@ -42,21 +42,6 @@ constexpr int kJoinThreads = 256;
 constexpr int64_t kPieceBytes = 1ll << 30;     // ds of one piece, all planes
 constexpr int64_t kLeastSide = 4096;           // rows or vocabulary of a piece, at least (a multiple of the tiles')
 constexpr int64_t kStatBytes = 256ll << 20;    // the tiles' pairs of one piece (forward)
-// fp16 (and fp32's planes) have 2^-14 as their least normal number: ds (at most 1
-// in magnitude after the division by the largest g) is held times 2^15, so that
-// probabilities down to 2^-29 keep all their bits.  bf16 has fp32's exponents and
-// needs no scale.  Rounding ds to 16 bits adds an error of the size of the
-// results' own rounding to the same type; fp32's three planes keep 22 bits of
-// probabilities down to 2^-51, and an error of 2^-62.
-template <typename T>
-struct Held {
-  static constexpr float kScale = 1.0f;
-};
-template <>
-struct Held<_Float16> {
-  static constexpr float kScale = 32768.0f;
-};
-
 // ------------------------------------------------------------------ packing
 // A matrix and where its layout for the tile loads goes: rows of dp = ceil(dim /
 // 8) * 8 16-bit values, zero past dim, from dst (null: it is read in place);
@@ -402,14 +387,14 @@ __global__ __launch_bounds__(256) void largest_kernel(const float* __restrict__ 
 
 // Per row: its RowInfo, and one bit: does the row count.  With a gradient for
 // each row the factors are g_i / G, G the largest, so that ds stays in the 16-bit
-// type's range; alpha, applied to the sums, holds the rest.
+// type's range; alpha holds the rest.
 __global__ __launch_bounds__(256) void rows_kernel(const float* __restrict__ grad, int64_t rows, int vocab,
                                                    Targets targets, int reduction, const int64_t* __restrict__ count,
                                                    const float4* __restrict__ norm, float logit_scale,
                                                    float logit_scale2, const float* __restrict__ units,
                                                    float held_scale, const float* __restrict__ largest, int largest_n,
                                                    RowInfo* __restrict__ info, uint64_t* __restrict__ counts,
-                                                   float* __restrict__ alpha) {
+                                                   double* __restrict__ alpha) {
   __shared__ float lds[4];
   const int lane = threadIdx.x & 63;
   float G = 1.0f;
@@ -445,10 +430,10 @@ __global__ __launch_bounds__(256) void rows_kernel(const float* __restrict__ gra
   const uint64_t bits = __ballot(use);
   if (lane == 0 && row < rows) counts[row / 64] = bits;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
-    float g = G;
+    double g = G;
     if (reduction == GS_REDUCE_SUM) g = grad[0];
-    if (reduction == GS_REDUCE_MEAN) g = *count ? grad[0] / (float)*count : 0.0f;  // no row counts: zeros
-    *alpha = g * logit_scale / held_scale;
+    if (reduction == GS_REDUCE_MEAN) g = *count ? (double)grad[0] / (double)*count : 0.0;  // no row counts: zeros
+    *alpha = g * (double)logit_scale;
   }
 }
 
@@ -550,13 +535,13 @@ __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, 
 // features or of the table), m the D columns.  kTableGrad: dw (both operands in
 // K rows, K the rows of the piece); else dh (ds along K, K the vocabulary).
 // With `part` set the tile goes, in fp32, to plane blockIdx.y of part (added to
-// what is there if `add`); else out = alpha * tile in the result's type (unit: x's, fp32).
+// what is there if `add`); else out = the gradient of the tile's sums in the result's type (alpha, unit: see factor_of).
 // rows_count (dh): rows that do not count are zero.
 template <class S, typename T, typename Out, bool kTableGrad>
 __global__ __launch_bounds__(S::kThreads) void grad_kernel(Operand x, Operand ds, int32_t K, int32_t k_part,
                                                            int products, const uint64_t* __restrict__ counts,
                                                            int tiles_m, int tiles_n, float* __restrict__ part, int64_t part_plane,
-                                                           bool add, const float* __restrict__ alpha,
+                                                           bool add, const double* __restrict__ alpha,
                                                            const float* __restrict__ unit, Out* __restrict__ out) {
   __shared__ __attribute__((aligned(16))) char lds[S::kLdsBytes];
   const gs_tile::TileAt tile = gs_tile::tile_at(tiles_m, tiles_n);
@@ -570,7 +555,7 @@ __global__ __launch_bounds__(S::kThreads) void grad_kernel(Operand x, Operand ds
                                              kTableGrad ? counts : nullptr, lds);
   const int lane = threadIdx.x & 63;
   const int wm = gs_tile::wave_m<S>(), wn = gs_tile::wave_n<S>();
-  const float al = part ? 0.0f : unit ? *alpha * *unit : *alpha;
+  const float factor = part ? 0.0f : factor_of(alpha, unit);
 #pragma unroll
   for (int b = 0; b < S::kNB; ++b) {
     const int n = n0 + wn + 32 * b + (lane & 31);
@@ -590,23 +575,23 @@ __global__ __launch_bounds__(S::kThreads) void grad_kernel(Operand x, Operand ds
         } else {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (m + j < D) out[at + j] = (Out)(use ? acc.c[a][b][4 * q + j] * al : 0.0f);
+            if (m + j < D) out[at + j] = (Out)(use ? gradient_of<T>(acc.c[a][b][4 * q + j], factor) : 0.0f);
         }
       }
   }
 }
 
-// out = alpha (and x's unit) * sum of the planes; counts (dh): rows that do not
+// out = the gradient of the planes' sum; counts (dh): rows that do not
 // count are zero.  kGroups threads share an element's planes, their sums joined in
 // order.
-template <int kGroups, typename Out>
+template <int kGroups, typename T, typename Out>
 __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ part, int planes, int64_t plane,
                                                      int64_t n, int D, const uint64_t* __restrict__ counts,
-                                                     const float* __restrict__ alpha, const float* __restrict__ unit,
+                                                     const double* __restrict__ alpha, const float* __restrict__ unit,
                                                      Out* __restrict__ out) {
   constexpr int kElements = 256 / kGroups;
   __shared__ float lds[256];
-  const float al = unit ? *alpha * *unit : *alpha;
+  const float factor = factor_of(alpha, unit);
   const int element = threadIdx.x % kElements, group = threadIdx.x / kElements;
   for (int64_t i0 = (int64_t)blockIdx.x * kElements; i0 < n; i0 += (int64_t)gridDim.x * kElements) {
     const int64_t i = i0 + element;
@@ -620,7 +605,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ p
       if (group > 0) continue;
       for (int g = 1; g < kGroups; ++g) s += lds[g * kElements + element];
     }
-    if (i < n) out[i] = (Out)(!counts || row_counts(counts, i / D) ? s * al : 0.0f);
+    if (i < n) out[i] = (Out)(!counts || row_counts(counts, i / D) ? gradient_of<T>(s, factor) : 0.0f);
   }
 }
 
@@ -656,11 +641,14 @@ struct Problem {
   size_t element() const { return dtype == GS_FP32 ? 4 : 2; }
 };
 
+constexpr int64_t kMaxRows = (1ll << 31) - 1024;
+
 static int check(const Problem& p) {
   if (p.rows < 0 || p.vocab <= 0 || p.dim <= 0 || p.dtype < GS_FP32 || p.dtype > GS_FP16)
     return GS_ERR_INVALID_ARGUMENT;
   if (p.ld_features < p.dim || p.ld_table < p.dim) return GS_ERR_INVALID_ARGUMENT;
-  if (p.rows > 0x7fffffffll || p.dim > gs_tile::kMaxLd - 8) return GS_ERR_OVERFLOW;
+  // (indices of rows, rounded up to a tile, are int32)
+  if (p.rows > kMaxRows || p.vocab > kMaxRows || p.dim > gs_tile::kMaxLd - 8) return GS_ERR_OVERFLOW;
   return GS_OK;
 }
 
@@ -927,7 +915,8 @@ struct BackwardPlan {
   bool direct_h, direct_t;  // one part and one piece: no fp32 sums in between
   uint16_t* ds;
   RowInfo* info;
-  float *alpha, *largest, *part_h, *part_t;
+  double* alpha;
+  float *largest, *part_h, *part_t;
   uint64_t* counts;
   size_t bytes;
 
@@ -966,7 +955,7 @@ struct BackwardPlan {
     ds = c.take<uint16_t>(rows_piece * ld * p.ds_planes());
     info = c.take<RowInfo>(p.rows);
     counts = c.take<uint64_t>(ceil_div(p.rows, 64));
-    alpha = c.take<float>(1);
+    alpha = c.take<double>(1);
     largest = c.take<float>(kLargestBlocks);
     part_h = c.take<float>(want_h && !direct_h ? parts_h * rows_piece * p.dim : 0);
     part_t = c.take<float>(want_t && !direct_t ? parts_t * (row_pieces > 1 ? (int64_t)p.vocab : cols_piece) * p.dim : 0);
@@ -976,12 +965,12 @@ struct BackwardPlan {
 
 static unsigned finish_blocks(int64_t n) { return (unsigned)min(ceil_div(n, 256), (int64_t)8192); }
 
-template <typename Out>
+template <typename T, typename Out>
 static void finish(const float* part, int planes, int64_t plane, int64_t n, int D, const uint64_t* counts,
-                   const float* alpha, const float* unit, Out* out, hipStream_t s) {
+                   const double* alpha, const float* unit, Out* out, hipStream_t s) {
   // many planes of few elements (a small table's) do not fill the chip by their elements alone
-  if (planes >= 16) finish_kernel<8><<<finish_blocks(n * 8), 256, 0, s>>>(part, planes, plane, n, D, counts, alpha, unit, out);
-  else finish_kernel<1><<<finish_blocks(n), 256, 0, s>>>(part, planes, plane, n, D, counts, alpha, unit, out);
+  if (planes >= 16) finish_kernel<8, T><<<finish_blocks(n * 8), 256, 0, s>>>(part, planes, plane, n, D, counts, alpha, unit, out);
+  else finish_kernel<1, T><<<finish_blocks(n), 256, 0, s>>>(part, planes, plane, n, D, counts, alpha, unit, out);
 }
 
 template <typename T, typename Out, int kPlanes>
@@ -1022,7 +1011,7 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
       a.out = out;
       launch_resident<T, decltype(kind)::value>(p, a, parts, s);
       if (parts > 1)
-        finish(sums, parts, a.part_plane, a.part_plane, D, nullptr, b.alpha, unit, out, s);
+        finish<T>(sums, parts, a.part_plane, a.part_plane, D, nullptr, b.alpha, unit, out, s);
     };
     if (grad_features)
       run(std::integral_constant<int, gs_resident::kFeatures>{}, features, table, b.parts_h, b.part_h, unit_w, grad_features);
@@ -1073,15 +1062,15 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
               x, ds, rows, k_part, p.ds_products(), counts, tiles_m, tiles_n, part, part_plane, r > 0, b.alpha, unit_h,
               grad_table + c * D);
           if (part && b.row_pieces == 1)
-            finish(part, b.parts_t, part_plane, (int64_t)cols * D, D, nullptr, b.alpha, unit_h, grad_table + c * D, s);
+            finish<T>(part, b.parts_t, part_plane, (int64_t)cols * D, D, nullptr, b.alpha, unit_h, grad_table + c * D, s);
         }
       });
     }
     if (grad_features && !b.direct_h)
-      finish(b.part_h, b.parts_h, (int64_t)rows * D, (int64_t)rows * D, D, counts, b.alpha, unit_w, grad_features + r * D, s);
+      finish<T>(b.part_h, b.parts_h, (int64_t)rows * D, (int64_t)rows * D, D, counts, b.alpha, unit_w, grad_features + r * D, s);
   }
   if (grad_table && b.row_pieces > 1)
-    finish(b.part_t, b.parts_t, (int64_t)p.vocab * D, (int64_t)p.vocab * D, D, nullptr, b.alpha, unit_h, grad_table, s);
+    finish<T>(b.part_t, b.parts_t, (int64_t)p.vocab * D, (int64_t)p.vocab * D, D, nullptr, b.alpha, unit_h, grad_table, s);
   return gs_status_from_hip(hipGetLastError());
 }
 

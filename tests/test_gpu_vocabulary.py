@@ -467,3 +467,31 @@ def test_refusals(device):
             (lambda: entropy(features.cpu(), table, tokens), "features must be")):
         with pytest.raises(ValueError, match=message):
             call()
+
+
+@pytest.mark.parametrize("h_scale,w_scale,logit_scale", [(1e15, 1e-15, 1.0), (1e-20, 1.0, 1e20), (1e-20, 1e-20, 1.0),
+                                                         (3e18, 3e18, 1e-36)])
+def test_entropy_fp32_magnitudes(device, h_scale, w_scale, logit_scale):
+    """fp32 features and tables far from 1, for short and for long rows."""
+    for rows, vocab, dim in ((150, 90, 40), (150, 90, 200)):
+        features, table, targets, gen = _problem(device, FP32, rows, vocab, dim)
+        features = (features.detach() * h_scale).requires_grad_(True)
+        table = (table.detach() * w_scale).requires_grad_(True)
+        _compare(features, table, targets, torch.tensor(1.0, device=device), logit_scale=logit_scale)
+
+
+@pytest.mark.parametrize("dim", [48, 144])
+def test_entropy_fp32_rows_of_many_magnitudes(device, dim):
+    """Rows and tables whose rows' sizes span six decades: as exact as fp32 for the largest of them."""
+    features, table, targets, gen = _problem(device, FP32, 300, 200, dim)
+    features = features.detach() * (10.0 ** (-6 * torch.rand(300, 1, generator=gen))).to(device)
+    table = table.detach() * (10.0 ** (-6 * torch.rand(200, 1, generator=gen))).to(device)
+    _compare(features.requires_grad_(True), table.requires_grad_(True), targets, torch.tensor(1.0, device=device),
+             reduction="sum")
+
+
+def test_language_scene_learns(device):
+    from examples.language_scene import train
+
+    losses = train(steps=12, count=4000, size=128)
+    assert all(math.isfinite(x) for x in losses) and losses[-1] < 0.8 * losses[0]
