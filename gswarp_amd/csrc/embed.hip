@@ -15,6 +15,8 @@
 // sort: see few_kernel.
 #include "gs_capi.h"
 
+#include <type_traits>
+
 namespace gs_embed {
 
 typedef unsigned u32;
@@ -32,18 +34,41 @@ struct Tokens {
   }
 };
 
+// Rows are moved in vectors of 16 bytes (V elements), or, shorter ones, element by
+// element.  kWhole: rows are whole vectors, on 16 bytes.  Else they may lie
+// anywhere (the memory unit takes any address), and a row's last vector ends with
+// the row, over elements that the one before it holds too: both carry the same.
 template <typename T, int V>
-struct __attribute__((aligned(sizeof(T) * V))) Vec {
+struct __attribute__((aligned(sizeof(T) * V < 16 ? sizeof(T) * V : 16))) Vec {
   T v[V];
 };
+
+template <int V>
+__device__ __forceinline__ int column_of(int vector, int D) {
+  return min(vector * V, D - V);
+}
+
+template <bool kWhole, typename T, int V>
+__device__ __forceinline__ Vec<T, V> load_vector(const T* __restrict__ p) {
+  if (kWhole) return *reinterpret_cast<const Vec<T, V>*>(p);
+  Vec<T, V> x;
+  __builtin_memcpy(&x, p, sizeof(x));
+  return x;
+}
+
+template <bool kWhole, typename T, int V>
+__device__ __forceinline__ void store_vector(T* __restrict__ p, const Vec<T, V>& x) {
+  if (kWhole) *reinterpret_cast<Vec<T, V>*>(p) = x;
+  else __builtin_memcpy(p, &x, sizeof(x));
+}
 
 // ------------------------------------------------------------------ forward
 // A thread moves a vector of V elements.  What bounds it is the write of out.
 // Blocks go to the 8 XCDs in turn, so each XCD is given a run of consecutive
 // blocks, and the stores bypass the caches: 960 MB of rows (5M x 48 fp32 from 8192)
 // are written at 7.2 TB/s, against 3.6 with cached stores in launch order.
-template <typename T, int V>
-__global__ __launch_bounds__(kThreads) void lookup_kernel(Tokens tokens, int64_t n, u32 vocab, u32 row_vectors,
+template <typename T, int V, bool kWhole>
+__global__ __launch_bounds__(kThreads) void lookup_kernel(Tokens tokens, int64_t n, u32 vocab, int D, u32 row_vectors,
                                                           const T* __restrict__ table, int64_t ld, float scale,
                                                           T* __restrict__ out) {
   const u32 share = gridDim.x / 8;
@@ -52,12 +77,13 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(Tokens tokens, int64_t
   const int64_t first = block * kThreads;
   const int64_t row0 = first / row_vectors;
   const u32 at = (u32)(first - row0 * row_vectors) + threadIdx.x;
-  const u32 r = at / row_vectors, column = at - r * row_vectors;
+  const u32 r = at / row_vectors;
   if (row0 + r >= n) return;
   const int64_t token = tokens.at(row0 + r);
+  const int column = column_of<V>((int)(at - r * row_vectors), D);
   Vec<T, V> x;
   if (token >= 0 && token < vocab) {
-    x = *reinterpret_cast<const Vec<T, V>*>(table + token * ld + (int64_t)column * V);
+    x = load_vector<kWhole, T, V>(table + token * ld + column);
     if (scale != 1.0f)
 #pragma unroll
       for (int e = 0; e < V; ++e) x.v[e] = (T)((float)x.v[e] * scale);
@@ -65,12 +91,12 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(Tokens tokens, int64_t
 #pragma unroll
     for (int e = 0; e < V; ++e) x.v[e] = (T)__builtin_nanf("");
   }
-  T* to = out + (first + threadIdx.x) * V;
-  if constexpr (sizeof(x) == 16) {
+  T* to = out + (row0 + r) * D + column;
+  if constexpr (kWhole && sizeof(x) == 16) {
     typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
     __builtin_nontemporal_store(__builtin_bit_cast(u32x4, x), reinterpret_cast<u32x4*>(to));
   } else {
-    *reinterpret_cast<Vec<T, V>*>(to) = x;
+    store_vector<kWhole, T, V>(to, x);
   }
 }
 
@@ -121,10 +147,10 @@ struct Level {
 constexpr int kRunThreads = 512;
 constexpr int kMaxChunk = 2048;  // entries of a chunk at most
 
-// blockIdx.y: columns (blockIdx.y lanes + l) V on are lane l's.
-template <typename S, typename T, int V>
-__global__ __launch_bounds__(kRunThreads) void runs_kernel(Level v, const S* __restrict__ src, T* __restrict__ out) {
-  constexpr int kBatch = 8;  // rows in flight
+// blockIdx.y: vector blockIdx.y lanes + l of a row is lane l's.
+template <typename S, typename T, int V, bool kWhole>
+__global__ __launch_bounds__(kRunThreads, 4) void runs_kernel(Level v, const S* __restrict__ src, T* __restrict__ out) {
+  constexpr int kBatch = sizeof(S) * V > 16 ? 4 : 8;  // rows of a batch; two are in flight
   __shared__ u32 lds_keys[kMaxChunk + 3];
   __shared__ int lds_positions[kMaxChunk];
   __shared__ float lds_head[kRunThreads * V], lds_tail[kRunThreads * V];
@@ -162,14 +188,14 @@ __global__ __launch_bounds__(kRunThreads) void runs_kernel(Level v, const S* __r
     for (int e = threadIdx.x; e < here; e += kRunThreads) lds_positions[e] = v.positions[begin + e];
   __syncthreads();
 
-  const int col = (blockIdx.y * v.lanes + lane) * V;
-  const bool in = col < v.D;
+  const bool in = (int)(blockIdx.y * v.lanes + lane) * V < v.D;
+  const int col = column_of<V>(blockIdx.y * v.lanes + lane, v.D);
   auto write = [&](u32 key, const float* acc) {
     if (!in) return;
     Vec<T, V> x;
 #pragma unroll
     for (int e = 0; e < V; ++e) x.v[e] = (T)(acc[e] * v.scale);
-    *reinterpret_cast<Vec<T, V>*>(out + (int64_t)key * v.D + col) = x;
+    store_vector<kWhole, T, V>(out + (int64_t)key * v.D + col, x);
   };
 
   // the group's own part
@@ -210,7 +236,7 @@ __global__ __launch_bounds__(kRunThreads) void runs_kernel(Level v, const S* __r
         const int e = e0 + j;
         if (e < e_end && in && keys[2 + e] < v.vocab) {
           const int64_t row = v.positions ? (int64_t)lds_positions[e] : begin + e;
-          to[j] = *reinterpret_cast<const Vec<S, V>*>(src + row * v.ld + col);
+          to[j] = load_vector<kWhole, S, V>(src + row * v.ld + col);
         }
       }
     };
@@ -272,24 +298,40 @@ __global__ __launch_bounds__(kRunThreads) void runs_kernel(Level v, const S* __r
     }
     cur = kNone;
   };
-  for (int g = 0; g < groups; ++g) {
-    const int at = g * v.lanes + lane;
-    if (head_key[g] != kNone) {
-      if (cur == kNone) {  // it comes in from the chunk before
-        cur = head_key[g];
-        from_left = true;
+  // (what a batch of groups left is read at once: their keys and heads do not wait for each other)
+  constexpr int kMerge = 8;
+  for (int g0 = 0; g0 < groups; g0 += kMerge) {
+    u32 heads[kMerge], tails[kMerge];
+    bool open[kMerge];
+    float head[kMerge][V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] = 0.0f;
-      }
+    for (int j = 0; j < kMerge; ++j) {
+      const int g = min(g0 + j, groups - 1);
+      heads[j] = g0 + j < groups ? head_key[g] : kNone;
+      tails[j] = g0 + j < groups ? tail_key[g] : kNone;
+      open[j] = head_open[g];
 #pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] += lds_head[e * kRunThreads + at];
-      if (!head_open[g]) close(false);
+      for (int e = 0; e < V; ++e) head[j][e] = lds_head[e * kRunThreads + g * v.lanes + lane];
     }
-    if (tail_key[g] != kNone) {
-      cur = tail_key[g];
-      from_left = false;
 #pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] = lds_tail[e * kRunThreads + at];
+    for (int j = 0; j < kMerge; ++j) {
+      if (heads[j] != kNone) {
+        if (cur == kNone) {  // it comes in from the chunk before
+          cur = heads[j];
+          from_left = true;
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[e] = 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] += head[j][e];
+        if (!open[j]) close(false);
+      }
+      if (tails[j] != kNone) {
+        cur = tails[j];
+        from_left = false;
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] = lds_tail[e * kRunThreads + (g0 + j) * v.lanes + lane];
+      }
     }
   }
   if (cur != kNone) close(true);
@@ -304,7 +346,7 @@ __global__ __launch_bounds__(kRunThreads) void runs_kernel(Level v, const S* __r
 // rows, a part of the list for each group of lanes, the parts joined in order.
 // The workgroups behind zero the rows of the table that no token names.
 constexpr int kFew = 2048;
-template <typename T, int V>
+template <typename T, int V, bool kWhole>
 __global__ __launch_bounds__(kThreads) void few_kernel(Tokens tokens, int n, u32 vocab, int64_t padding, int D,
                                                        int lanes, float scale, const T* __restrict__ grad,
                                                        T* __restrict__ out) {
@@ -360,8 +402,8 @@ __global__ __launch_bounds__(kThreads) void few_kernel(Tokens tokens, int n, u32
   if (list[0] != me) return;  // the token's first position does the work
 
   const int groups = kThreads / lanes, group = threadIdx.x / lanes, lane = threadIdx.x % lanes;
-  const int col = (blockIdx.y * lanes + lane) * V;
-  const bool in = col < D;
+  const bool in = (int)(blockIdx.y * lanes + lane) * V < D;
+  const int col = column_of<V>(blockIdx.y * lanes + lane, D);
   const int part = (all + groups - 1) / groups;
   const int p_begin = min(all, group * part), p_end = min(all, p_begin + part);
   float acc[V];
@@ -373,7 +415,7 @@ __global__ __launch_bounds__(kThreads) void few_kernel(Tokens tokens, int n, u32
       Vec<T, V> x[kBatch];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j)
-        if (p0 + j < p_end) x[j] = *reinterpret_cast<const Vec<T, V>*>(grad + (int64_t)list[p0 + j] * D + col);
+        if (p0 + j < p_end) x[j] = load_vector<kWhole, T, V>(grad + (int64_t)list[p0 + j] * D + col);
 #pragma unroll
       for (int j = 0; j < kBatch; ++j)
         if (p0 + j < p_end)
@@ -394,7 +436,7 @@ __global__ __launch_bounds__(kThreads) void few_kernel(Tokens tokens, int n, u32
   Vec<T, V> x;
 #pragma unroll
   for (int e = 0; e < V; ++e) x.v[e] = (T)(acc[e] * scale);
-  *reinterpret_cast<Vec<T, V>*>(out + (int64_t)mine * D + col) = x;
+  store_vector<kWhole, T, V>(out + (int64_t)mine * D + col, x);
 }
 
 template <typename T>
@@ -404,34 +446,31 @@ __global__ __launch_bounds__(kThreads) void zero_kernel(T* __restrict__ out, int
 }
 
 // ------------------------------------------------------------------ host
-// Elements of a vector access: 16 bytes where the rows allow it, else two or one elements.
-template <typename T>
-static int vector_of(int64_t D, int64_t ld, const void* a, const void* b) {
-  auto fits = [&](int v) {
-    const uintptr_t bytes = sizeof(T) * v;
-    return D % v == 0 && ld % v == 0 && (uintptr_t)a % bytes == 0 && (uintptr_t)b % bytes == 0;
-  };
-  const int most = 16 / (int)sizeof(T);
-  return fits(most) ? most : fits(2) ? 2 : 1;
+static int vector_of(int32_t dtype, int64_t D) {
+  const int V = dtype == GS_FP32 ? 4 : 8;
+  return D < V ? 1 : V;
 }
 
-template <typename T, int V>
-static int lookup(int64_t n, int32_t vocab, int32_t dim, Tokens tokens, const T* table, int64_t ld, float scale, T* out,
-                  hipStream_t s) {
-  const int64_t vectors = n * (dim / V);
-  const int64_t blocks = ceil_div(vectors, kThreads);
-  if (blocks > 0x7fffffffll) return GS_ERR_OVERFLOW;
-  lookup_kernel<T, V><<<(unsigned)blocks, kThreads, 0, s>>>(tokens, n, (u32)vocab, (u32)(dim / V), table, ld, scale, out);
-  return gs_status_from_hip(hipGetLastError());
+// Calls f with V and kWhole for rows of D elements, ld apart in a and contiguous in b.
+template <typename T, class F>
+static int with_vectors(int64_t D, int64_t ld, const void* a, const void* b, F f) {
+  constexpr int V = 16 / sizeof(T);
+  if (D < V) return f(std::integral_constant<int, 1>{}, std::true_type{});
+  if (D % V == 0 && ld % V == 0 && (uintptr_t)a % 16 == 0 && (uintptr_t)b % 16 == 0)
+    return f(std::integral_constant<int, V>{}, std::true_type{});
+  return f(std::integral_constant<int, V>{}, std::false_type{});
 }
 
 template <typename T>
 static int forward(int64_t n, int32_t vocab, int32_t dim, Tokens tokens, const void* table, int64_t ld, float scale,
                    void* out, hipStream_t s) {
-  const int v = vector_of<T>(dim, ld, table, out);
-  if (v == 16 / (int)sizeof(T)) return lookup<T, 16 / sizeof(T)>(n, vocab, dim, tokens, (const T*)table, ld, scale, (T*)out, s);
-  if (v == 2) return lookup<T, 2>(n, vocab, dim, tokens, (const T*)table, ld, scale, (T*)out, s);
-  return lookup<T, 1>(n, vocab, dim, tokens, (const T*)table, ld, scale, (T*)out, s);
+  return with_vectors<T>(dim, ld, table, out, [&](auto V, auto kWhole) {
+    const int64_t row_vectors = ceil_div(dim, V), blocks = ceil_div(n * row_vectors, kThreads);
+    if (blocks > 0x7fffffffll) return (int)GS_ERR_OVERFLOW;
+    lookup_kernel<T, V, kWhole><<<(unsigned)blocks, kThreads, 0, s>>>(tokens, n, (u32)vocab, dim, (u32)row_vectors,
+                                                                     (const T*)table, ld, scale, (T*)out);
+    return gs_status_from_hip(hipGetLastError());
+  });
 }
 
 // Lanes of a row: a power of two, at most a wave.
@@ -441,16 +480,23 @@ static int lanes_of(int D, int V) {
   return lanes;
 }
 
-// Entries of a group: 16 to 64, so that a first level of few positions still
-// fills the chip, as far as a chunk holds them.
-static int group_length(int64_t n, int lanes) {
-  const int groups = kRunThreads / lanes;
-  int length = 16;
-  while (length < 64 && n / (length * groups) > 1024 && 2 * length * groups <= kMaxChunk) length *= 2;
-  return length * groups <= kMaxChunk ? length : kMaxChunk / groups;
+// Entries of a group.  On the first level 4 to 64, by how many make 1024 chunks,
+// which fill the chip; above, all of them where that is 8 at most, else 8 and on,
+// so that at most 64 chunks hand on to the next level: few levels, and none that
+// leaves many rows to one workgroup (2048 rows of 256 bytes take one 43 us).
+static int group_length(int64_t n, int lanes, bool first) {
+  const int groups = kRunThreads / lanes, most = min(64, kMaxChunk / groups);
+  // (above, even: a part begins with a chunk's first entry, so that what is empty
+  // between two entries of a run is one at most, and before the part)
+  if (!first && n <= groups * min(8, most)) return (int)round_up(ceil_div(n, groups), 2);
+  int length = first ? 4 : min(8, most);
+  while (2 * length <= most && n / (length * groups) > (first ? 1024 : 64)) length *= 2;
+  return min(length, most);
 }
 
-static int64_t chunks_of(int64_t n, int lanes) { return ceil_div(n, (int64_t)kRunThreads / lanes * group_length(n, lanes)); }
+static int64_t chunks_of(int64_t n, int lanes, bool first) {
+  return ceil_div(n, (int64_t)kRunThreads / lanes * group_length(n, lanes, first));
+}
 
 struct BackwardPlan {
   u32 *keys, *keys_alt, *next_keys[2];
@@ -460,7 +506,8 @@ struct BackwardPlan {
   char* sort_scratch;
   size_t sort_bytes, bytes;
 
-  BackwardPlan(int64_t n, int32_t dim, void* ws) {
+  // vector: elements of a vector of the rows' type
+  BackwardPlan(int64_t n, int32_t dim, int vector, void* ws) {
     char* base = (char*)ws;
     size_t at = 0;
     auto take = [&](int64_t size) {
@@ -477,14 +524,11 @@ struct BackwardPlan {
     positions = (int*)take(n * 4);
     positions_alt = (int*)take(n * 4);
     sort_scratch = take((int64_t)sort_bytes);
-    // the levels' entries, in turn in two places, for whatever vectors the addresses will allow
-    int64_t entries[2] = {0, 0};
-    for (int V = 1; V <= 8; V *= 2) {
-      const int lanes = lanes_of(dim, V);
-      const int64_t first = 2 * chunks_of(n, lanes);
-      entries[0] = max(entries[0], first);
-      entries[1] = max(entries[1], 2 * chunks_of(first, lanes));
-    }
+    // the levels' entries, in turn in two places
+    const int lanes = lanes_of(dim, vector);
+    int64_t entries[2];
+    entries[0] = 2 * chunks_of(n, lanes, true);
+    entries[1] = 2 * chunks_of(entries[0], lanes, false);
     for (int level = 0; level < 2; ++level) {
       next_keys[level] = (u32*)take(entries[level] * 4);
       next[level] = (float*)take(entries[level] * next_ld * 4);
@@ -493,24 +537,24 @@ struct BackwardPlan {
   }
 };
 
-template <typename S, typename T, int V>
-static int64_t runs(Level v, const S* src, T* out, bool zero_absent, hipStream_t s) {
+template <bool kFirst, typename S, typename T, int V, bool kWhole>
+static int64_t runs(Level v, const S* src, T* out, hipStream_t s) {
   v.lanes = lanes_of(v.D, V);
-  v.length = group_length(v.n, v.lanes);
-  v.chunks = (int)chunks_of(v.n, v.lanes);
-  const int64_t blocks = v.chunks + (zero_absent ? ceil_div(v.vocab, kRunThreads) : 0);
+  v.length = group_length(v.n, v.lanes, kFirst);
+  v.chunks = (int)chunks_of(v.n, v.lanes, kFirst);
+  const int64_t blocks = v.chunks + (kFirst ? ceil_div(v.vocab, kRunThreads) : 0);
   const dim3 grid((unsigned)blocks, (unsigned)ceil_div(v.D, v.lanes * V));
-  runs_kernel<S, T, V><<<grid, kRunThreads, 0, s>>>(v, src, out);
+  runs_kernel<S, T, V, kWhole><<<grid, kRunThreads, 0, s>>>(v, src, out);
   return v.chunks;
 }
 
-template <typename T, int V>
+template <typename T, int V, bool kWhole>
 static int gradient(int64_t n, int32_t vocab, int32_t dim, Tokens tokens, const T* grad, float scale, int64_t padding,
                     T* out, const BackwardPlan& b, hipStream_t s) {
   if (n <= kFew) {
     const int lanes = lanes_of(dim, V);
     const dim3 grid((unsigned)(n + ceil_div(vocab, kThreads)), (unsigned)ceil_div(dim, lanes * V));
-    few_kernel<T, V><<<grid, kThreads, 0, s>>>(tokens, (int)n, (u32)vocab, padding, dim, lanes, scale, grad, out);
+    few_kernel<T, V, kWhole><<<grid, kThreads, 0, s>>>(tokens, (int)n, (u32)vocab, padding, dim, lanes, scale, grad, out);
     return gs_status_from_hip(hipGetLastError());
   }
   keys_kernel<<<(unsigned)min(ceil_div(n, kThreads), (int64_t)8192), kThreads, 0, s>>>(tokens, n, (u32)vocab, padding,
@@ -530,7 +574,7 @@ static int gradient(int64_t n, int32_t vocab, int32_t dim, Tokens tokens, const 
   v.next_keys = b.next_keys[0];
   v.next = b.next[0];
   v.next_ld = b.next_ld;
-  int64_t chunks = runs<T, T, V>(v, grad, out, true, s);
+  int64_t chunks = runs<true, T, T, V, kWhole>(v, grad, out, s);
   // a level of one chunk hands nothing on
   for (int level = 1; chunks > 1; ++level) {
     const int from = (level - 1) & 1, to = level & 1;
@@ -540,7 +584,7 @@ static int gradient(int64_t n, int32_t vocab, int32_t dim, Tokens tokens, const 
     v.ld = b.next_ld;
     v.next_keys = b.next_keys[to];
     v.next = b.next[to];
-    chunks = runs<float, T, V>(v, b.next[from], out, false, s);
+    chunks = runs<false, float, T, V, kWhole>(v, b.next[from], out, s);
   }
   return gs_status_from_hip(hipGetLastError());
 }
@@ -553,11 +597,9 @@ static int backward(int64_t n, int32_t vocab, int32_t dim, Tokens tokens, const 
     zero_kernel<T><<<(unsigned)min(ceil_div(all, kThreads), (int64_t)8192), kThreads, 0, s>>>((T*)out, all);
     return gs_status_from_hip(hipGetLastError());
   }
-  const int v = vector_of<T>(dim, dim, grad, out);
-  if (v == 16 / (int)sizeof(T))
-    return gradient<T, 16 / sizeof(T)>(n, vocab, dim, tokens, (const T*)grad, scale, padding, (T*)out, b, s);
-  if (v == 2) return gradient<T, 2>(n, vocab, dim, tokens, (const T*)grad, scale, padding, (T*)out, b, s);
-  return gradient<T, 1>(n, vocab, dim, tokens, (const T*)grad, scale, padding, (T*)out, b, s);
+  return with_vectors<T>(dim, dim, grad, out, [&](auto V, auto kWhole) {
+    return gradient<T, V, kWhole>(n, vocab, dim, tokens, (const T*)grad, scale, padding, (T*)out, b, s);
+  });
 }
 
 static int check(int64_t n, int32_t vocab, int32_t dim, int32_t dtype, const void* tokens, int32_t bits, float scale) {
@@ -586,7 +628,7 @@ extern "C" int gs_embed_fwd(int64_t n, int32_t vocab, int32_t dim, int32_t dtype
 
 extern "C" size_t gs_embed_bwd_workspace_bytes(int64_t n, int32_t vocab, int32_t dim, int32_t dtype) {
   if (n <= 0 || vocab <= 0 || dim <= 0 || dtype < GS_FP32 || dtype > GS_FP16 || n > 0x7fffffffll) return 0;
-  return gs_embed::BackwardPlan(n, dim, nullptr).bytes;
+  return gs_embed::BackwardPlan(n, dim, gs_embed::vector_of(dtype, dim), nullptr).bytes;
 }
 
 extern "C" int gs_embed_bwd(int64_t n, int32_t vocab, int32_t dim, int32_t dtype, const void* tokens,
@@ -598,7 +640,7 @@ extern "C" int gs_embed_bwd(int64_t n, int32_t vocab, int32_t dim, int32_t dtype
   const size_t need = gs_embed_bwd_workspace_bytes(n, vocab, dim, dtype);
   if (need > 0 && ((uintptr_t)workspace & 255)) return GS_ERR_MISALIGNED;
   if (need > 0 && (!workspace || workspace_bytes < need)) return GS_ERR_SCRATCH_TOO_SMALL;
-  const gs_embed::BackwardPlan b(n, dim, workspace);
+  const gs_embed::BackwardPlan b(n, dim, gs_embed::vector_of(dtype, dim), workspace);
   const gs_embed::Tokens t = {tokens, token_bits};
   hipStream_t s = (hipStream_t)stream;
   if (dtype == GS_FP32)
