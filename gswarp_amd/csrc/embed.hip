@@ -22,6 +22,7 @@ namespace gs_embed {
 typedef unsigned u32;
 constexpr u32 kNone = 0xffffffffu;  // an entry that holds nothing
 constexpr int kThreads = 256;
+constexpr int64_t kMaxLookup = 1ll << 31;  // vectors of a launch of the lookup
 
 static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
@@ -32,6 +33,7 @@ struct Tokens {
   __device__ __forceinline__ int64_t at(int64_t i) const {
     return bits == 64 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
   }
+  Tokens from(int64_t i) const { return {(const char*)p + i * (bits / 8), bits}; }
 };
 
 // Rows are moved in vectors of 16 bytes (V elements), or, shorter ones, element by
@@ -465,10 +467,14 @@ template <typename T>
 static int forward(int64_t n, int32_t vocab, int32_t dim, Tokens tokens, const void* table, int64_t ld, float scale,
                    void* out, hipStream_t s) {
   return with_vectors<T>(dim, ld, table, out, [&](auto V, auto kWhole) {
-    const int64_t row_vectors = ceil_div(dim, V), blocks = ceil_div(n * row_vectors, kThreads);
-    if (blocks > 0x7fffffffll) return (int)GS_ERR_OVERFLOW;
-    lookup_kernel<T, V, kWhole><<<(unsigned)blocks, kThreads, 0, s>>>(tokens, n, (u32)vocab, dim, (u32)row_vectors,
-                                                                     (const T*)table, ld, scale, (T*)out);
+    const int64_t row_vectors = ceil_div(dim, V);
+    // a launch has fewer than 2^32 threads
+    const int64_t most = max((int64_t)1, kMaxLookup / row_vectors);
+    for (int64_t i = 0; i < n; i += most) {
+      const int64_t here = min(most, n - i);
+      lookup_kernel<T, V, kWhole><<<(unsigned)ceil_div(here * row_vectors, kThreads), kThreads, 0, s>>>(
+          tokens.from(i), here, (u32)vocab, dim, (u32)row_vectors, (const T*)table, ld, scale, (T*)out + i * dim);
+    }
     return gs_status_from_hip(hipGetLastError());
   });
 }
@@ -480,7 +486,7 @@ static int lanes_of(int D, int V) {
   return lanes;
 }
 
-// Entries of a group.  On the first level 4 to 64, by how many make 1024 chunks,
+// Entries of a group.  On the first level 4 to 64, by how many make 512 chunks,
 // which fill the chip; above, all of them where that is 8 at most, else 8 and on,
 // so that at most 64 chunks hand on to the next level: few levels, and none that
 // leaves many rows to one workgroup (2048 rows of 256 bytes take one 43 us).
@@ -490,7 +496,7 @@ static int group_length(int64_t n, int lanes, bool first) {
   // between two entries of a run is one at most, and before the part)
   if (!first && n <= groups * min(8, most)) return (int)round_up(ceil_div(n, groups), 2);
   int length = first ? 4 : min(8, most);
-  while (2 * length <= most && n / (length * groups) > (first ? 1024 : 64)) length *= 2;
+  while (2 * length <= most && n / (length * groups) > (first ? 512 : 64)) length *= 2;
   return min(length, most);
 }
 

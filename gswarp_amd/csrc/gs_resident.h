@@ -68,7 +68,7 @@ struct Args {
 
 // The held rows' matrix-core operands: lane l holds row l % 32 of the wave's, columns 16 s + 8 (l / 32) ..+7.
 template <typename T, int KB, int PL>
-struct Held {
+struct HeldRows {
   typename Pack<T>::v8 v[PL][4 * KB];
   // row: the lane's row of the operand (any; none: nothing but zeros)
   __device__ __forceinline__ void load(const Operand& o, int64_t row, bool some, int dim) {
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(kThreads, kKind == kForward && KB * PL <= 2 ? 4 : 2
   const int held_row = blockIdx.x * kHeldRows + wave * 32 + (lane & 31);
   const bool held_in = held_row < a.held.extent;
 
-  Held<T, KB, PL> held;
+  HeldRows<T, KB, PL> held;
   RowInfo row = {0.0f, 0.0f, 0.0f, -1};
   bool counts = held_in;
   if (kKind == kForward) {
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(kThreads, kKind == kForward && KB * PL <= 2 ? 4 : 2
     held.load(a.held, held_row, counts, a.dim);
     if (blockIdx.y == 0) {
       // the label's logit: the diagonal of the labels' rows against the held ones
-      Held<T, KB, PL> at_label;
+      HeldRows<T, KB, PL> at_label;
       at_label.load(a.stream, max(label, 0), label >= 0, a.dim);
       f32x16 s;
       logits<T, KB, PL>(s, [&](int p, int k) { return at_label.v[p][k]; }, [&](int p, int k) { return held.v[p][k]; });

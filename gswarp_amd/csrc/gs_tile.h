@@ -106,9 +106,10 @@ struct Stage {
   static constexpr int kRowVectors = kAlongK ? 8 : BT / 8;      // 16-byte chunks of a row of the layout
   static constexpr int kLoadRows = 64 / kRowVectors;            // rows of the layout that an instruction fills
   static_assert(kLoads * kWaves * 1024 == kBytes, "every wave issues the same loads");
+  static_assert(kAlongK || BT >= 128, "the four K rows of a transposing load need four chunks to lie apart in");
 
   static __device__ __forceinline__ int spread(int i) { return ((i >> 2) & 3) | ((i << 1) & 4); }
-  static __device__ __forceinline__ int turn(int k) { return BT >= 128 ? 2 * (k & 3) : 2 * ((k >> 1) & 1); }
+  static __device__ __forceinline__ int turn(int k) { return 2 * (k & 3); }
 
   // Byte offsets of the lane's chunk from the step's first element, for
   // instructions of even and of odd number (the permutation repeats every two).

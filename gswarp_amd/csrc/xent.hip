@@ -27,12 +27,10 @@ using gs_tile::Operand;
 
 // The tile shapes (BM, BN, waves along each, stages).  Big has twice Mid's reuse
 // of what it loads and one workgroup a CU; Mid wastes less on small sides and
-// two of its workgroups overlap.  Narrow: gradients of at most 64 columns.
-// Thin: few rows, where the table streams through once and what counts is how
+// two of its workgroups overlap.  Thin: few rows, where the table streams through once and what counts is how
 // many bytes are under way (two workgroups a CU, four or five steps each).
 typedef gs_tile::Shape<256, 256, 2, 4> Big;
 typedef gs_tile::Shape<128, 128, 2, 2> Mid;
-typedef gs_tile::Shape<64, 256, 1, 4> Narrow;
 typedef gs_tile::Shape<64, 32, 2, 1, 6> Thin32;
 typedef gs_tile::Shape<64, 64, 2, 1, 5> Thin64;
 
@@ -642,13 +640,14 @@ struct Problem {
 };
 
 constexpr int64_t kMaxRows = (1ll << 31) - 1024;
+constexpr int64_t kMaxVocab = 1ll << 29;
 
 static int check(const Problem& p) {
   if (p.rows < 0 || p.vocab <= 0 || p.dim <= 0 || p.dtype < GS_FP32 || p.dtype > GS_FP16)
     return GS_ERR_INVALID_ARGUMENT;
   if (p.ld_features < p.dim || p.ld_table < p.dim) return GS_ERR_INVALID_ARGUMENT;
-  // (indices of rows, rounded up to a tile, are int32)
-  if (p.rows > kMaxRows || p.vocab > kMaxRows || p.dim > gs_tile::kMaxLd - 8) return GS_ERR_OVERFLOW;
+  // (indices of rows, rounded up to a tile, are int32, and a launch has fewer than 2^32 threads)
+  if (p.rows > kMaxRows || p.vocab > kMaxVocab || p.dim > gs_tile::kMaxLd - 8) return GS_ERR_OVERFLOW;
   return GS_OK;
 }
 
@@ -734,7 +733,10 @@ struct State {
 // Short rows: the kernels that hold one operand in registers (gs_resident.h).
 // The forward alone needs fewer of them, and goes twice as far.
 static bool resident(const Problem& p) { return p.dp() <= (p.dtype == GS_FP32 ? 64 : 128); }
-static bool resident_forward(const Problem& p) { return p.dp() <= (p.dtype == GS_FP32 ? 128 : 256); }
+static bool resident_forward(const Problem& p) {
+  const int64_t blocks = ceil_div(p.dp(), 64) * p.planes();
+  return blocks <= 4 && p.rows * p.vocab >= blocks * (3ll << 22);
+}
 // Two workgroups of a forward on rows of one or two 128-byte blocks (counting planes) share a CU, else one has it.
 static int resident_forward_slots(const Problem& p) { return ceil_div(p.dp(), 64) * p.planes() <= 2 ? 512 : 256; }
 
@@ -797,6 +799,12 @@ static void with_logits_shape(int64_t vocab, int64_t rows, F f) {
   f(Mid{});
 }
 
+template <class S>
+static int64_t tiles_of(const Problem& p) {
+  return ceil_div(p.vocab, S::BM) * ceil_div(p.rows, S::BN);
+}
+constexpr int64_t kThinTiles = 512;
+
 struct ForwardPlan {
   enum { kThin32, kThin64, kResident, kMid, kBig } shape;
   int64_t rows_piece, tiles_m, blocks;
@@ -809,13 +817,13 @@ struct ForwardPlan {
 
   // kept: the layouts lie in a state
   ForwardPlan(const Problem& p, bool kept, void* ws) {
-    shape = p.rows <= 32 ? kThin32 : p.rows <= 64 ? kThin64 : resident_forward(p) ? kResident
-            : takes_big(p.vocab, p.rows) ? kBig : kMid;
+    shape = tiles_of<Thin32>(p) <= kThinTiles ? kThin32 : tiles_of<Thin64>(p) <= kThinTiles ? kThin64
+            : resident_forward(p) ? kResident : takes_big(p.vocab, p.rows) ? kBig : kMid;
     const int bm = shape == kBig ? Big::BM : shape == kMid ? Mid::BM : Thin32::BM;
     tiles_m = shape == kResident ? resident_parts(p.rows, p.vocab, resident_forward_slots(p), 0.0) : ceil_div(p.vocab, bm);
     rows_piece = max((int64_t)256, kStatBytes / (tiles_m * (int64_t)sizeof(float2)) / 256 * 256);
     rows_piece = min(p.rows, min(rows_piece, (int64_t)1 << 20));
-    lanes = p.rows <= 4096 ? 64 : 1;
+    lanes = p.rows <= 4096 && tiles_m >= 16 ? 64 : 1;
     blocks = 0;
     for (int64_t r = 0; r < p.rows; r += rows_piece)
       blocks += ceil_div(min(rows_piece, p.rows - r), kJoinThreads / lanes);
@@ -881,37 +889,45 @@ static int forward(const Problem& p, Targets targets, float logit_scale, int red
   return gs_status_from_hip(hipGetLastError());
 }
 
-// The shape of a gradient's tiles, D columns of m: 64 wide where D fits, else 256
-// unless 128 leaves so much less of the last tile empty that its smaller reuse pays.
-enum class Columns { kNarrow, kMid, kBig };
-static Columns columns_of(int64_t D) {
-  if (D <= Narrow::BM) return Columns::kNarrow;
-  return round_up(D, Big::BM) * 100 <= round_up(D, Mid::BM) * 115 ? Columns::kBig : Columns::kMid;
+// How a gradient's product of (N x D) over K is done: in which tiles, and in how
+// many parts along K.  The time in microseconds: whole rounds of the chip's 256
+// CUs (one Big workgroup each, or two Mid ones), each a part's steps and about
+// four steps' time to begin and end; and what it takes to write and add the parts' fp32 sums.
+struct Split {
+  bool big;
+  int parts;
+};
+static Split split_of(int64_t N, int64_t D, int64_t K, int products) {
+  Split best = {true, 1};
+  double least = 1e300;
+  const int64_t steps = ceil_div(K, kBK) * products;
+  for (int big = 0; big < 2; ++big) {
+    const int64_t tiles = big ? ceil_div(N, Big::BN) * ceil_div(D, Big::BM) : ceil_div(N, Mid::BN) * ceil_div(D, Mid::BM);
+    const int64_t most = max((int64_t)1, min(K / (4 * kBK), (int64_t)256));
+    for (int64_t n = 1; n <= most; ++n) {
+      const int64_t blocks = tiles * n;
+      const double round = big ? 2.1 * ceil_div(blocks, 256) : blocks <= 256 ? 0.8 : 1.24 * ceil_div(blocks, 512);
+      const double cost = round * (double)(ceil_div(steps, n) + 4) + (n > 1 ? 3.0 + (double)n * N * D * 8.0 / 4.0e6 : 0.0);
+      if (cost < least) {
+        least = cost;
+        best = {big == 1, (int)n};
+      }
+    }
+  }
+  return best;
 }
 
+// Calls f with a value of the shape.
 template <class F>
-static void with_columns(Columns c, F f) {
-  if (c == Columns::kNarrow) f(Narrow{});
-  else if (c == Columns::kMid) f(Mid{});
-  else f(Big{});
-}
-
-// How many parts a gradient's product of (N x D) over K is cut into along K, so
-// that the launch fills the chip (512 workgroups where two share a CU); a part has at least four steps.
-static int parts_for(int64_t N, int64_t D, int64_t K) {
-  int64_t want = 1;
-  with_columns(columns_of(D), [&](auto shape) {
-    typedef decltype(shape) S;
-    const int64_t tiles = ceil_div(N, S::BN) * ceil_div(D, S::BM);
-    const int64_t fill = 2 * S::kLdsBytes <= 160 * 1024 ? 512 : 256;
-    want = tiles * 4 >= fill * 3 ? 1 : ceil_div(fill, tiles);
-  });
-  return (int)max((int64_t)1, min(want, K / (4 * kBK)));
+static void with_shape(bool big, F f) {
+  if (big) f(Big{});
+  else f(Mid{});
 }
 
 struct BackwardPlan {
   int64_t rows_piece, cols_piece, ld, row_pieces, col_pieces;
-  int parts_h, parts_t;  // parts along K of dh and dw
+  int parts_h, parts_t;  // parts along K of dh and dw, and their tiles
+  bool big_h, big_t;
   bool direct_h, direct_t;  // one part and one piece: no fp32 sums in between
   uint16_t* ds;
   RowInfo* info;
@@ -941,8 +957,12 @@ struct BackwardPlan {
       cols_piece = min((int64_t)p.vocab, most / rows_piece / 256 * 256);
     }
     ld = round_up(cols_piece, 256);
-    parts_h = want_h ? parts_for(rows_piece, p.dim, cols_piece) : 1;
-    parts_t = want_t ? parts_for(cols_piece, p.dim, rows_piece) : 1;
+    const Split h = split_of(rows_piece, p.dim, cols_piece, p.ds_products());
+    const Split t = split_of(cols_piece, p.dim, rows_piece, p.ds_products());
+    big_h = h.big;
+    big_t = t.big;
+    parts_h = want_h ? h.parts : 1;
+    parts_t = want_t ? t.parts : 1;
     carve(p, want_h, want_t, ws);
   }
 
@@ -1037,10 +1057,10 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
             piece, features, (int)p.dp(), p.products(), scale2, layouts.units, (int32_t)c, tiles_m, tiles_n,
             b.info + r, counts, b.ds, b.ld, ds_plane);
       });
-      with_columns(columns_of(D), [&](auto shape) {
-        typedef decltype(shape) S;
-        const int tiles_m = (int)ceil_div(D, S::BM);
-        if (grad_features) {
+      if (grad_features) {
+        with_shape(b.big_h, [&](auto shape) {
+          typedef decltype(shape) S;
+          const int tiles_m = (int)ceil_div(D, S::BM);
           const Operand ds = {b.ds, b.ld, ds_plane, rows};
           Operand x = piece;  // D columns of the piece's rows
           x.extent = D;
@@ -1049,8 +1069,12 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
           grad_kernel<S, T, Out, false><<<dim3((unsigned)((int64_t)tiles_m * tiles_n), b.parts_h), S::kThreads, 0, s>>>(
               x, ds, cols, k_part, p.ds_products(), counts, tiles_m, tiles_n, b.direct_h ? nullptr : b.part_h,
               (int64_t)rows * D, c > 0, b.alpha, unit_w, grad_features + r * D);
-        }
-        if (grad_table) {
+        });
+      }
+      if (grad_table) {
+        with_shape(b.big_t, [&](auto shape) {
+          typedef decltype(shape) S;
+          const int tiles_m = (int)ceil_div(D, S::BM);
           const Operand ds = {b.ds, b.ld, ds_plane, cols};
           Operand x = features;
           x.extent = D;
@@ -1063,8 +1087,8 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
               grad_table + c * D);
           if (part && b.row_pieces == 1)
             finish<T>(part, b.parts_t, part_plane, (int64_t)cols * D, D, nullptr, b.alpha, unit_h, grad_table + c * D, s);
-        }
-      });
+        });
+      }
     }
     if (grad_features && !b.direct_h)
       finish<T>(b.part_h, b.parts_h, (int64_t)rows * D, (int64_t)rows * D, D, counts, b.alpha, unit_w, grad_features + r * D, s);
@@ -1164,6 +1188,7 @@ extern "C" int gs_xent_bwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dty
   }
   if (!targets || !state || !grad_loss || !count) return GS_ERR_INVALID_ARGUMENT;
   if ((status = gs_xent::check_pointers(p)) != GS_OK) return status;
+  if (((uintptr_t)grad_features & 15) || ((uintptr_t)grad_table & 15)) return GS_ERR_MISALIGNED;
   if (((uintptr_t)workspace & 255) || ((uintptr_t)state & 255)) return GS_ERR_MISALIGNED;
   const bool want_h = grad_features != nullptr, want_t = grad_table != nullptr;
   if (!workspace || workspace_bytes < gs_xent::BackwardPlan(p, want_h, want_t, nullptr).bytes)

@@ -27,13 +27,14 @@ _INDEX_BITS = {torch.int32: 32, torch.int64: 64}
 _REDUCTIONS = {"none": _lib.GS_REDUCE_NONE, "sum": _lib.GS_REDUCE_SUM, "mean": _lib.GS_REDUCE_MEAN}
 _INT32_MAX = 2**31 - 1
 _MAX_DIM = 2**21 - 8
+_MAX_CLASSES = 2**29
 _FP32_MAX = torch.finfo(torch.float32).max
 
 
-def _check_table(table, name: str) -> None:
+def _check_table(table, name: str, most: int = _INT32_MAX) -> None:
     if isinstance(table, torch.Tensor) and table.is_cuda and table.dtype in _DTYPES and table.ndim == 2:
         vocab, dim = table.shape
-        if 0 < vocab <= _INT32_MAX and 0 < dim <= _MAX_DIM:
+        if 0 < vocab <= most and 0 < dim <= _MAX_DIM:
             return
     if not isinstance(table, torch.Tensor) or not table.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
@@ -41,7 +42,7 @@ def _check_table(table, name: str) -> None:
         raise ValueError(f"{name} must have dtype float32, bfloat16 or float16, got {table.dtype}")
     if table.ndim != 2 or table.shape[0] == 0 or table.shape[1] == 0:
         raise ValueError(f"{name} must have shape (vocabulary, dim), got {tuple(table.shape)}")
-    raise ValueError(f"{name} must have at most 2**31 - 1 rows of at most 2**21 - 8 values")
+    raise ValueError(f"{name} must have at most {most} rows of at most {_MAX_DIM} values")
 
 
 def _check_indices(indices, name: str, device: torch.device) -> None:
@@ -227,8 +228,10 @@ def linear_cross_entropy(features: torch.Tensor, table: torch.Tensor, targets: t
     ``"mean"`` over the rows that count (NaN over none).  Rows whose target is ``ignore_index`` do not
     count: their loss and gradient are zero and they bring nothing to the table's gradient, whatever
     their features hold.  Any other target outside the vocabulary makes its row's loss NaN.
+    The logits' gradients enter the products in the inputs' type (float32: with 22 bits or more, in
+    steps of 2**-62 of the largest row's), and so rounded they decide the gradients' precision.
     """
-    _check_table(table, "table")
+    _check_table(table, "table", _MAX_CLASSES)
     device, dim = table.device, table.shape[1]
     if not isinstance(features, torch.Tensor) or features.device != device:
         raise ValueError(f"features must be a tensor on {device}")

@@ -610,7 +610,8 @@ int gs_embed_bwd(int64_t n, int32_t vocab, int32_t dim, int32_t dtype, const voi
  * GS_REDUCE_NONE, the number of rows that count, which gs_xent_bwd takes too.
  * features and table must be 16-byte aligned unless they are fp32 or have a dim
  * or row distance that is not a multiple of 8 (those are laid out first).  workspace:
- * gs_xent_fwd_workspace_bytes bytes on 256, of any content.
+ * gs_xent_fwd_workspace_bytes bytes on 256, of any content.  At most 2^29 rows of
+ * the table and 2^31 - 1024 of the features (else GS_ERR_OVERFLOW).
  */
 size_t gs_xent_state_bytes(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, int64_t ld_features,
                            int64_t ld_table);
@@ -623,7 +624,7 @@ int gs_xent_fwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const v
 
 /*
  * The gradients of gs_xent_fwd: grad_features (rows x dim) and grad_table
- * (vocab x dim), contiguous, either may be NULL (not computed); the logits
+ * (vocab x dim), contiguous, on 16 bytes, either may be NULL (not computed); the logits
  * are formed again, a piece of rows and vocabulary at a time.  grad_loss:
  * `rows` fp32 for GS_REDUCE_NONE, else one.  Rows that do not count get zero
  * and bring nothing, whatever their features hold.  The other arguments are the forward's.

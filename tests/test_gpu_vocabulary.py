@@ -495,3 +495,75 @@ def test_language_scene_learns(device):
 
     losses = train(steps=12, count=4000, size=128)
     assert all(math.isfinite(x) for x in losses) and losses[-1] < 0.8 * losses[0]
+
+
+def _marked(rows, dim, gen):
+    """A few hundred row numbers: the ends, and both sides of the offsets that pass 2^31 and 2^32 bytes and elements."""
+    at = [0, 1, rows - 1, rows - 2]
+    for size in (2 ** 30, 2 ** 31, 2 ** 32):
+        at += [r for r in (size // dim - 1, size // dim, size // dim + 1) if r < rows]
+    return torch.cat([torch.tensor(at), torch.randint(0, rows, (300,), generator=gen)]).unique()
+
+
+@pytest.mark.parametrize("dtype,rows,vocab,dim", [(BF16, 2 ** 24 + 5, 100, 136), (FP16, 2 ** 25 + 3, 70, 72),
+                                                  (FP32, 2 ** 25 + 3, 50, 40), (FP32, 2 ** 23 + 1, 50, 260)])
+def test_entropy_of_rows_past_32_bits(device, dtype, rows, vocab, dim):
+    """The marked rows' losses, and gradients where only they have one; the others' terms are exact zeros."""
+    print(f"entropy {dtype} rows={rows} vocab={vocab} dim={dim}", flush=True)
+    gen = _gen(dim)
+    marked = _marked(rows, dim, gen).to(device)
+    features = torch.full((rows, dim), 0.25, dtype=dtype, device=device)
+    features[marked] = torch.randn(len(marked), dim, generator=gen).to(device, dtype)
+    table = (torch.randn(vocab, dim, generator=gen) / math.sqrt(dim)).to(device, dtype).requires_grad_(True)
+    targets = torch.randint(0, vocab, (rows,), generator=gen, dtype=torch.int32).to(device)
+    up = torch.zeros(rows, device=device)
+    up[marked] = torch.rand(len(marked), generator=gen).to(device) + 0.5
+    features.requires_grad_(True)
+    loss = vocabulary.linear_cross_entropy(features, table, targets, reduction="none")
+    want = ref.entropy(features.detach()[marked], table.detach(), targets[marked], up[marked], reduction="none")
+    ref.check(loss.detach()[marked], want["loss"], "loss")
+    grad_features, grad_table = torch.autograd.grad(loss, (features, table), up)
+    ref.check(grad_features[marked], want["features"], "features")
+    ref.check(grad_table, want["table"], "table")
+    grad_features[marked] = 0
+    assert not grad_features.any()
+
+
+@pytest.mark.parametrize("dtype,rows,vocab,dim", [(BF16, 33, 2 ** 24 + 5, 136), (FP16, 300, 2 ** 25 + 1, 72),
+                                                  (FP32, 70, 2 ** 23 + 1, 136), (BF16, 300, 2 ** 23 + 1, 264)])
+def test_entropy_of_tables_past_32_bits(device, dtype, rows, vocab, dim):
+    """Marked rows of the table hold all but 2^-30 of every probability; the others are zeros, of logit 0."""
+    print(f"entropy {dtype} rows={rows} vocab={vocab} dim={dim}", flush=True)
+    gen = _gen(dim)
+    marked = _marked(vocab, dim, gen).to(device)
+    table = torch.zeros(vocab, dim, dtype=dtype, device=device)
+    table[marked] = (torch.randn(len(marked), dim, generator=gen) / math.sqrt(dim)).to(device, dtype)
+    features = (30.0 * torch.sign(torch.randn(rows, dim, generator=gen))).to(device, dtype).requires_grad_(True)
+    label = torch.randint(0, len(marked), (rows,), generator=gen).to(device)
+    few = table[marked]
+    lse = torch.logsumexp(features.detach().double() @ few.double().T, 1)
+    rest = vocab * torch.exp(-lse)
+    assert float(rest.max()) < 2.0 ** -30
+    up = torch.rand(rows, generator=gen).to(device) + 0.5
+    want = ref.entropy(features.detach(), few, label, up, reduction="none")
+    table.requires_grad_(True)
+    loss = vocabulary.linear_cross_entropy(features, table, marked[label], reduction="none")
+    ref.check(loss, want["loss"], "loss")
+    grad_features, grad_table = torch.autograd.grad(loss, (features, table), up)
+    ref.check(grad_features, want["features"], "features")
+    value, bound = want["table"]
+    if dtype == FP32:
+        # the gradients of the logits are held as three planes of 22 bits in steps of 2^-62 of the largest
+        bound = bound + 2.0 ** -62 * up.max().double() * features.detach().double().abs().sum(0)
+    ref.check(grad_table[marked], (value, bound), "table")
+    grad_table[marked] = 0
+    assert float(grad_table.abs().max()) <= rows * 30.0 * 1.5 * 2.0 ** -30
+
+
+def test_lookup_of_more_vectors_than_a_launch_has_threads(device):
+    n, dim = 2 ** 30 + 77, 16  # two vectors a row
+    table = torch.randn(5, dim, generator=_gen(4)).to(device, BF16)
+    tokens = torch.arange(n, dtype=torch.int32, device=device) % 5
+    out = vocabulary.embed_tokens(tokens, table)
+    for at in (0, 2 ** 27, 2 ** 28, 2 ** 29, 2 ** 30 - 100, n - 100):
+        assert torch.equal(out[at:at + 100], table[tokens[at:at + 100]])

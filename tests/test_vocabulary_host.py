@@ -99,3 +99,12 @@ def test_reference_agrees_with_autograd():
         assert torch.allclose(loss, f32["loss"][0], atol=1e-5)
         assert torch.allclose(grads[0], f32["features"][0], atol=1e-5)
         assert torch.allclose(grads[1], f32["table"][0], atol=1e-5)
+
+
+def test_limits_and_alignment_of_gradients(lib):
+    p = 4096
+    sizes = (4, 10, 16, 1, p, 16, p, 16, p, 64, -100, 1.0, 2)
+    assert lib.gs_xent_bwd(*sizes, p, p, p, p + 8, p, p, 1 << 40, None) == -2
+    assert lib.gs_xent_bwd(*sizes, p, p, p, p, p + 4, p, 1 << 40, None) == -2
+    wide = (4, 2 ** 29 + 1, 16, 1, p, 16, p, 16, p, 64, -100, 1.0, 2)
+    assert lib.gs_xent_fwd(*wide, p, p, p, p, 1 << 40, None) == -4
