@@ -47,10 +47,10 @@ constexpr int kStages = 4;
 
 struct Args {
   Operand held, stream;
-  int32_t part;  // stream rows of a part (blockIdx.y), a multiple of the tile's
   int32_t dim;   // of the operands, padded to 8
   float logit_scale2;
   const float* units;
+  gs_xent::Order order;  // of the features' rows
   // kForward: stats[part * rows + row], and the rows' labels' dot products, upright
   float* label_dot;
   gs_xent::Targets targets;
@@ -151,11 +151,18 @@ __global__ __launch_bounds__(kThreads, kKind == kForward && KB * PL <= 2 ? 4 : 2
   const int held_row = blockIdx.x * kHeldRows + wave * 32 + (lane & 31);
   const bool held_in = held_row < a.held.extent;
 
+  // what there is to do of the features; the parts (blockIdx.y) share the streamed rows in whole tiles
+  const int held_used = kKind == kTable ? a.held.extent : a.order.used(a.held.extent);
+  const int stream_used = kKind == kTable ? a.order.used(a.stream.extent) : a.stream.extent;
+  const bool idle = (int)(blockIdx.x * kHeldRows) >= held_used;  // none of the held rows count
+  if (kKind == kForward && idle) return;
+  const int64_t part = (((int64_t)stream_used + gridDim.y - 1) / gridDim.y + kTileRows - 1) / kTileRows * kTileRows;
+
   HeldRows<T, KB, PL> held;
   RowInfo row = {0.0f, 0.0f, 0.0f, -1};
   bool counts = held_in;
   if (kKind == kForward) {
-    const int64_t target = held_in ? a.targets.at(held_row) : -1;
+    const int64_t target = held_in ? a.targets.at(a.order.row(held_row)) : -1;
     const int label = target >= 0 && target < a.stream.extent ? (int)target : -1;
     counts = held_in && target != a.targets.ignore;
     held.load(a.held, held_row, counts, a.dim);
@@ -180,9 +187,9 @@ __global__ __launch_bounds__(kThreads, kKind == kForward && KB * PL <= 2 ? 4 : 2
   // loop would be one for the ring's loads as well.  (vmcnt 0, nothing else)
   constexpr int kWaitLoads = 0x0f70;
   __builtin_amdgcn_s_waitcnt(kWaitLoads);
-  const int begin = (int)min((int64_t)a.stream.extent, (int64_t)blockIdx.y * a.part);
-  const int end = (int)min((int64_t)a.stream.extent, (int64_t)begin + a.part);
-  const int tiles = (end - begin + kTileRows - 1) / kTileRows;
+  const int begin = (int)min((int64_t)stream_used, blockIdx.y * part);
+  const int end = (int)min((int64_t)stream_used, begin + part);
+  const int tiles = idle ? 0 : (end - begin + kTileRows - 1) / kTileRows;
 
   Stage stage;
   stage.init(a.stream, 0);
@@ -435,7 +442,8 @@ __global__ __launch_bounds__(kThreads, kKind == kForward && KB * PL <= 2 ? 4 : 2
           if constexpr (PL > 1)
             v[j] += (acc[1][d][4 * q + j] + acc[2][d][4 * q + j] * (1.0f / kPlaneStep)) * (1.0f / kPlaneStep);
         }
-        const int64_t at = (int64_t)held_row * a.D + first;
+        const int64_t to_row = kKind == kFeatures && !a.part_sums ? a.order.row(held_row) : (int64_t)held_row;
+        const int64_t at = to_row * a.D + first;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           v[j] = !counts ? 0.0f : a.part_sums ? v[j] : gs_xent::gradient_of<T>(v[j], factor);

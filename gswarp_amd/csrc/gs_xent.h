@@ -14,9 +14,19 @@ struct Targets {
   __device__ __forceinline__ int64_t at(int64_t i) const {
     return bits == 64 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
   }
-  __host__ __device__ Targets from(int64_t row) const {
-    return {(const char*)p + row * (bits / 8), bits, ignore};
-  }
+};
+
+// The order in which the rows of the features are taken: as they are (at null), or
+// those that count first and the others behind, each in their order, so that the
+// products are formed for `count` rows only.  A kernel works on a piece of it from `first`.
+struct Order {
+  const int* at;
+  const int* count;
+  int32_t first;
+  __device__ __forceinline__ int64_t row(int i) const { return at ? at[first + i] : (int64_t)first + i; }
+  // how many of the piece's n rows have to be looked at
+  __device__ __forceinline__ int32_t used(int32_t n) const { return at ? max(0, min(n, *count - first)) : n; }
+  Order from(int64_t i) const { return {at, count, (int32_t)i}; }
 };
 
 // What the dot products of laid-out rows are multiplied by for base-2 logits:

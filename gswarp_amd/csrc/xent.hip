@@ -52,6 +52,65 @@ struct Matrix {
   int64_t plane;
 };
 
+// The order of the rows (struct Order), where it is worth a copy of them.  Each
+// workgroup takes `share` rows; counts[b]: how many of workgroup b's count.
+constexpr int kOrderBlocks = 1024;
+__device__ __forceinline__ bool row_is_used(const Targets& targets, int64_t row, int64_t end) {
+  return row < end && targets.at(row) != targets.ignore;
+}
+
+__global__ __launch_bounds__(256) void used_kernel(Targets targets, int64_t rows, int64_t share,
+                                                   int* __restrict__ counts) {
+  __shared__ int lds[4];
+  const int64_t begin = blockIdx.x * share, end = min(rows, begin + share);
+  int n = 0;
+  for (int64_t r = begin; r < end; r += 256) n += __builtin_popcountll(__ballot(row_is_used(targets, r + threadIdx.x, end)));
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) counts[blockIdx.x] = lds[0] + lds[1] + lds[2] + lds[3];
+}
+
+__global__ __launch_bounds__(256) void order_kernel(Targets targets, int64_t rows, int64_t share,
+                                                    const int* __restrict__ counts, int* __restrict__ order,
+                                                    int* __restrict__ count) {
+  __shared__ int before_lds[4], all_lds[4], wave_lds[2][4];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  int before = 0, all = 0;
+  for (int b = threadIdx.x; b < (int)gridDim.x; b += 256) {
+    all += counts[b];
+    if (b < (int)blockIdx.x) before += counts[b];
+  }
+#pragma unroll
+  for (int off = 32; off; off >>= 1) {
+    before += __shfl_xor(before, off);
+    all += __shfl_xor(all, off);
+  }
+  if (lane == 0) {
+    before_lds[wave] = before;
+    all_lds[wave] = all;
+  }
+  __syncthreads();
+  before = before_lds[0] + before_lds[1] + before_lds[2] + before_lds[3];  // used rows before this one
+  all = all_lds[0] + all_lds[1] + all_lds[2] + all_lds[3];
+  if (blockIdx.x == 0 && threadIdx.x == 0) *count = all;
+  const int64_t begin = blockIdx.x * share, end = min(rows, begin + share);
+  int turn = 0;
+  for (int64_t r = begin; r < end; r += 256, turn ^= 1) {
+    const int64_t row = r + threadIdx.x;
+    const bool use = row_is_used(targets, row, end);
+    const uint64_t who = __ballot(use);
+    if (lane == 0) wave_lds[turn][wave] = __builtin_popcountll(who);
+    __syncthreads();  // (two places in turn: one barrier does)
+    int rank = before + __builtin_popcountll(who & ((1ull << lane) - 1));
+    for (int w = 0; w < 4; ++w) {
+      const int n = wave_lds[turn][w];
+      if (w < wave) rank += n;
+      before += n;
+    }
+    if (row < end) order[use ? (int64_t)rank : all + row - rank] = (int)row;
+  }
+}
+
 // fp32: the largest finite magnitudes of the features (of the rows that count
 // only, so that what ignored rows hold does not reach the unit of the others) and
 // of the table, one value a block, the features' blocks first.  A group of
@@ -117,10 +176,11 @@ __device__ __forceinline__ float unit_of(const float* __restrict__ largest, int 
   return ldexpf(1.0f, max(e - 14, -126));
 }
 
-// Lays two matrices out, the first's blocks first; fp32: their units, from
-// largest (the first's magnitudes, then the second's), go to units[0] and units[1].
+// Lays two matrices out, the first's blocks first, the first's rows in their order;
+// fp32: their units, from largest (the first's magnitudes, then the second's), go to
+// units[0] and units[1].
 template <typename T>
-__global__ __launch_bounds__(256) void layout_kernel(Matrix first, int first_blocks, Matrix second, int dim, int dp,
+__global__ __launch_bounds__(256) void layout_kernel(Matrix first, Order order, int first_blocks, Matrix second, int dim, int dp,
                                                      const float* __restrict__ largest, int first_n, int second_n,
                                                      float* __restrict__ units) {
   const bool other = (int)blockIdx.x >= first_blocks;
@@ -135,11 +195,12 @@ __global__ __launch_bounds__(256) void layout_kernel(Matrix first, int first_blo
   }
   const T* src = (const T*)m.src;
   const uint32_t vectors = dp / 8;
-  const int64_t total = m.rows * vectors;
+  const int64_t total = (other ? m.rows : (int64_t)order.used((int)m.rows)) * vectors;
+  const bool whole = sizeof(T) == 2 && dim % 8 == 0 && m.ld % 8 == 0 && (uintptr_t)src % 16 == 0;
   for (int64_t v = (int64_t)block * 256 + threadIdx.x; v < total; v += (int64_t)blocks * 256) {
     const int64_t row = v / vectors;
     const int col = (int)(v - row * vectors) * 8;
-    const T* s = src + row * m.ld + col;
+    const T* s = src + (other ? row : order.row((int)row)) * m.ld + col;
     uint16_t* d = m.dst + row * dp + col;
     if constexpr (sizeof(T) == 4) {
       gs_tile::f16x8 hi, lo;
@@ -152,6 +213,8 @@ __global__ __launch_bounds__(256) void layout_kernel(Matrix first, int first_blo
       }
       *reinterpret_cast<gs_tile::f16x8*>(d) = hi;
       *reinterpret_cast<gs_tile::f16x8*>(d + m.plane) = lo;
+    } else if (whole) {
+      *reinterpret_cast<gs_tile::u32x4*>(d) = *reinterpret_cast<const gs_tile::u32x4*>(s);
     } else {
       uint16_t out[8];
 #pragma unroll
@@ -191,12 +254,13 @@ template <class S, typename T>
 __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, Operand features, int dim,
                                                                  int products, float logit_scale2,
                                                                  const float* __restrict__ units, Targets targets,
-                                                                 int tiles_m, int tiles_n,
+                                                                 Order order, int tiles_m, int tiles_n,
                                                                  float2* __restrict__ stats,
                                                                  float* __restrict__ label_dot) {
   __shared__ __attribute__((aligned(16))) char lds[S::kLdsBytes];
   const gs_tile::TileAt tile = gs_tile::tile_at(tiles_m, tiles_n);
   const int m0 = tile.m * S::BM, n0 = tile.n * S::BN;
+  if (n0 >= order.used(features.extent)) return;
   Accumulators<S> acc;
   gs_tile::product<S, T, true, true>(acc, table, features, m0, n0, 0, dim, products, nullptr, lds);
 
@@ -216,7 +280,7 @@ __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, 
 #pragma unroll
   for (int b = 0; b < S::kNB; ++b) {
     const int n = n0 + wn + 32 * b + (lane & 31);
-    const int label_at = from_first(n < features.extent ? targets.at(n) : -1, 0, first, S::kWaveM, table.extent);
+    const int label_at = from_first(n < features.extent ? targets.at(order.row(n)) : -1, 0, first, S::kWaveM, table.extent);
     if (__any(label_at >= 0)) {
       float label = 0.0f;
       bool mine = false;
@@ -303,14 +367,14 @@ __device__ __forceinline__ void write_total(Sum s, int reduction, float* loss, i
 
 // Joins the tiles' pairs of each row (kLanes lanes a row, in a fixed order):
 // norm = (x, 1 / sum, the label's dot product) for the backward, and the loss;
-// ignored rows give 0, targets outside the vocabulary NaN.  With a reduction the
+// (by the order's rows; the loss by the features'); ignored rows give 0, targets outside the vocabulary NaN.  With a reduction the
 // block's sum goes to partial[block], or, when there is one block in all, to the result.
 template <int kLanes>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float2* __restrict__ stats,
                                                             const float* __restrict__ label_dot, int rows,
                                                             int tiles, int vocab, float logit_scale2,
                                                             const float* __restrict__ units, Targets targets,
-                                                            int reduction, float4* __restrict__ norm,
+                                                            Order order, int reduction, float4* __restrict__ norm,
                                                             float* __restrict__ loss_rows,
                                                             Sum* __restrict__ partial, bool last,
                                                             float* __restrict__ loss, int64_t* __restrict__ count) {
@@ -326,7 +390,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float2* __rest
     sum = sum * (double)weight(x, all, scale) + osum * (double)weight(ox, all, scale);
     x = all;
   };
-  if (row < rows) {
+  if (row < order.used(rows)) {
     for (int t = sub; t < tiles; t += kLanes) {
       const float2 o = stats[(int64_t)t * rows + row];
       add(o.x, (double)o.y);
@@ -336,7 +400,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float2* __rest
   for (int off = kLanes / 2; off; off >>= 1) add(__shfl_xor(x, off), __shfl_xor(sum, off));
   Sum mine = {0.0, 0};
   if (row < rows && sub == 0) {
-    const int64_t t = targets.at(row);
+    const int64_t from = order.row((int)row), t = targets.at(from);
     float value = 0.0f;
     if (t != targets.ignore) {
       value = t >= 0 && t < vocab ? (float)(log(sum) + kLn2 * (double)scale * ((double)x - (double)label_dot[row]))
@@ -344,7 +408,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float2* __rest
       mine = {(double)value, 1};
     }
     if (norm) norm[row] = make_float4(x, (float)(1.0 / sum), label_dot[row], 0.0f);
-    if (loss_rows) loss_rows[row] = value;
+    if (loss_rows) loss_rows[from] = value;
   }
   if (reduction == GS_REDUCE_NONE) return;
   const Sum s = block_sum(mine, lds);
@@ -383,11 +447,12 @@ __global__ __launch_bounds__(256) void largest_kernel(const float* __restrict__ 
   if (threadIdx.x == 0) largest[blockIdx.x] = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
 }
 
-// Per row: its RowInfo, and one bit: does the row count.  With a gradient for
+// Per row of the order: its RowInfo, and one bit: does the row count.  With a gradient for
 // each row the factors are g_i / G, G the largest, so that ds stays in the 16-bit
 // type's range; alpha holds the rest.
 __global__ __launch_bounds__(256) void rows_kernel(const float* __restrict__ grad, int64_t rows, int vocab,
-                                                   Targets targets, int reduction, const int64_t* __restrict__ count,
+                                                   Targets targets, Order order, int reduction,
+                                                   const int64_t* __restrict__ count,
                                                    const float4* __restrict__ norm, float logit_scale,
                                                    float logit_scale2, const float* __restrict__ units,
                                                    float held_scale, const float* __restrict__ largest, int largest_n,
@@ -409,13 +474,13 @@ __global__ __launch_bounds__(256) void rows_kernel(const float* __restrict__ gra
   const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
   bool use = false;
   if (row < rows) {
-    const int64_t t = targets.at(row);
+    const int64_t from = order.row((int)row), t = targets.at(from);
     const float4 z = norm[row];
     use = t != targets.ignore;
     RowInfo r = {0.0f, 0.0f, 0.0f, -1};
     if (use) {
       const bool in = t >= 0 && t < vocab;
-      const float f = (reduction == GS_REDUCE_NONE ? grad[row] / G : 1.0f) * (in ? held_scale : __builtin_nanf(""));
+      const float f = (reduction == GS_REDUCE_NONE ? grad[from] / G : 1.0f) * (in ? held_scale : __builtin_nanf(""));
       const float scale = fabsf(scale_of(logit_scale2, units));
       r.top = z.x * scale;
       const float off = __builtin_fmaf(z.x, scale, -r.top);
@@ -446,7 +511,7 @@ template <class S, typename T, int kPlanes>
 __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, Operand features, int dim,
                                                                  int products, float logit_scale2,
                                                                  const float* __restrict__ units, int32_t m_base,
-                                                                 int tiles_m, int tiles_n,
+                                                                 Order order, int tiles_m, int tiles_n,
                                                                  const RowInfo* __restrict__ info,
                                                                  const uint64_t* __restrict__ counts,
                                                                  uint16_t* __restrict__ ds, int64_t ld,
@@ -454,6 +519,7 @@ __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, 
   __shared__ __attribute__((aligned(16))) char lds[S::kLdsBytes];
   const gs_tile::TileAt tile = gs_tile::tile_at(tiles_m, tiles_n);
   const int m0 = tile.m * S::BM, n0 = tile.n * S::BN;
+  if (n0 >= order.used(features.extent)) return;
   Accumulators<S> acc;
   gs_tile::product<S, T, true, true>(acc, table, features, m0, n0, 0, dim, products, nullptr, lds);
   const float scale2 = scale_of(logit_scale2, units);
@@ -534,20 +600,24 @@ __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, 
 // K rows, K the rows of the piece); else dh (ds along K, K the vocabulary).
 // With `part` set the tile goes, in fp32, to plane blockIdx.y of part (added to
 // what is there if `add`); else out = the gradient of the tile's sums in the result's type (alpha, unit: see factor_of).
-// rows_count (dh): rows that do not count are zero.
+// counts (dh): rows that do not count are zero; order: of the features, K (dw) or n (dh).
 template <class S, typename T, typename Out, bool kTableGrad>
-__global__ __launch_bounds__(S::kThreads) void grad_kernel(Operand x, Operand ds, int32_t K, int32_t k_part,
+__global__ __launch_bounds__(S::kThreads) void grad_kernel(Operand x, Operand ds, int32_t K,
                                                            int products, const uint64_t* __restrict__ counts,
-                                                           int tiles_m, int tiles_n, float* __restrict__ part, int64_t part_plane,
+                                                           Order order, int tiles_m, int tiles_n,
+                                                           float* __restrict__ part, int64_t part_plane,
                                                            bool add, const double* __restrict__ alpha,
                                                            const float* __restrict__ unit, Out* __restrict__ out) {
   __shared__ __attribute__((aligned(16))) char lds[S::kLdsBytes];
   const gs_tile::TileAt tile = gs_tile::tile_at(tiles_m, tiles_n);
   const int m0 = tile.m * S::BM, n0 = tile.n * S::BN;
   const int D = x.extent;
-  // a part past the end (k_part is rounded up) has nothing to add
-  const int32_t k_begin = (int32_t)min((int64_t)K, (int64_t)blockIdx.y * k_part);
-  const int32_t k_end = (int32_t)min((int64_t)K, (int64_t)k_begin + k_part);
+  // The parts share what there is of K in whole steps; one past the end has nothing
+  // to add, and neither has a tile of features that do not count.
+  const int32_t k_used = kTableGrad ? order.used(K) : n0 >= order.used(ds.extent) ? 0 : K;
+  const int64_t k_part = (((int64_t)k_used + gridDim.y - 1) / gridDim.y + kBK - 1) / kBK * kBK;
+  const int32_t k_begin = (int32_t)min((int64_t)k_used, blockIdx.y * k_part);
+  const int32_t k_end = (int32_t)min((int64_t)k_used, k_begin + k_part);
   Accumulators<S> acc;
   gs_tile::product<S, T, false, !kTableGrad>(acc, x, ds, m0, n0, k_begin, k_end, products,
                                              kTableGrad ? counts : nullptr, lds);
@@ -564,13 +634,13 @@ __global__ __launch_bounds__(S::kThreads) void grad_kernel(Operand x, Operand ds
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int m = m0 + wm + 32 * a + 8 * q + 4 * (lane >> 5);
-        const int64_t at = (int64_t)n * D + m;
         if (part) {
-          float* p = part + (int64_t)blockIdx.y * part_plane + at;
+          float* p = part + (int64_t)blockIdx.y * part_plane + (int64_t)n * D + m;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             if (m + j < D) p[j] = acc.c[a][b][4 * q + j] + (add ? p[j] : 0.0f);
         } else {
+          const int64_t at = (kTableGrad ? (int64_t)n : order.row(n)) * D + m;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             if (m + j < D) out[at + j] = (Out)(use ? gradient_of<T>(acc.c[a][b][4 * q + j], factor) : 0.0f);
@@ -579,13 +649,13 @@ __global__ __launch_bounds__(S::kThreads) void grad_kernel(Operand x, Operand ds
   }
 }
 
-// out = the gradient of the planes' sum; counts (dh): rows that do not
-// count are zero.  kGroups threads share an element's planes, their sums joined in
+// out = the gradient of the planes' sum; dh: counts, rows that do not count are
+// zero, and order, where they go.  dw: counts null, order as it is.  kGroups threads share an element's planes, their sums joined in
 // order.
 template <int kGroups, typename T, typename Out>
 __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ part, int planes, int64_t plane,
                                                      int64_t n, int D, const uint64_t* __restrict__ counts,
-                                                     const double* __restrict__ alpha, const float* __restrict__ unit,
+                                                     Order order, const double* __restrict__ alpha, const float* __restrict__ unit,
                                                      Out* __restrict__ out) {
   constexpr int kElements = 256 / kGroups;
   __shared__ float lds[256];
@@ -603,7 +673,11 @@ __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ p
       if (group > 0) continue;
       for (int g = 1; g < kGroups; ++g) s += lds[g * kElements + element];
     }
-    if (i < n) out[i] = (Out)(!counts || row_counts(counts, i / D) ? gradient_of<T>(s, factor) : 0.0f);
+    if (i < n) {
+      const int64_t row = counts ? i / D : 0;
+      const int64_t at = counts ? order.row((int)row) * D + (i - row * D) : i;
+      out[at] = (Out)(!counts || row_counts(counts, row) ? gradient_of<T>(s, factor) : 0.0f);
+    }
   }
 }
 
@@ -637,6 +711,14 @@ struct Problem {
   int64_t dp() const { return round_up(dim, 8); }
   bool packs(int64_t ld) const { return dtype == GS_FP32 || dim % 8 || ld % 8 || ld > gs_tile::kMaxLd; }
   size_t element() const { return dtype == GS_FP32 ? 4 : 2; }
+  // Are the features' rows put in an order (struct Order)?  It takes two small
+  // kernels and, for rows that the loads can take in place, a copy of them, whether
+  // rows are ignored or not.
+  bool orders() const {
+    const int64_t logits = rows * vocab;
+    return packs(ld_features) ? logits >= 1ll << 26 : vocab >= 8192 && logits >= 1ll << 28;
+  }
+  bool packs_features() const { return packs(ld_features) || orders(); }
 };
 
 constexpr int64_t kMaxRows = (1ll << 31) - 1024;
@@ -665,17 +747,22 @@ static int check_pointers(const Problem& p) {
 struct Layouts {
   uint16_t *features_space, *table_space;
   float *units, *largest;
+  int *order_space, *used, *order_counts;
   int64_t rows;  // that features_space holds
   int features_n, table_n;
 
   Layouts() = default;
   Layouts(const Problem& p, int64_t rows_held, Carve& c) : rows(rows_held), features_n(0), table_n(0) {
     const bool fp32 = p.dtype == GS_FP32;
-    features_space = c.take<uint16_t>(p.packs(p.ld_features) ? rows * p.dp() * p.planes() : 0);
+    features_space = c.take<uint16_t>(p.packs_features() ? rows * p.dp() * p.planes() : 0);
     table_space = c.take<uint16_t>(p.packs(p.ld_table) ? p.vocab * p.dp() * p.planes() : 0);
     units = c.take<float>(fp32 ? 2 : 0);
     if (!fp32) units = nullptr;
+    order_space = c.take<int>(p.orders() ? p.rows : 0);
+    used = c.take<int>(p.orders() ? 1 : 0);
+    if (!p.orders()) order_space = used = nullptr;
   }
+  Order order() const { return {order_space, used, 0}; }
   const float* features_unit() const { return units; }
   const float* table_unit() const { return units ? units + 1 : nullptr; }
 
@@ -683,6 +770,12 @@ struct Layouts {
   void prepare(const Problem& p, Targets targets, hipStream_t s) {
     const Matrix f = {p.features, p.ld_features, p.rows, features_space, rows * p.dp()};
     const Matrix t = {p.table, p.ld_table, p.vocab, table_space, p.vocab * p.dp()};
+    if (order_space) {
+      const int64_t share = round_up(ceil_div(p.rows, kOrderBlocks), 256);
+      const int blocks = (int)ceil_div(p.rows, share);
+      used_kernel<<<blocks, 256, 0, s>>>(targets, p.rows, share, order_counts);
+      order_kernel<<<blocks, 256, 0, s>>>(targets, p.rows, share, order_counts, order_space, used);
+    }
     if (units) {
       auto fits = [](const Matrix& m) { return m.ld % 4 == 0 && (uintptr_t)m.src % 16 == 0; };
       const int V = p.dim % 4 == 0 && fits(f) && fits(t) ? 4 : 1;
@@ -694,21 +787,20 @@ struct Layouts {
       auto* kernel = V == 4 ? magnitude_kernel<4> : magnitude_kernel<1>;
       kernel<<<features_n + table_n, 256, 0, s>>>(f, features_n, t, p.dim, lanes, targets, largest);
     }
-    lay_out(p, rows == p.rows && p.packs(p.ld_features) ? f : Matrix{}, p.packs(p.ld_table) ? t : Matrix{}, s);
+    lay_out(p, rows == p.rows && p.packs_features() ? f : Matrix{}, order(), p.packs(p.ld_table) ? t : Matrix{}, s);
   }
-  void lay_out(const Problem& p, const Matrix& f, const Matrix& t, hipStream_t s) const {
+  void lay_out(const Problem& p, const Matrix& f, const Order& order, const Matrix& t, hipStream_t s) const {
     auto blocks = [&](const Matrix& m) { return (int)min(ceil_div(m.rows * (p.dp() / 8), 256), (int64_t)4096); };
     const int fn = blocks(f), tn = blocks(t);
     if (fn + tn == 0) return;
     auto* kernel = p.dtype == GS_FP32 ? layout_kernel<float> : layout_kernel<_Float16>;
-    kernel<<<fn + tn, 256, 0, s>>>(f, fn, t, p.dim, (int)p.dp(), largest, features_n, table_n, units);
+    kernel<<<fn + tn, 256, 0, s>>>(f, order, fn, t, p.dim, (int)p.dp(), largest, features_n, table_n, units);
   }
   Operand features(const Problem& p, int64_t first, int64_t n, hipStream_t s) const {
-    const char* at = (const char*)p.features + first * p.ld_features * (int64_t)p.element();
-    if (!p.packs(p.ld_features)) return {(const uint16_t*)at, p.ld_features, 0, (int32_t)n};
+    if (!p.packs_features()) return {(const uint16_t*)p.features + first * p.ld_features, p.ld_features, 0, (int32_t)n};
     const int64_t plane = rows * p.dp();
     if (rows == p.rows) return {features_space + first * p.dp(), p.dp(), plane, (int32_t)n};
-    lay_out(p, {at, p.ld_features, n, features_space, plane}, Matrix{}, s);
+    lay_out(p, {p.features, p.ld_features, n, features_space, plane}, order().from(first), Matrix{}, s);
     return {features_space, p.dp(), plane, (int32_t)n};
   }
   Operand table(const Problem& p) const {
@@ -758,10 +850,6 @@ static int resident_parts(int64_t held, int64_t stream, int64_t slots, double su
     }
   }
   return (int)best;
-}
-
-static int32_t part_rows(int64_t stream, int64_t parts) {
-  return (int32_t)round_up(ceil_div(stream, parts), gs_resident::kTileRows);
 }
 
 template <typename T, int kKind>
@@ -830,6 +918,7 @@ struct ForwardPlan {
     Carve c{(char*)ws};
     if (!kept) layouts = Layouts(p, rows_piece, c);
     layouts.largest = c.take<float>(p.dtype == GS_FP32 ? 2 * kLargestBlocks : 0);
+    layouts.order_counts = c.take<int>(p.orders() ? kOrderBlocks : 0);
     stats = c.take<float2>(tiles_m * rows_piece);
     label = c.take<float>(rows_piece);
     partial = c.take<Sum>(blocks);
@@ -839,10 +928,10 @@ struct ForwardPlan {
 
 template <class S, typename T>
 static void launch_logits_fwd(const Problem& p, const ForwardPlan& f, const Operand& table, const Operand& features,
-                              float scale2, Targets targets, hipStream_t s) {
+                              float scale2, Targets targets, const Order& order, hipStream_t s) {
   const int64_t tiles_n = ceil_div(features.extent, S::BN);
   logits_fwd_kernel<S, T><<<(unsigned)(f.tiles_m * tiles_n), S::kThreads, 0, s>>>(
-      table, features, (int)p.dp(), p.products(), scale2, f.layouts.units, targets, (int)f.tiles_m, (int)tiles_n,
+      table, features, (int)p.dp(), p.products(), scale2, f.layouts.units, targets, order, (int)f.tiles_m, (int)tiles_n,
       f.stats, f.label);
 }
 
@@ -856,32 +945,32 @@ static int forward(const Problem& p, Targets targets, float logit_scale, int red
   for (int64_t r = 0; r < p.rows; r += f.rows_piece) {
     const int64_t rows = min(f.rows_piece, p.rows - r);
     const Operand features = f.layouts.features(p, r, rows, s);
-    const Targets t = targets.from(r);
+    const Order order = f.layouts.order().from(r);
     switch (f.shape) {
-      case ForwardPlan::kThin32: launch_logits_fwd<Thin32, T>(p, f, table, features, scale2, t, s); break;
-      case ForwardPlan::kThin64: launch_logits_fwd<Thin64, T>(p, f, table, features, scale2, t, s); break;
+      case ForwardPlan::kThin32: launch_logits_fwd<Thin32, T>(p, f, table, features, scale2, targets, order, s); break;
+      case ForwardPlan::kThin64: launch_logits_fwd<Thin64, T>(p, f, table, features, scale2, targets, order, s); break;
       case ForwardPlan::kResident: {
         gs_resident::Args a = {};
         a.held = features;
         a.stream = table;
-        a.part = part_rows(p.vocab, f.tiles_m);
         a.dim = (int32_t)p.dp();
         a.logit_scale2 = scale2;
         a.units = f.layouts.units;
-        a.targets = t;
+        a.targets = targets;
+        a.order = order;
         a.stats = f.stats;
         a.label_dot = f.label;
         launch_resident<T, gs_resident::kForward>(p, a, (int)f.tiles_m, s);
         break;
       }
-      case ForwardPlan::kMid: launch_logits_fwd<Mid, T>(p, f, table, features, scale2, t, s); break;
-      case ForwardPlan::kBig: launch_logits_fwd<Big, T>(p, f, table, features, scale2, t, s); break;
+      case ForwardPlan::kMid: launch_logits_fwd<Mid, T>(p, f, table, features, scale2, targets, order, s); break;
+      case ForwardPlan::kBig: launch_logits_fwd<Big, T>(p, f, table, features, scale2, targets, order, s); break;
     }
     const int64_t blocks = ceil_div(rows, kJoinThreads / f.lanes);
     auto* join = f.lanes == 64 ? join_kernel<64> : join_kernel<1>;
     join<<<(unsigned)blocks, kJoinThreads, 0, s>>>(f.stats, f.label, (int)rows, (int)f.tiles_m, p.vocab, scale2,
-                                                   f.layouts.units, t, reduction, norm ? norm + r : nullptr,
-                                                   reduction == GS_REDUCE_NONE ? loss + r : nullptr,
+                                                   f.layouts.units, targets, order, reduction, norm ? norm + r : nullptr,
+                                                   reduction == GS_REDUCE_NONE ? loss : nullptr,
                                                    f.partial + block, f.blocks == 1, loss, count);
     block += blocks;
   }
@@ -987,10 +1076,10 @@ static unsigned finish_blocks(int64_t n) { return (unsigned)min(ceil_div(n, 256)
 
 template <typename T, typename Out>
 static void finish(const float* part, int planes, int64_t plane, int64_t n, int D, const uint64_t* counts,
-                   const double* alpha, const float* unit, Out* out, hipStream_t s) {
+                   const Order& order, const double* alpha, const float* unit, Out* out, hipStream_t s) {
   // many planes of few elements (a small table's) do not fill the chip by their elements alone
-  if (planes >= 16) finish_kernel<8, T><<<finish_blocks(n * 8), 256, 0, s>>>(part, planes, plane, n, D, counts, alpha, unit, out);
-  else finish_kernel<1, T><<<finish_blocks(n), 256, 0, s>>>(part, planes, plane, n, D, counts, alpha, unit, out);
+  if (planes >= 16) finish_kernel<8, T><<<finish_blocks(n * 8), 256, 0, s>>>(part, planes, plane, n, D, counts, order, alpha, unit, out);
+  else finish_kernel<1, T><<<finish_blocks(n), 256, 0, s>>>(part, planes, plane, n, D, counts, order, alpha, unit, out);
 }
 
 template <typename T, typename Out, int kPlanes>
@@ -1006,7 +1095,7 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
   }
   const Layouts& layouts = state.layouts;
   const float *unit_h = layouts.features_unit(), *unit_w = layouts.table_unit();
-  rows_kernel<<<(unsigned)ceil_div(p.rows, 256), 256, 0, s>>>(grad_loss, p.rows, p.vocab, targets, reduction, count, state.norm,
+  rows_kernel<<<(unsigned)ceil_div(p.rows, 256), 256, 0, s>>>(grad_loss, p.rows, p.vocab, targets, layouts.order(), reduction, count, state.norm,
                                                               logit_scale, scale2, layouts.units, Held<T>::kScale,
                                                               b.largest, largest_n, b.info, b.counts, b.alpha);
   const Operand table = layouts.table(p);
@@ -1016,33 +1105,34 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
     a.dim = (int32_t)p.dp();
     a.logit_scale2 = scale2;
     a.units = layouts.units;
+    a.order = layouts.order();
     a.info = b.info;
     a.counts = b.counts;
     a.alpha = b.alpha;
     a.D = D;
     auto run = [&](auto kind, const Operand& held, const Operand& stream, int parts, float* sums, const float* unit,
-                   Out* out) {
+                   Out* out, const uint64_t* counts) {
       a.held = held;
       a.stream = stream;
-      a.part = part_rows(stream.extent, parts);
       a.part_sums = parts > 1 ? sums : nullptr;
       a.part_plane = (int64_t)held.extent * D;
       a.unit = unit;
       a.out = out;
       launch_resident<T, decltype(kind)::value>(p, a, parts, s);
       if (parts > 1)
-        finish<T>(sums, parts, a.part_plane, a.part_plane, D, nullptr, b.alpha, unit, out, s);
+        finish<T>(sums, parts, a.part_plane, a.part_plane, D, counts, layouts.order(), b.alpha, unit, out, s);
     };
     if (grad_features)
-      run(std::integral_constant<int, gs_resident::kFeatures>{}, features, table, b.parts_h, b.part_h, unit_w, grad_features);
+      run(std::integral_constant<int, gs_resident::kFeatures>{}, features, table, b.parts_h, b.part_h, unit_w, grad_features, b.counts);
     if (grad_table)
-      run(std::integral_constant<int, gs_resident::kTable>{}, table, features, b.parts_t, b.part_t, unit_h, grad_table);
+      run(std::integral_constant<int, gs_resident::kTable>{}, table, features, b.parts_t, b.part_t, unit_h, grad_table, nullptr);
     return gs_status_from_hip(hipGetLastError());
   }
   for (int64_t r = 0; r < p.rows; r += b.rows_piece) {
     const int32_t rows = (int32_t)min(b.rows_piece, p.rows - r);
     const Operand features = layouts.features(p, r, rows, s);
     const uint64_t* counts = b.counts + r / 64;
+    const Order order = layouts.order().from(r);
     const int64_t ds_plane = rows * b.ld;
     for (int64_t c = 0; c < p.vocab; c += b.cols_piece) {
       const int32_t cols = (int32_t)min(b.cols_piece, p.vocab - c);
@@ -1054,7 +1144,7 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
         typedef decltype(shape) S;
         const int tiles_m = (int)ceil_div(cols, S::BM), tiles_n = (int)ceil_div(rows, S::BN);
         logits_bwd_kernel<S, T, kPlanes><<<(unsigned)((int64_t)tiles_m * tiles_n), S::kThreads, 0, s>>>(
-            piece, features, (int)p.dp(), p.products(), scale2, layouts.units, (int32_t)c, tiles_m, tiles_n,
+            piece, features, (int)p.dp(), p.products(), scale2, layouts.units, (int32_t)c, order, tiles_m, tiles_n,
             b.info + r, counts, b.ds, b.ld, ds_plane);
       });
       if (grad_features) {
@@ -1065,10 +1155,9 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
           Operand x = piece;  // D columns of the piece's rows
           x.extent = D;
           const int tiles_n = (int)ceil_div(rows, S::BN);
-          const int32_t k_part = (int32_t)round_up(ceil_div(cols, b.parts_h), kBK);
           grad_kernel<S, T, Out, false><<<dim3((unsigned)((int64_t)tiles_m * tiles_n), b.parts_h), S::kThreads, 0, s>>>(
-              x, ds, cols, k_part, p.ds_products(), counts, tiles_m, tiles_n, b.direct_h ? nullptr : b.part_h,
-              (int64_t)rows * D, c > 0, b.alpha, unit_w, grad_features + r * D);
+              x, ds, cols, p.ds_products(), counts, order, tiles_m, tiles_n, b.direct_h ? nullptr : b.part_h,
+              (int64_t)rows * D, c > 0, b.alpha, unit_w, grad_features);
         });
       }
       if (grad_table) {
@@ -1079,22 +1168,21 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
           Operand x = features;
           x.extent = D;
           const int tiles_n = (int)ceil_div(cols, S::BN);
-          const int32_t k_part = (int32_t)round_up(ceil_div(rows, b.parts_t), kBK);
           float* part = b.direct_t ? nullptr : b.part_t + (b.row_pieces > 1 ? c * D : 0);
           const int64_t part_plane = (b.row_pieces > 1 ? (int64_t)p.vocab : cols) * D;
           grad_kernel<S, T, Out, true><<<dim3((unsigned)((int64_t)tiles_m * tiles_n), b.parts_t), S::kThreads, 0, s>>>(
-              x, ds, rows, k_part, p.ds_products(), counts, tiles_m, tiles_n, part, part_plane, r > 0, b.alpha, unit_h,
+              x, ds, rows, p.ds_products(), counts, order, tiles_m, tiles_n, part, part_plane, r > 0, b.alpha, unit_h,
               grad_table + c * D);
           if (part && b.row_pieces == 1)
-            finish<T>(part, b.parts_t, part_plane, (int64_t)cols * D, D, nullptr, b.alpha, unit_h, grad_table + c * D, s);
+            finish<T>(part, b.parts_t, part_plane, (int64_t)cols * D, D, nullptr, Order{}, b.alpha, unit_h, grad_table + c * D, s);
         });
       }
     }
     if (grad_features && !b.direct_h)
-      finish<T>(b.part_h, b.parts_h, (int64_t)rows * D, (int64_t)rows * D, D, counts, b.alpha, unit_w, grad_features + r * D, s);
+      finish<T>(b.part_h, b.parts_h, (int64_t)rows * D, (int64_t)rows * D, D, counts, order, b.alpha, unit_w, grad_features, s);
   }
   if (grad_table && b.row_pieces > 1)
-    finish<T>(b.part_t, b.parts_t, (int64_t)p.vocab * D, (int64_t)p.vocab * D, D, nullptr, b.alpha, unit_h, grad_table, s);
+    finish<T>(b.part_t, b.parts_t, (int64_t)p.vocab * D, (int64_t)p.vocab * D, D, nullptr, Order{}, b.alpha, unit_h, grad_table, s);
   return gs_status_from_hip(hipGetLastError());
 }
 
@@ -1150,9 +1238,10 @@ extern "C" int gs_xent_fwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dty
   float4* norm = nullptr;
   if (state) {
     const gs_xent::State kept(p, state);
-    float* largest = f.layouts.largest;
+    const gs_xent::Layouts scratch = f.layouts;
     f.layouts = kept.layouts;
-    f.layouts.largest = largest;
+    f.layouts.largest = scratch.largest;
+    f.layouts.order_counts = scratch.order_counts;
     norm = kept.norm;
   }
   const gs_xent::Targets t = {targets, target_bits, ignore_index};

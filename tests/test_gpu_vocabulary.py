@@ -567,3 +567,43 @@ def test_lookup_of_more_vectors_than_a_launch_has_threads(device):
     out = vocabulary.embed_tokens(tokens, table)
     for at in (0, 2 ** 27, 2 ** 28, 2 ** 29, 2 ** 30 - 100, n - 100):
         assert torch.equal(out[at:at + 100], table[tokens[at:at + 100]])
+
+
+@pytest.mark.parametrize("dtype,rows,vocab,dim", [
+    (FP32, 70_001, 1000, 40), (FP32, 70_001, 1000, 136), (FP16, 130_003, 520, 100), (BF16, 130_003, 520, 9),
+    (FP32, 1_100_003, 64, 8), (FP32, 1_100_003, 64, 72), (BF16, 66_001, 8192, 72), (FP16, 66_001, 8192, 136)])
+@pytest.mark.parametrize("ignored", [0.0, 0.4, "half", "all but one"])
+def test_entropy_of_many_rows_of_which_some_count(device, dtype, rows, vocab, dim, ignored):
+    """Sizes at which the rows that count are put first: with and without a gradient, in one piece and in several."""
+    print(f"entropy {dtype} rows={rows} vocab={vocab} dim={dim} ignored={ignored}", flush=True)
+    gen = torch.Generator(device=device).manual_seed(dim)
+    features = torch.randn(rows, dim, generator=gen, device=device).to(dtype)
+    table = (torch.randn(vocab, dim, generator=gen, device=device) / math.sqrt(dim)).to(dtype).requires_grad_(True)
+    targets = torch.randint(0, vocab, (rows,), generator=gen, device=device)
+    if ignored == "half":
+        out = torch.arange(rows, device=device) < rows // 2
+    elif ignored == "all but one":
+        out = torch.arange(rows, device=device) != rows - 3
+    else:
+        out = torch.rand(rows, generator=gen, device=device) < ignored
+    targets[out] = -100
+    features[out] = math.nan
+    features.requires_grad_(True)
+    up = torch.rand(rows, generator=gen, device=device) + 0.5
+    loss = vocabulary.linear_cross_entropy(features, table, targets, reduction="none")
+    grads = torch.autograd.grad(loss, (features, table), up)
+    with torch.no_grad():
+        assert torch.equal(loss, vocabulary.linear_cross_entropy(features, table, targets, reduction="none"))
+        mean = vocabulary.linear_cross_entropy(features, table, targets)
+    assert not loss[out].any() and not grads[0][out].any()
+    # the rows that count, a part of them at a time; the table's gradient from the bounds of all parts
+    kept = (~out).nonzero().squeeze(1)
+    total, value, bound = 0.0, 0.0, 0.0
+    for ids in kept.split(max(1, 2 ** 26 // vocab)):
+        want = ref.entropy(features.detach()[ids], table.detach(), targets[ids], up[ids], reduction="none")
+        ref.check(loss[ids], want["loss"], "loss")
+        ref.check(grads[0][ids], want["features"], "features")
+        total += float(want["loss"][0].sum())
+        value, bound = value + want["table"][0], bound + want["table"][1]
+    ref.check(grads[1], (value, bound), "table")
+    assert abs(float(mean) - total / len(kept)) <= 1e-5 * max(1.0, abs(total / len(kept)))
