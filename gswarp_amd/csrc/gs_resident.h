@@ -124,9 +124,14 @@ __device__ __forceinline__ void planes_of(const f32x16& s, int from, typename Pa
 #pragma unroll
   for (int p = 0; p < kPlanes; ++p)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      out[p][e] = (T)v[e];
-      if (kPlanes > 1) v[e] = (v[e] - (float)out[p][e]) * kPlaneStep;
+    for (int e = 0; e < 8; e += 2) {
+      T pair[2];
+      gs_tile::round_pair(v[e], v[e + 1], p + 1 < kPlanes, pair);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        out[p][e + i] = pair[i];
+        if (p + 1 < kPlanes) v[e + i] = gs_tile::behind(v[e + i], pair[i]);
+      }
     }
 }
 
@@ -342,10 +347,14 @@ __global__ __launch_bounds__(kThreads, kKind == kForward && KB * PL <= 2 ? 4 : 2
           for (int q = 0; q < 4; ++q) {
             typename Pack<T>::v4 held4;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float v = s[b][4 * q + j];
-              held4[j] = (T)v;
-              if (kDsPlanes > 1) s[b][4 * q + j] = (v - (float)held4[j]) * kPlaneStep;
+            for (int j = 0; j < 4; j += 2) {
+              T pair[2];
+              gs_tile::round_pair(s[b][4 * q + j], s[b][4 * q + j + 1], p + 1 < kDsPlanes, pair);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                held4[j + i] = pair[i];
+                if (p + 1 < kDsPlanes) s[b][4 * q + j + i] = gs_tile::behind(s[b][4 * q + j + i], pair[i]);
+              }
             }
             *reinterpret_cast<typename Pack<T>::v4*>(turn + n * 64 + (((2 * q + half) ^ swap) << 3)) = held4;
           }
@@ -354,7 +363,7 @@ __global__ __launch_bounds__(kThreads, kKind == kForward && KB * PL <= 2 ? 4 : 2
           if (at >= 0 && at < 32 && ((at >> 2) & 1) == half) {
             const T v = (T)r[b].label;
             *reinterpret_cast<T*>(turn + n * 64 + (((at >> 2) ^ swap) << 3) + (at & 3) * 2) = v;
-            if (kDsPlanes > 1) r[b].label = (r[b].label - (float)v) * kPlaneStep;
+            if (p + 1 < kDsPlanes) r[b].label = gs_tile::behind(r[b].label, v);
           }
         }
 #pragma unroll

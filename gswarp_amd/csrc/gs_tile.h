@@ -56,6 +56,12 @@ struct Operand {
 constexpr int kSplitPlanes = 2, kWidePlanes = 3;      // of an fp32 operand, of one of wide range
 constexpr int kSplitProducts = 3, kWideProducts = 4;  // of two fp32 operands, with a wide Y
 constexpr float kPlaneStep = 2048.0f;                 // what each plane is held times more than the one before
+// What is left of v behind its plane h, for the next one: exact, and two
+// instructions (the second takes h in 16 bits).
+__device__ __forceinline__ float behind(float v, _Float16 h) {
+  return __builtin_fmaf((float)h, -kPlaneStep, v * kPlaneStep);
+}
+__device__ __forceinline__ float behind(float, __bf16) { return 0.0f; }  // (one plane only)
 // The planes of X and Y that product s of `products` takes: (hi, tiny) if there are
 // four, (lo, hi), (hi, lo), (hi, hi).  Before (lo, hi), if not the first, and
 // before (hi, hi) the sums so far are divided by a step.
@@ -85,6 +91,19 @@ struct Pack<_Float16> {
   typedef f16x8 v8;
   typedef f16x4 v4;
 };
+
+// Two values in 16 bits.  As planes go on from what was rounded, the compiler would
+// round for that once more, one by one, if it saw where the pair comes from.
+template <typename T>
+__device__ __forceinline__ void round_pair(float a, float b, bool goes_on, T* out) {
+  typedef T pair __attribute__((ext_vector_type(2)));
+  typedef float floats __attribute__((ext_vector_type(2)));
+  uint32_t bits = __builtin_bit_cast(uint32_t, __builtin_convertvector(floats{a, b}, pair));
+  if (goes_on) asm("" : "+v"(bits));
+  const pair p = __builtin_bit_cast(pair, bits);
+  out[0] = p[0];
+  out[1] = p[1];
+}
 
 // One operand's part of a K step, BT rows (m or n) x 64 columns of K, loaded
 // straight into LDS: each load instruction of a wave fills 1024 bytes, lane l

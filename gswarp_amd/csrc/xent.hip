@@ -209,7 +209,7 @@ __global__ __launch_bounds__(256) void layout_kernel(Matrix first, Order order, 
         const float x = (col + e < dim ? s[e] : 0.0f) * scale;
         hi[e] = (_Float16)x;
         // nothing is left of infinities and NaN
-        lo[e] = fabsf(x) < INFINITY ? (_Float16)((x - (float)hi[e]) * gs_tile::kPlaneStep) : (_Float16)0.0f;
+        lo[e] = fabsf(x) < INFINITY ? (_Float16)gs_tile::behind(x, hi[e]) : (_Float16)0.0f;
       }
       *reinterpret_cast<gs_tile::f16x8*>(d) = hi;
       *reinterpret_cast<gs_tile::f16x8*>(d + m.plane) = lo;
@@ -570,10 +570,14 @@ __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, 
         for (int q = 0; q < 4; ++q) {
           typename gs_tile::Pack<T>::v4 held;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float v = acc.c[a][b][4 * q + j];
-            held[j] = (T)v;
-            if (kPlanes > 1) acc.c[a][b][4 * q + j] = (v - (float)held[j]) * gs_tile::kPlaneStep;
+          for (int j = 0; j < 4; j += 2) {
+            T pair[2];
+            gs_tile::round_pair(acc.c[a][b][4 * q + j], acc.c[a][b][4 * q + j + 1], p + 1 < kPlanes, pair);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              held[j + i] = pair[i];
+              if (p + 1 < kPlanes) acc.c[a][b][4 * q + j + i] = gs_tile::behind(acc.c[a][b][4 * q + j + i], pair[i]);
+            }
           }
           // a row that does not count holds zeros whatever came out above
           gs_tile::u32x2 bits = __builtin_bit_cast(gs_tile::u32x2, held);
