@@ -370,16 +370,21 @@ __device__ __forceinline__ void product(Accumulators<S>& acc, const Operand& x, 
 
 // The tile of a block: blocks go to the 8 XCDs (each with an L2 of its own) in
 // turn, so each XCD is given a run of consecutive tiles, in bands of 8 tiles
-// of m, m first inside a band: tiles that run side by side share operands.
+// of m, m first inside a band: tiles that run side by side share operands.  Those
+// from used_n on have nothing to multiply and come last.
 struct TileAt {
   int m, n;
 };
-__device__ __forceinline__ TileAt tile_at(int tiles_m, int tiles_n) {
-  const int total = tiles_m * tiles_n;
+__device__ __forceinline__ TileAt tile_at(int tiles_m, int used_n) {
+  const int total = tiles_m * used_n;
+  if ((int)blockIdx.x >= total) {
+    const int rest = blockIdx.x - total;
+    return {rest % tiles_m, used_n + rest / tiles_m};
+  }
   const int id = blockIdx.x, q = total / 8, r = total % 8, xcd = id % 8;
   const int t = xcd * q + min(xcd, r) + id / 8;
-  const int band = t / (8 * tiles_n);
-  const int height = min(8, tiles_m - 8 * band), in = t - band * 8 * tiles_n;
+  const int band = t / (8 * used_n);
+  const int height = min(8, tiles_m - 8 * band), in = t - band * 8 * used_n;
   return {8 * band + in % height, in / height};
 }
 

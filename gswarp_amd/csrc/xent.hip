@@ -254,13 +254,14 @@ template <class S, typename T>
 __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, Operand features, int dim,
                                                                  int products, float logit_scale2,
                                                                  const float* __restrict__ units, Targets targets,
-                                                                 Order order, int tiles_m, int tiles_n,
+                                                                 Order order, int tiles_m,
                                                                  float2* __restrict__ stats,
                                                                  float* __restrict__ label_dot) {
   __shared__ __attribute__((aligned(16))) char lds[S::kLdsBytes];
-  const gs_tile::TileAt tile = gs_tile::tile_at(tiles_m, tiles_n);
+  const int used_n = (order.used(features.extent) + S::BN - 1) / S::BN;
+  const gs_tile::TileAt tile = gs_tile::tile_at(tiles_m, used_n);
+  if (tile.n >= used_n) return;
   const int m0 = tile.m * S::BM, n0 = tile.n * S::BN;
-  if (n0 >= order.used(features.extent)) return;
   Accumulators<S> acc;
   gs_tile::product<S, T, true, true>(acc, table, features, m0, n0, 0, dim, products, nullptr, lds);
 
@@ -511,15 +512,16 @@ template <class S, typename T, int kPlanes>
 __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, Operand features, int dim,
                                                                  int products, float logit_scale2,
                                                                  const float* __restrict__ units, int32_t m_base,
-                                                                 Order order, int tiles_m, int tiles_n,
+                                                                 Order order, int tiles_m,
                                                                  const RowInfo* __restrict__ info,
                                                                  const uint64_t* __restrict__ counts,
                                                                  uint16_t* __restrict__ ds, int64_t ld,
                                                                  int64_t plane) {
   __shared__ __attribute__((aligned(16))) char lds[S::kLdsBytes];
-  const gs_tile::TileAt tile = gs_tile::tile_at(tiles_m, tiles_n);
+  const int used_n = (order.used(features.extent) + S::BN - 1) / S::BN;
+  const gs_tile::TileAt tile = gs_tile::tile_at(tiles_m, used_n);
+  if (tile.n >= used_n) return;
   const int m0 = tile.m * S::BM, n0 = tile.n * S::BN;
-  if (n0 >= order.used(features.extent)) return;
   Accumulators<S> acc;
   gs_tile::product<S, T, true, true>(acc, table, features, m0, n0, 0, dim, products, nullptr, lds);
   const float scale2 = scale_of(logit_scale2, units);
@@ -608,17 +610,18 @@ __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, 
 template <class S, typename T, typename Out, bool kTableGrad>
 __global__ __launch_bounds__(S::kThreads) void grad_kernel(Operand x, Operand ds, int32_t K,
                                                            int products, const uint64_t* __restrict__ counts,
-                                                           Order order, int tiles_m, int tiles_n,
+                                                           Order order, int tiles_m,
                                                            float* __restrict__ part, int64_t part_plane,
                                                            bool add, const double* __restrict__ alpha,
                                                            const float* __restrict__ unit, Out* __restrict__ out) {
   __shared__ __attribute__((aligned(16))) char lds[S::kLdsBytes];
-  const gs_tile::TileAt tile = gs_tile::tile_at(tiles_m, tiles_n);
+  const int used_n = (int)(((int64_t)(kTableGrad ? ds.extent : order.used(ds.extent)) + S::BN - 1) / S::BN);
+  const gs_tile::TileAt tile = gs_tile::tile_at(tiles_m, used_n);
   const int m0 = tile.m * S::BM, n0 = tile.n * S::BN;
   const int D = x.extent;
   // The parts share what there is of K in whole steps; one past the end has nothing
   // to add, and neither has a tile of features that do not count.
-  const int32_t k_used = kTableGrad ? order.used(K) : n0 >= order.used(ds.extent) ? 0 : K;
+  const int32_t k_used = kTableGrad ? order.used(K) : tile.n >= used_n ? 0 : K;
   const int64_t k_part = (((int64_t)k_used + gridDim.y - 1) / gridDim.y + kBK - 1) / kBK * kBK;
   const int32_t k_begin = (int32_t)min((int64_t)k_used, blockIdx.y * k_part);
   const int32_t k_end = (int32_t)min((int64_t)k_used, k_begin + k_part);
@@ -935,7 +938,7 @@ static void launch_logits_fwd(const Problem& p, const ForwardPlan& f, const Oper
                               float scale2, Targets targets, const Order& order, hipStream_t s) {
   const int64_t tiles_n = ceil_div(features.extent, S::BN);
   logits_fwd_kernel<S, T><<<(unsigned)(f.tiles_m * tiles_n), S::kThreads, 0, s>>>(
-      table, features, (int)p.dp(), p.products(), scale2, f.layouts.units, targets, order, (int)f.tiles_m, (int)tiles_n,
+      table, features, (int)p.dp(), p.products(), scale2, f.layouts.units, targets, order, (int)f.tiles_m,
       f.stats, f.label);
 }
 
@@ -1148,7 +1151,7 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
         typedef decltype(shape) S;
         const int tiles_m = (int)ceil_div(cols, S::BM), tiles_n = (int)ceil_div(rows, S::BN);
         logits_bwd_kernel<S, T, kPlanes><<<(unsigned)((int64_t)tiles_m * tiles_n), S::kThreads, 0, s>>>(
-            piece, features, (int)p.dp(), p.products(), scale2, layouts.units, (int32_t)c, order, tiles_m, tiles_n,
+            piece, features, (int)p.dp(), p.products(), scale2, layouts.units, (int32_t)c, order, tiles_m,
             b.info + r, counts, b.ds, b.ld, ds_plane);
       });
       if (grad_features) {
@@ -1160,7 +1163,7 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
           x.extent = D;
           const int tiles_n = (int)ceil_div(rows, S::BN);
           grad_kernel<S, T, Out, false><<<dim3((unsigned)((int64_t)tiles_m * tiles_n), b.parts_h), S::kThreads, 0, s>>>(
-              x, ds, cols, p.ds_products(), counts, order, tiles_m, tiles_n, b.direct_h ? nullptr : b.part_h,
+              x, ds, cols, p.ds_products(), counts, order, tiles_m, b.direct_h ? nullptr : b.part_h,
               (int64_t)rows * D, c > 0, b.alpha, unit_w, grad_features);
         });
       }
@@ -1175,7 +1178,7 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
           float* part = b.direct_t ? nullptr : b.part_t + (b.row_pieces > 1 ? c * D : 0);
           const int64_t part_plane = (b.row_pieces > 1 ? (int64_t)p.vocab : cols) * D;
           grad_kernel<S, T, Out, true><<<dim3((unsigned)((int64_t)tiles_m * tiles_n), b.parts_t), S::kThreads, 0, s>>>(
-              x, ds, rows, p.ds_products(), counts, order, tiles_m, tiles_n, part, part_plane, r > 0, b.alpha, unit_h,
+              x, ds, rows, p.ds_products(), counts, order, tiles_m, part, part_plane, r > 0, b.alpha, unit_h,
               grad_table + c * D);
           if (part && b.row_pieces == 1)
             finish<T>(part, b.parts_t, part_plane, (int64_t)cols * D, D, nullptr, Order{}, b.alpha, unit_h, grad_table + c * D, s);
