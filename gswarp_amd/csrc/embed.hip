@@ -65,10 +65,12 @@ __device__ __forceinline__ void store_vector(T* __restrict__ p, const Vec<T, V>&
 }
 
 // ------------------------------------------------------------------ forward
-// A thread moves a vector of V elements.  What bounds it is the write of out.
-// Blocks go to the 8 XCDs in turn, so each XCD is given a run of consecutive
-// blocks, and the stores bypass the caches: 960 MB of rows (5M x 48 fp32 from 8192)
-// are written at 7.2 TB/s, against 3.6 with cached stores in launch order.
+// A thread moves a vector of V elements.  What bounds it is the write of out, and
+// the table's read where it does not stay in the caches.  Blocks go to the 8 XCDs in
+// turn, so each XCD is given a run of consecutive blocks, and the stores bypass the
+// caches: 5M x 48 fp32 from 8192 rows takes 155 us (6.2 TB/s written; cached stores
+// in launch order reach 3.6), 65536 x 1024 bf16 from 32768 rows 40 us (6.7 TB/s of
+// reads and writes).
 template <typename T, int V, bool kWhole>
 __global__ __launch_bounds__(kThreads) void lookup_kernel(Tokens tokens, int64_t n, u32 vocab, int D, u32 row_vectors,
                                                           const T* __restrict__ table, int64_t ld, float scale,
@@ -130,7 +132,11 @@ __device__ __forceinline__ void zero_rows(uint64_t absent, int64_t first, int D,
   }
 }
 
-// One level of sums.  Entry e of n has key keys[e] (>= vocab: nothing) and its
+// One level of sums.  Reading grad_out row by row in the tokens' order bounds it:
+// 5M rows of 192 bytes take 300 us (3.2 TB/s, 4.3 of whole 128-byte lines), 65536
+// rows of 2 KB 54 us with the 32768 rows that they are summed to (3.7 TB/s).  Each
+// lane has two batches of rows on their way, at addresses that are in LDS before.
+// Entry e of n has key keys[e] (>= vocab: nothing) and its
 // row at src + (positions ? positions[e] : e) * ld.
 struct Level {
   const u32* keys;
@@ -346,7 +352,10 @@ __global__ __launch_bounds__(kRunThreads, 4) void runs_kernel(Level v, const S* 
 // Few positions: no sort.  Workgroup i < n looks for its position's token among
 // all of them; if it is the token's first, it lists the others and sums their
 // rows, a part of the list for each group of lanes, the parts joined in order.
-// The workgroups behind zero the rows of the table that no token names.
+// The workgroups behind zero the rows of the table that no token names.  One launch
+// in place of the sort's eight or so, at n reads of n tokens: 2048 positions take
+// 10 to 20 us against 32 to 46 sorted, 4096 take as long as sorted or longer (55
+// against 42 at 64 columns of 32000 rows).
 constexpr int kFew = 2048;
 template <typename T, int V, bool kWhole>
 __global__ __launch_bounds__(kThreads) void few_kernel(Tokens tokens, int n, u32 vocab, int64_t padding, int D,
@@ -486,8 +495,10 @@ static int lanes_of(int D, int V) {
   return lanes;
 }
 
-// Entries of a group.  On the first level 4 to 64, by how many make 512 chunks,
-// which fill the chip; above, all of them where that is 8 at most, else 8 and on,
+// Entries of a group.  On the first level 4 to 64, by how many make 512 chunks, two
+// a CU (1M x 16 bf16 into 256 rows, with the lookup: 153 us, and 190 at 1024 chunks;
+// 65536 x 1024 into 32768 rows: 126, 152 at 2048, 128 at 128); above, all of them
+// where that is 8 at most, else 8 and on,
 // so that at most 64 chunks hand on to the next level: few levels, and none that
 // leaves many rows to one workgroup (2048 rows of 256 bytes take one 43 us).
 static int group_length(int64_t n, int lanes, bool first) {
@@ -560,7 +571,8 @@ static int gradient(int64_t n, int32_t vocab, int32_t dim, Tokens tokens, const 
   if (n <= kFew) {
     const int lanes = lanes_of(dim, V);
     const dim3 grid((unsigned)(n + ceil_div(vocab, kThreads)), (unsigned)ceil_div(dim, lanes * V));
-    few_kernel<T, V, kWhole><<<grid, kThreads, 0, s>>>(tokens, (int)n, (u32)vocab, padding, dim, lanes, scale, grad, out);
+    few_kernel<T, V, kWhole><<<grid, kThreads, 0, s>>>(tokens, (int)n, (u32)vocab, padding, dim, lanes, scale, grad,
+                                                       out);
     return gs_status_from_hip(hipGetLastError());
   }
   keys_kernel<<<(unsigned)min(ceil_div(n, kThreads), (int64_t)8192), kThreads, 0, s>>>(tokens, n, (u32)vocab, padding,

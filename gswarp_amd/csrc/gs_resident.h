@@ -1,7 +1,7 @@
 // The cross entropy's products for short rows (up to 128 values of 16 bits or 64
-// of fp32, and twice that where only the loss is wanted): one operand's rows stay in registers, the other's stream through LDS in
-// tiles of 64 rows, and the logits of a tile never leave the registers of the
-// wave that formed them.
+// of fp32, and twice that for the forward): one operand's rows stay in registers,
+// the other's stream through LDS in tiles of 64 rows, and the logits of a tile never
+// leave the registers of the wave that formed them.
 //
 //   kForward  features held, table streamed: the running maximum and sum of a
 //             softmax over the tiles, one pair per row and part;
@@ -12,7 +12,13 @@
 //
 // Against the tiles of logits in memory this forms the logits once more (10 N V D
 // flops in all instead of 8) and moves no logits: at D = 64 a logit costs 256
-// flops and, there, 6 to 22 bytes.
+// flops and, there, 6 to 22 bytes.  Forward and gradients, this against tiles, in us:
+//   16384 rows x 32768: bf16 D = 64 461 / 931, D = 128 678 / 1099; fp32 D = 64 1209 / 3365
+//   1024 rows x 512:    bf16 D = 64 42 / 59, fp32 81 / 93
+// What bounds it: the vector instructions, with the matrix ones (37 to 48 % busy).
+// 640000 x 512 x 64 fp32, a fifth of the rows ignored: kForward 134 us, kFeatures
+// 336, kTable 285 (the products alone would take 73, 171 and 171 at the rate of a
+// large fp16 product).
 //
 // What the products bring per element is little, so the vector instructions
 // count: an element takes an fma, an exponential and a multiplication.  The label
@@ -220,8 +226,8 @@ __global__ __launch_bounds__(kThreads, kKind == kForward && KB * PL <= 2 ? 4 : 2
     if (kKind == kTable) {
       const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
           (void*)(a.info + first), 0, (uint32_t)min(kTileRows, end - first) * 16u, 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(to + kTile + wave * 1024),
-                                               16, lane * 16, 0, 0, 0);
+      typedef __attribute__((address_space(3))) void lds_void;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(to + kTile + wave * 1024), 16, lane * 16, 0, 0, 0);
     }
     ++loaded;
   };
@@ -374,7 +380,8 @@ __global__ __launch_bounds__(kThreads, kKind == kForward && KB * PL <= 2 ? 4 : 2
               (gs_tile::lds_s16x4*)(turn + n * 64 + ((unit ^ ((n >> 2) & 7)) << 3)));
           const gs_tile::s16x4 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
               (gs_tile::lds_s16x4*)(turn + (n + 4) * 64 + ((unit ^ (((n + 4) >> 2) & 7)) << 3)));
-          const v8 ds = __builtin_bit_cast(v8, (gs_tile::s16x8)__builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7));
+          const gs_tile::s16x8 both = __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
+          const v8 ds = __builtin_bit_cast(v8, both);
 #pragma unroll
           for (int d = 0; d < kDBlocks; ++d) {
             const char* block = tile + d / 2 * Stage::kBytes;

@@ -26,9 +26,12 @@ using gs_tile::kBK;
 using gs_tile::Operand;
 
 // The tile shapes (BM, BN, waves along each, stages).  Big has twice Mid's reuse
-// of what it loads and one workgroup a CU; Mid wastes less on small sides and
-// two of its workgroups overlap.  Thin: few rows, where the table streams through once and what counts is how
-// many bytes are under way (two workgroups a CU, four or five steps each).
+// of what it loads and one workgroup a CU (forward of 16384 x 8192 x 512 bf16: 158
+// us, Mid 182); Mid wastes less on small sides and two of its workgroups overlap
+// (512 x 4096: 16 us, Big 25).  256 x 128 and 128 x 256 tiles were slower than both
+// (65536 x 32768 x 512 with gradients: 13.6 to 14 ms, Mid 12.2, Big 11).  Thin: few
+// tiles, where what counts is how many bytes are under way (two workgroups a CU,
+// four or five steps each); see kThinTiles.
 typedef gs_tile::Shape<256, 256, 2, 4> Big;
 typedef gs_tile::Shape<128, 128, 2, 2> Mid;
 typedef gs_tile::Shape<64, 32, 2, 1, 6> Thin32;
@@ -37,9 +40,12 @@ typedef gs_tile::Shape<64, 64, 2, 1, 5> Thin64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.6931471805599453;
 constexpr int kJoinThreads = 256;
-constexpr int64_t kPieceBytes = 1ll << 30;     // ds of one piece, all planes
-constexpr int64_t kLeastSide = 4096;           // rows or vocabulary of a piece, at least (a multiple of the tiles')
-constexpr int64_t kStatBytes = 256ll << 20;    // the tiles' pairs of one piece (forward)
+// ds of one piece, all planes: 65536 x 32768 x 512 bf16 takes 13.3, 11.1, 10.3, 10.0
+// and 9.8 ms at 128, 256, 512, 1024 and 2048 MiB (fewer sums of dh and dw go through memory).
+constexpr int64_t kPieceBytes = 1ll << 30;
+constexpr int64_t kLeastSide = 4096;         // rows or vocabulary of a piece, at least (a multiple of the tiles')
+constexpr int64_t kStatBytes = 256ll << 20;  // the tiles' pairs of one piece (forward)
+
 // ------------------------------------------------------------------ packing
 // A matrix and where its layout for the tile loads goes: rows of dp = ceil(dim /
 // 8) * 8 16-bit values, zero past dim, from dst (null: it is read in place);
@@ -52,8 +58,9 @@ struct Matrix {
   int64_t plane;
 };
 
-// The order of the rows (struct Order), where it is worth a copy of them.  Each
-// workgroup takes `share` rows; counts[b]: how many of workgroup b's count.
+// The order of the rows (struct Order), where it is worth a copy of them: the rows
+// that count are counted by workgroups of `share` rows (counts[b]), then each puts
+// its rows behind those of the workgroups before it.  5 us each for 640000 rows.
 constexpr int kOrderBlocks = 1024;
 __device__ __forceinline__ bool row_is_used(const Targets& targets, int64_t row, int64_t end) {
   return row < end && targets.at(row) != targets.ignore;
@@ -64,7 +71,8 @@ __global__ __launch_bounds__(256) void used_kernel(Targets targets, int64_t rows
   __shared__ int lds[4];
   const int64_t begin = blockIdx.x * share, end = min(rows, begin + share);
   int n = 0;
-  for (int64_t r = begin; r < end; r += 256) n += __builtin_popcountll(__ballot(row_is_used(targets, r + threadIdx.x, end)));
+  for (int64_t r = begin; r < end; r += 256)
+    n += __builtin_popcountll(__ballot(row_is_used(targets, r + threadIdx.x, end)));
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = n;
   __syncthreads();
   if (threadIdx.x == 0) counts[blockIdx.x] = lds[0] + lds[1] + lds[2] + lds[3];
@@ -111,6 +119,8 @@ __global__ __launch_bounds__(256) void order_kernel(Targets targets, int64_t row
   }
 }
 
+// Bound by its read: 640000 x 64 fp32 (164 MB) in 48 us, and their layout, 164 MB
+// to 131 MB of the rows that count, in 75 us (3.5 and 3.7 TB/s).
 // fp32: the largest finite magnitudes of the features (of the rows that count
 // only, so that what ignored rows hold does not reach the unit of the others) and
 // of the table, one value a block, the features' blocks first.  A group of
@@ -180,7 +190,8 @@ __device__ __forceinline__ float unit_of(const float* __restrict__ largest, int 
 // fp32: their units, from largest (the first's magnitudes, then the second's), go to
 // units[0] and units[1].
 template <typename T>
-__global__ __launch_bounds__(256) void layout_kernel(Matrix first, Order order, int first_blocks, Matrix second, int dim, int dp,
+__global__ __launch_bounds__(256) void layout_kernel(Matrix first, Order order, int first_blocks, Matrix second,
+                                                     int dim, int dp,
                                                      const float* __restrict__ largest, int first_n, int second_n,
                                                      float* __restrict__ units) {
   const bool other = (int)blockIdx.x >= first_blocks;
@@ -249,7 +260,9 @@ __device__ __forceinline__ float weight(float x, float x_all, float scale) {
 // ------------------------------------------------------------------ forward
 // The logits of a tile (vocabulary m x rows n), reduced to one pair per row:
 // stats[tile * rows + row] = (x, sum), see settled().  The tile that holds a row's
-// target also writes its dot product, upright.
+// target also writes its dot product, upright.  Bound by the matrix cores (and the
+// power they may draw) where rows are many, 65536 x 32768 x 512 bf16 at 880 TFLOP/s;
+// by the read of the table where they are few, one row x 32000 x 512 in 11 us (3 TB/s).
 template <class S, typename T>
 __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, Operand features, int dim,
                                                                  int products, float logit_scale2,
@@ -281,7 +294,8 @@ __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, 
 #pragma unroll
   for (int b = 0; b < S::kNB; ++b) {
     const int n = n0 + wn + 32 * b + (lane & 31);
-    const int label_at = from_first(n < features.extent ? targets.at(order.row(n)) : -1, 0, first, S::kWaveM, table.extent);
+    const int64_t target = n < features.extent ? targets.at(order.row(n)) : -1;
+    const int label_at = from_first(target, 0, first, S::kWaveM, table.extent);
     if (__any(label_at >= 0)) {
       float label = 0.0f;
       bool mine = false;
@@ -367,9 +381,10 @@ __device__ __forceinline__ void write_total(Sum s, int reduction, float* loss, i
 }
 
 // Joins the tiles' pairs of each row (kLanes lanes a row, in a fixed order):
-// norm = (x, 1 / sum, the label's dot product) for the backward, and the loss;
-// (by the order's rows; the loss by the features'); ignored rows give 0, targets outside the vocabulary NaN.  With a reduction the
-// block's sum goes to partial[block], or, when there is one block in all, to the result.
+// norm = (x, 1 / sum, the label's dot product) for the backward, at the row's place
+// in the order, and the loss at its own; ignored rows give 0, targets outside the
+// vocabulary NaN.  With a reduction the block's sum goes to partial[block], or, when
+// there is one block in all, to the result.
 template <int kLanes>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float2* __restrict__ stats,
                                                             const float* __restrict__ label_dot, int rows,
@@ -507,7 +522,8 @@ __device__ __forceinline__ bool row_counts(const uint64_t* counts, int64_t row) 
 
 // ds of a piece: tiles of (vocabulary m x rows n) like the forward's, stored as
 // ds[row * ld + m] (planes for fp32); rows that do not count and vocabulary
-// past the end are zeros.
+// past the end are zeros.  As the forward, with an epilogue that the one workgroup
+// of a CU does not hide: 65536 x 32768 x 512 bf16 in 3.0 ms where the forward takes 2.5.
 template <class S, typename T, int kPlanes>
 __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, Operand features, int dim,
                                                                  int products, float logit_scale2,
@@ -605,8 +621,10 @@ __global__ __launch_bounds__(S::kThreads) void logits_bwd_kernel(Operand table, 
 // features or of the table), m the D columns.  kTableGrad: dw (both operands in
 // K rows, K the rows of the piece); else dh (ds along K, K the vocabulary).
 // With `part` set the tile goes, in fp32, to plane blockIdx.y of part (added to
-// what is there if `add`); else out = the gradient of the tile's sums in the result's type (alpha, unit: see factor_of).
+// what is there if `add`); else out = the gradient of the tile's sums in the
+// result's type (alpha, unit: see factor_of).
 // counts (dh): rows that do not count are zero; order: of the features, K (dw) or n (dh).
+// Bound by the matrix cores: 1000 TFLOP/s for either gradient of 65536 x 32768 x 512 bf16.
 template <class S, typename T, typename Out, bool kTableGrad>
 __global__ __launch_bounds__(S::kThreads) void grad_kernel(Operand x, Operand ds, int32_t K,
                                                            int products, const uint64_t* __restrict__ counts,
@@ -656,13 +674,14 @@ __global__ __launch_bounds__(S::kThreads) void grad_kernel(Operand x, Operand ds
   }
 }
 
-// out = the gradient of the planes' sum; dh: counts, rows that do not count are
-// zero, and order, where they go.  dw: counts null, order as it is.  kGroups threads share an element's planes, their sums joined in
-// order.
+// out = the gradient of the planes' sum.  dh: rows that do not count (counts) are
+// zero, and order says where a row goes; dw: counts null.  kGroups threads share an
+// element's planes, their sums joined in order.
 template <int kGroups, typename T, typename Out>
 __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ part, int planes, int64_t plane,
                                                      int64_t n, int D, const uint64_t* __restrict__ counts,
-                                                     Order order, const double* __restrict__ alpha, const float* __restrict__ unit,
+                                                     Order order, const double* __restrict__ alpha,
+                                                     const float* __restrict__ unit,
                                                      Out* __restrict__ out) {
   constexpr int kElements = 256 / kGroups;
   __shared__ float lds[256];
@@ -720,7 +739,10 @@ struct Problem {
   size_t element() const { return dtype == GS_FP32 ? 4 : 2; }
   // Are the features' rows put in an order (struct Order)?  It takes two small
   // kernels and, for rows that the loads can take in place, a copy of them, whether
-  // rows are ignored or not.
+  // rows are ignored or not.  With gradients, without and with it, at 0, 10 and 40 %
+  // of rows ignored: 65536 x 1024 x 64 fp32 202 / 208, 200 / 197, 190 / 165 us (half
+  // the vocabulary: 145 / 149, 139 / 140, 131 / 121); 32768 x 8192 x 512 bf16, in
+  // place, 1286 / 1305, 1291 / 1216, 1273 / 922 us.
   bool orders() const {
     const int64_t logits = rows * vocab;
     return packs(ld_features) ? logits >= 1ll << 26 : vocab >= 8192 && logits >= 1ll << 28;
@@ -832,6 +854,8 @@ struct State {
 // Short rows: the kernels that hold one operand in registers (gs_resident.h).
 // The forward alone needs fewer of them, and goes twice as far.
 static bool resident(const Problem& p) { return p.dp() <= (p.dtype == GS_FP32 ? 64 : 128); }
+// Against tiles it needs logits enough to fill its parts: 4096 x 4096 bf16 17 and 18
+// us at D = 64, 25 and 22 at 256; 65536 x 1024 24 and 42, 48 and 61.
 static bool resident_forward(const Problem& p) {
   const int64_t blocks = ceil_div(p.dp(), 64) * p.planes();
   return blocks <= 4 && p.rows * p.vocab >= blocks * (3ll << 22);
@@ -898,6 +922,9 @@ template <class S>
 static int64_t tiles_of(const Problem& p) {
   return ceil_div(p.vocab, S::BM) * ceil_div(p.rows, S::BN);
 }
+// Thin tiles, where a launch of them fits the chip at once: 200 rows x 1203 x 512 bf16
+// take 12.5 us in 32-wide, 13.6 in 64-wide and 16.1 in Mid tiles, 64 x 32000 20.7,
+// 17.0 (500 tiles) and 17.4, 100 x 32000 30.2, 22.7 (1000 tiles) and 17.9.
 constexpr int64_t kThinTiles = 512;
 
 struct ForwardPlan {
@@ -915,9 +942,12 @@ struct ForwardPlan {
     shape = tiles_of<Thin32>(p) <= kThinTiles ? kThin32 : tiles_of<Thin64>(p) <= kThinTiles ? kThin64
             : resident_forward(p) ? kResident : takes_big(p.vocab, p.rows) ? kBig : kMid;
     const int bm = shape == kBig ? Big::BM : shape == kMid ? Mid::BM : Thin32::BM;
-    tiles_m = shape == kResident ? resident_parts(p.rows, p.vocab, resident_forward_slots(p), 0.0) : ceil_div(p.vocab, bm);
+    tiles_m = shape == kResident ? resident_parts(p.rows, p.vocab, resident_forward_slots(p), 0.0)
+                                 : ceil_div(p.vocab, bm);
     rows_piece = max((int64_t)256, kStatBytes / (tiles_m * (int64_t)sizeof(float2)) / 256 * 256);
     rows_piece = min(p.rows, min(rows_piece, (int64_t)1 << 20));
+    // of a row, in the kernel that joins (1024 rows x 32768 x 256 in all: 35 us with 64
+    // lanes, 55 with one; 8192 rows 155 and 146)
     lanes = p.rows <= 4096 && tiles_m >= 16 ? 64 : 1;
     blocks = 0;
     for (int64_t r = 0; r < p.rows; r += rows_piece)
@@ -976,19 +1006,24 @@ static int forward(const Problem& p, Targets targets, float logit_scale, int red
     const int64_t blocks = ceil_div(rows, kJoinThreads / f.lanes);
     auto* join = f.lanes == 64 ? join_kernel<64> : join_kernel<1>;
     join<<<(unsigned)blocks, kJoinThreads, 0, s>>>(f.stats, f.label, (int)rows, (int)f.tiles_m, p.vocab, scale2,
-                                                   f.layouts.units, targets, order, reduction, norm ? norm + r : nullptr,
+                                                   f.layouts.units, targets, order, reduction,
+                                                   norm ? norm + r : nullptr,
                                                    reduction == GS_REDUCE_NONE ? loss : nullptr,
                                                    f.partial + block, f.blocks == 1, loss, count);
     block += blocks;
   }
-  if (f.blocks > 1 && reduction != GS_REDUCE_NONE) total_kernel<<<1, kJoinThreads, 0, s>>>(f.partial, f.blocks, reduction, loss, count);
+  if (f.blocks > 1 && reduction != GS_REDUCE_NONE)
+    total_kernel<<<1, kJoinThreads, 0, s>>>(f.partial, f.blocks, reduction, loss, count);
   return gs_status_from_hip(hipGetLastError());
 }
 
 // How a gradient's product of (N x D) over K is done: in which tiles, and in how
 // many parts along K.  The time in microseconds: whole rounds of the chip's 256
 // CUs (one Big workgroup each, or two Mid ones), each a part's steps and about
-// four steps' time to begin and end; and what it takes to write and add the parts' fp32 sums.
+// four steps' time to begin and end; and what it takes to write and add the parts'
+// fp32 sums.  Of all tiles and parts it takes the fastest or one within 6 % for dh
+// and dw of 15 sizes from 16 x 32000 x 512 to 65536 x 64 x 512, where the worst are 2
+// to 4 times slower.
 struct Split {
   bool big;
   int parts;
@@ -998,12 +1033,14 @@ static Split split_of(int64_t N, int64_t D, int64_t K, int products) {
   double least = 1e300;
   const int64_t steps = ceil_div(K, kBK) * products;
   for (int big = 0; big < 2; ++big) {
-    const int64_t tiles = big ? ceil_div(N, Big::BN) * ceil_div(D, Big::BM) : ceil_div(N, Mid::BN) * ceil_div(D, Mid::BM);
+    const int64_t tiles = big ? ceil_div(N, Big::BN) * ceil_div(D, Big::BM)
+                              : ceil_div(N, Mid::BN) * ceil_div(D, Mid::BM);
     const int64_t most = max((int64_t)1, min(K / (4 * kBK), (int64_t)256));
     for (int64_t n = 1; n <= most; ++n) {
       const int64_t blocks = tiles * n;
       const double round = big ? 2.1 * ceil_div(blocks, 256) : blocks <= 256 ? 0.8 : 1.24 * ceil_div(blocks, 512);
-      const double cost = round * (double)(ceil_div(steps, n) + 4) + (n > 1 ? 3.0 + (double)n * N * D * 8.0 / 4.0e6 : 0.0);
+      const double sums = n > 1 ? 3.0 + (double)n * N * D * 8.0 / 4.0e6 : 0.0;
+      const double cost = round * (double)(ceil_div(steps, n) + 4) + sums;
       if (cost < least) {
         least = cost;
         best = {big == 1, (int)n};
@@ -1074,7 +1111,8 @@ struct BackwardPlan {
     alpha = c.take<double>(1);
     largest = c.take<float>(kLargestBlocks);
     part_h = c.take<float>(want_h && !direct_h ? parts_h * rows_piece * p.dim : 0);
-    part_t = c.take<float>(want_t && !direct_t ? parts_t * (row_pieces > 1 ? (int64_t)p.vocab : cols_piece) * p.dim : 0);
+    const int64_t table_rows = row_pieces > 1 ? (int64_t)p.vocab : cols_piece;
+    part_t = c.take<float>(want_t && !direct_t ? parts_t * table_rows * p.dim : 0);
     bytes = c.at;
   }
 };
@@ -1084,9 +1122,11 @@ static unsigned finish_blocks(int64_t n) { return (unsigned)min(ceil_div(n, 256)
 template <typename T, typename Out>
 static void finish(const float* part, int planes, int64_t plane, int64_t n, int D, const uint64_t* counts,
                    const Order& order, const double* alpha, const float* unit, Out* out, hipStream_t s) {
-  // many planes of few elements (a small table's) do not fill the chip by their elements alone
-  if (planes >= 16) finish_kernel<8, T><<<finish_blocks(n * 8), 256, 0, s>>>(part, planes, plane, n, D, counts, order, alpha, unit, out);
-  else finish_kernel<1, T><<<finish_blocks(n), 256, 0, s>>>(part, planes, plane, n, D, counts, order, alpha, unit, out);
+  // many planes of few elements (a small table's) do not fill the chip by their
+  // elements alone: 65536 x 512 x 64 with gradients 69 us, and 100 with a thread an element
+  const bool many = planes >= 16;
+  auto* kernel = many ? finish_kernel<8, T, Out> : finish_kernel<1, T, Out>;
+  kernel<<<finish_blocks(many ? n * 8 : n), 256, 0, s>>>(part, planes, plane, n, D, counts, order, alpha, unit, out);
 }
 
 template <typename T, typename Out, int kPlanes>
@@ -1102,9 +1142,9 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
   }
   const Layouts& layouts = state.layouts;
   const float *unit_h = layouts.features_unit(), *unit_w = layouts.table_unit();
-  rows_kernel<<<(unsigned)ceil_div(p.rows, 256), 256, 0, s>>>(grad_loss, p.rows, p.vocab, targets, layouts.order(), reduction, count, state.norm,
-                                                              logit_scale, scale2, layouts.units, Held<T>::kScale,
-                                                              b.largest, largest_n, b.info, b.counts, b.alpha);
+  rows_kernel<<<(unsigned)ceil_div(p.rows, 256), 256, 0, s>>>(
+      grad_loss, p.rows, p.vocab, targets, layouts.order(), reduction, count, state.norm, logit_scale, scale2,
+      layouts.units, Held<T>::kScale, b.largest, largest_n, b.info, b.counts, b.alpha);
   const Operand table = layouts.table(p);
   if (resident(p)) {
     const Operand features = layouts.features(p, 0, p.rows, s);
@@ -1130,9 +1170,11 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
         finish<T>(sums, parts, a.part_plane, a.part_plane, D, counts, layouts.order(), b.alpha, unit, out, s);
     };
     if (grad_features)
-      run(std::integral_constant<int, gs_resident::kFeatures>{}, features, table, b.parts_h, b.part_h, unit_w, grad_features, b.counts);
+      run(std::integral_constant<int, gs_resident::kFeatures>{}, features, table, b.parts_h, b.part_h, unit_w,
+          grad_features, b.counts);
     if (grad_table)
-      run(std::integral_constant<int, gs_resident::kTable>{}, table, features, b.parts_t, b.part_t, unit_h, grad_table, nullptr);
+      run(std::integral_constant<int, gs_resident::kTable>{}, table, features, b.parts_t, b.part_t, unit_h,
+          grad_table, nullptr);
     return gs_status_from_hip(hipGetLastError());
   }
   for (int64_t r = 0; r < p.rows; r += b.rows_piece) {
@@ -1181,15 +1223,18 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
               x, ds, rows, p.ds_products(), counts, order, tiles_m, part, part_plane, r > 0, b.alpha, unit_h,
               grad_table + c * D);
           if (part && b.row_pieces == 1)
-            finish<T>(part, b.parts_t, part_plane, (int64_t)cols * D, D, nullptr, Order{}, b.alpha, unit_h, grad_table + c * D, s);
+            finish<T>(part, b.parts_t, part_plane, (int64_t)cols * D, D, nullptr, Order{}, b.alpha, unit_h,
+                      grad_table + c * D, s);
         });
       }
     }
     if (grad_features && !b.direct_h)
-      finish<T>(b.part_h, b.parts_h, (int64_t)rows * D, (int64_t)rows * D, D, counts, order, b.alpha, unit_w, grad_features, s);
+      finish<T>(b.part_h, b.parts_h, (int64_t)rows * D, (int64_t)rows * D, D, counts, order, b.alpha, unit_w,
+                grad_features, s);
   }
   if (grad_table && b.row_pieces > 1)
-    finish<T>(b.part_t, b.parts_t, (int64_t)p.vocab * D, (int64_t)p.vocab * D, D, nullptr, Order{}, b.alpha, unit_h, grad_table, s);
+    finish<T>(b.part_t, b.parts_t, (int64_t)p.vocab * D, (int64_t)p.vocab * D, D, nullptr, Order{}, b.alpha, unit_h,
+              grad_table, s);
   return gs_status_from_hip(hipGetLastError());
 }
 
@@ -1293,8 +1338,8 @@ extern "C" int gs_xent_bwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dty
   const gs_xent::State kept(p, const_cast<void*>(state));
   const gs_xent::Targets t = {targets, target_bits, ignore_index};
   if (dtype == GS_FP32)
-    return gs_xent::backward<_Float16, float, gs_tile::kWidePlanes>(p, t, logit_scale, reduction, kept, count, grad_loss,
-                                                                    (float*)grad_features, (float*)grad_table, b, s);
+    return gs_xent::backward<_Float16, float, gs_tile::kWidePlanes>(
+        p, t, logit_scale, reduction, kept, count, grad_loss, (float*)grad_features, (float*)grad_table, b, s);
   if (dtype == GS_BF16)
     return gs_xent::backward<__bf16, __bf16, 1>(p, t, logit_scale, reduction, kept, count, grad_loss,
                                                 (__bf16*)grad_features, (__bf16*)grad_table, b, s);
