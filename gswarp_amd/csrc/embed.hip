@@ -15,6 +15,7 @@
 // sort: see few_kernel.
 #include "gs_capi.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace gs_embed {
@@ -478,9 +479,9 @@ static int forward(int64_t n, int32_t vocab, int32_t dim, Tokens tokens, const v
   return with_vectors<T>(dim, ld, table, out, [&](auto V, auto kWhole) {
     const int64_t row_vectors = ceil_div(dim, V);
     // a launch has fewer than 2^32 threads
-    const int64_t most = max((int64_t)1, kMaxLookup / row_vectors);
+    const int64_t most = std::max((int64_t)1, kMaxLookup / row_vectors);
     for (int64_t i = 0; i < n; i += most) {
-      const int64_t here = min(most, n - i);
+      const int64_t here = std::min(most, n - i);
       lookup_kernel<T, V, kWhole><<<(unsigned)ceil_div(here * row_vectors, kThreads), kThreads, 0, s>>>(
           tokens.from(i), here, (u32)vocab, dim, (u32)row_vectors, (const T*)table, ld, scale, (T*)out + i * dim);
     }
@@ -502,13 +503,13 @@ static int lanes_of(int D, int V) {
 // so that at most 64 chunks hand on to the next level: few levels, and none that
 // leaves many rows to one workgroup (2048 rows of 256 bytes take one 43 us).
 static int group_length(int64_t n, int lanes, bool first) {
-  const int groups = kRunThreads / lanes, most = min(64, kMaxChunk / groups);
+  const int groups = kRunThreads / lanes, most = std::min(64, kMaxChunk / groups);
   // (above, even: a part begins with a chunk's first entry, so that what is empty
   // between two entries of a run is one at most, and before the part)
-  if (!first && n <= groups * min(8, most)) return (int)round_up(ceil_div(n, groups), 2);
-  int length = first ? 4 : min(8, most);
+  if (!first && n <= groups * std::min(8, most)) return (int)round_up(ceil_div(n, groups), 2);
+  int length = first ? 4 : std::min(8, most);
   while (2 * length <= most && n / (length * groups) > (first ? 512 : 64)) length *= 2;
-  return min(length, most);
+  return std::min(length, most);
 }
 
 static int64_t chunks_of(int64_t n, int lanes, bool first) {
@@ -575,8 +576,9 @@ static int gradient(int64_t n, int32_t vocab, int32_t dim, Tokens tokens, const 
                                                        out);
     return gs_status_from_hip(hipGetLastError());
   }
-  keys_kernel<<<(unsigned)min(ceil_div(n, kThreads), (int64_t)8192), kThreads, 0, s>>>(tokens, n, (u32)vocab, padding,
-                                                                                     b.keys, b.positions);
+  const int64_t key_blocks = std::min(ceil_div(n, kThreads), (int64_t)8192);
+  keys_kernel<<<(unsigned)key_blocks, kThreads, 0, s>>>(tokens, n, (u32)vocab, padding,
+                                                        b.keys, b.positions);
   int passes = 0;
   const int status = gs_sort_pairs_u32_any(n, gs_bit_length(vocab), b.keys, b.positions, b.keys_alt, b.positions_alt,
                                            b.sort_scratch, b.sort_bytes, &passes, (void*)s);
@@ -612,7 +614,7 @@ static int backward(int64_t n, int32_t vocab, int32_t dim, Tokens tokens, const 
                     int64_t padding, void* out, const BackwardPlan& b, hipStream_t s) {
   if (n == 0) {
     const int64_t all = (int64_t)vocab * dim;
-    zero_kernel<T><<<(unsigned)min(ceil_div(all, kThreads), (int64_t)8192), kThreads, 0, s>>>((T*)out, all);
+    zero_kernel<T><<<(unsigned)std::min(ceil_div(all, kThreads), (int64_t)8192), kThreads, 0, s>>>((T*)out, all);
     return gs_status_from_hip(hipGetLastError());
   }
   return with_vectors<T>(dim, dim, grad, out, [&](auto V, auto kWhole) {

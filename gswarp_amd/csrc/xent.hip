@@ -17,6 +17,7 @@
 #include "gs_tile.h"
 #include "gs_xent.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace gs_xent {
@@ -810,7 +811,7 @@ struct Layouts {
       const int V = p.dim % 4 == 0 && fits(f) && fits(t) ? 4 : 1;
       int lanes = 1;
       while (lanes < 64 && lanes * V < p.dim) lanes *= 2;
-      auto blocks = [&](int64_t n) { return (int)min(ceil_div(n, 8 * (256 / lanes)), (int64_t)kLargestBlocks); };
+      auto blocks = [&](int64_t n) { return (int)std::min(ceil_div(n, 8 * (256 / lanes)), (int64_t)kLargestBlocks); };
       features_n = blocks(p.rows);
       table_n = blocks(p.vocab);
       auto* kernel = V == 4 ? magnitude_kernel<4> : magnitude_kernel<1>;
@@ -819,7 +820,7 @@ struct Layouts {
     lay_out(p, rows == p.rows && p.packs_features() ? f : Matrix{}, order(), p.packs(p.ld_table) ? t : Matrix{}, s);
   }
   void lay_out(const Problem& p, const Matrix& f, const Order& order, const Matrix& t, hipStream_t s) const {
-    auto blocks = [&](const Matrix& m) { return (int)min(ceil_div(m.rows * (p.dp() / 8), 256), (int64_t)4096); };
+    auto blocks = [&](const Matrix& m) { return (int)std::min(ceil_div(m.rows * (p.dp() / 8), 256), (int64_t)4096); };
     const int fn = blocks(f), tn = blocks(t);
     if (fn + tn == 0) return;
     auto* kernel = p.dtype == GS_FP32 ? layout_kernel<float> : layout_kernel<_Float16>;
@@ -869,7 +870,7 @@ static int resident_forward_slots(const Problem& p) { return ceil_div(p.dp(), 64
 // a tile's microsecond.
 static int resident_parts(int64_t held, int64_t stream, int64_t slots, double sum_bytes) {
   const int64_t blocks = ceil_div(held, gs_resident::kHeldRows), tiles = ceil_div(stream, gs_resident::kTileRows);
-  const int64_t most = min(max((int64_t)1, tiles / 4), max((int64_t)4, 2 * ceil_div(slots, blocks)));
+  const int64_t most = std::min(std::max((int64_t)1, tiles / 4), std::max((int64_t)4, 2 * ceil_div(slots, blocks)));
   int64_t best = 1;
   double least = 1e300;
   for (int64_t n = 1; n <= most; ++n) {
@@ -944,14 +945,14 @@ struct ForwardPlan {
     const int bm = shape == kBig ? Big::BM : shape == kMid ? Mid::BM : Thin32::BM;
     tiles_m = shape == kResident ? resident_parts(p.rows, p.vocab, resident_forward_slots(p), 0.0)
                                  : ceil_div(p.vocab, bm);
-    rows_piece = max((int64_t)256, kStatBytes / (tiles_m * (int64_t)sizeof(float2)) / 256 * 256);
-    rows_piece = min(p.rows, min(rows_piece, (int64_t)1 << 20));
+    rows_piece = std::max((int64_t)256, kStatBytes / (tiles_m * (int64_t)sizeof(float2)) / 256 * 256);
+    rows_piece = std::min(p.rows, std::min(rows_piece, (int64_t)1 << 20));
     // of a row, in the kernel that joins (1024 rows x 32768 x 256 in all: 35 us with 64
     // lanes, 55 with one; 8192 rows 155 and 146)
     lanes = p.rows <= 4096 && tiles_m >= 16 ? 64 : 1;
     blocks = 0;
     for (int64_t r = 0; r < p.rows; r += rows_piece)
-      blocks += ceil_div(min(rows_piece, p.rows - r), kJoinThreads / lanes);
+      blocks += ceil_div(std::min(rows_piece, p.rows - r), kJoinThreads / lanes);
     Carve c{(char*)ws};
     if (!kept) layouts = Layouts(p, rows_piece, c);
     layouts.largest = c.take<float>(p.dtype == GS_FP32 ? 2 * kLargestBlocks : 0);
@@ -980,7 +981,7 @@ static int forward(const Problem& p, Targets targets, float logit_scale, int red
   const Operand table = f.layouts.table(p);
   int64_t block = 0;
   for (int64_t r = 0; r < p.rows; r += f.rows_piece) {
-    const int64_t rows = min(f.rows_piece, p.rows - r);
+    const int64_t rows = std::min(f.rows_piece, p.rows - r);
     const Operand features = f.layouts.features(p, r, rows, s);
     const Order order = f.layouts.order().from(r);
     switch (f.shape) {
@@ -1035,7 +1036,7 @@ static Split split_of(int64_t N, int64_t D, int64_t K, int products) {
   for (int big = 0; big < 2; ++big) {
     const int64_t tiles = big ? ceil_div(N, Big::BN) * ceil_div(D, Big::BM)
                               : ceil_div(N, Mid::BN) * ceil_div(D, Mid::BM);
-    const int64_t most = max((int64_t)1, min(K / (4 * kBK), (int64_t)256));
+    const int64_t most = std::max((int64_t)1, std::min(K / (4 * kBK), (int64_t)256));
     for (int64_t n = 1; n <= most; ++n) {
       const int64_t blocks = tiles * n;
       const double round = big ? 2.1 * ceil_div(blocks, 256) : blocks <= 256 ? 0.8 : 1.24 * ceil_div(blocks, 512);
@@ -1083,11 +1084,11 @@ struct BackwardPlan {
     // shorter, whose gradient's sums then wait from piece to piece; that one is the smaller.
     const int64_t most = kPieceBytes / (2 * p.ds_planes());  // elements of ds
     if (p.rows > p.vocab) {
-      cols_piece = min((int64_t)p.vocab, most / kLeastSide / 256 * 256);
-      rows_piece = min(p.rows, most / round_up(cols_piece, 256) / 256 * 256);
+      cols_piece = std::min((int64_t)p.vocab, most / kLeastSide / 256 * 256);
+      rows_piece = std::min(p.rows, most / round_up(cols_piece, 256) / 256 * 256);
     } else {
-      rows_piece = min(p.rows, most / kLeastSide / 256 * 256);
-      cols_piece = min((int64_t)p.vocab, most / rows_piece / 256 * 256);
+      rows_piece = std::min(p.rows, most / kLeastSide / 256 * 256);
+      cols_piece = std::min((int64_t)p.vocab, most / rows_piece / 256 * 256);
     }
     ld = round_up(cols_piece, 256);
     const Split h = split_of(rows_piece, p.dim, cols_piece, p.ds_products());
@@ -1117,7 +1118,7 @@ struct BackwardPlan {
   }
 };
 
-static unsigned finish_blocks(int64_t n) { return (unsigned)min(ceil_div(n, 256), (int64_t)8192); }
+static unsigned finish_blocks(int64_t n) { return (unsigned)std::min(ceil_div(n, 256), (int64_t)8192); }
 
 template <typename T, typename Out>
 static void finish(const float* part, int planes, int64_t plane, int64_t n, int D, const uint64_t* counts,
@@ -1137,7 +1138,7 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
   const int D = p.dim;
   int largest_n = 0;
   if (reduction == GS_REDUCE_NONE) {
-    largest_n = (int)min(ceil_div(p.rows, 256), (int64_t)kLargestBlocks);
+    largest_n = (int)std::min(ceil_div(p.rows, 256), (int64_t)kLargestBlocks);
     largest_kernel<<<largest_n, 256, 0, s>>>(grad_loss, p.rows, targets, b.largest);
   }
   const Layouts& layouts = state.layouts;
@@ -1178,13 +1179,13 @@ static int backward(const Problem& p, Targets targets, float logit_scale, int re
     return gs_status_from_hip(hipGetLastError());
   }
   for (int64_t r = 0; r < p.rows; r += b.rows_piece) {
-    const int32_t rows = (int32_t)min(b.rows_piece, p.rows - r);
+    const int32_t rows = (int32_t)std::min(b.rows_piece, p.rows - r);
     const Operand features = layouts.features(p, r, rows, s);
     const uint64_t* counts = b.counts + r / 64;
     const Order order = layouts.order().from(r);
     const int64_t ds_plane = rows * b.ld;
     for (int64_t c = 0; c < p.vocab; c += b.cols_piece) {
-      const int32_t cols = (int32_t)min(b.cols_piece, p.vocab - c);
+      const int32_t cols = (int32_t)std::min(b.cols_piece, p.vocab - c);
       Operand piece = table;  // the piece's rows of the table
       piece.p += c * table.ld;
       piece.extent = cols;

@@ -607,3 +607,15 @@ def test_entropy_of_many_rows_of_which_some_count(device, dtype, rows, vocab, di
         value, bound = value + want["table"][0], bound + want["table"][1]
     ref.check(grads[1], (value, bound), "table")
     assert abs(float(mean) - total / len(kept)) <= 1e-5 * max(1.0, abs(total / len(kept)))
+
+
+@pytest.mark.parametrize("dim", [1, 8, 13])
+def test_lookup_of_short_rows_is_few_launches(device, dim):
+    """Rows of one vector: a pass costs what its bytes do, not a launch for each row."""
+    table = torch.randn(34, dim, generator=_gen(dim)).to(device, BF16)
+    tokens = torch.randint(0, 34, (300_001,), generator=_gen(dim)).to(device)
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as trace:
+        out = vocabulary.embed_tokens(tokens, table)
+        torch.cuda.synchronize()
+    assert torch.equal(out, table[tokens])
+    assert sum(e.count for e in trace.key_averages() if "lookup" in e.key) <= 1
