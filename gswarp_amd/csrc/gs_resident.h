@@ -237,7 +237,7 @@ __global__ __launch_bounds__(kThreads, kKind == kForward && KB * PL <= 2 ? 4 : 2
   for (int t = 0; t < kAhead; ++t)
     if (t < tiles) load();
 
-  float x = -INFINITY, sum = 0.0f;  // kForward, see settled()
+  float x = -INFINITY, sum = -1.0f;  // kForward: the largest, and the sum over all but it; see settled()
   f32x16 acc[kSums][kDBlocks];
   if (kKind != kForward) {
 #pragma unroll
@@ -288,7 +288,7 @@ __global__ __launch_bounds__(kThreads, kKind == kForward && KB * PL <= 2 ? 4 : 2
         for (int e = 0; e < 16; ++e) part[e & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], scale, -top));
       const float all = (part[0] + part[1]) + (part[2] + part[3]);
       if (now > x) {  // the largest so far is among these
-        sum = sum * __builtin_amdgcn_exp2f((x - now) * scale) + settled(now, scale, all);
+        sum = (1.0f + sum) * __builtin_amdgcn_exp2f((x - now) * scale) + settled(now, scale, all);
         x = now;
       } else {
         sum += all * (1.0f - (now == -INFINITY ? 0.0f : __builtin_fmaf(now, scale, -top)) * kLn2f);
@@ -439,10 +439,9 @@ __global__ __launch_bounds__(kThreads, kKind == kForward && KB * PL <= 2 ? 4 : 2
 
   if constexpr (kKind == kForward) {
     // the two halves of the wave hold the same rows
-    const float ox = __shfl_xor(x, 32), osum = __shfl_xor(sum, 32), all = fmaxf(x, ox), scale = fabsf(scale2);
-    sum = sum * (x == all ? 1.0f : __builtin_amdgcn_exp2f((x - all) * scale)) +
-          osum * (ox == all ? 1.0f : __builtin_amdgcn_exp2f((ox - all) * scale));
-    if (held_in && half == 0) a.stats[(int64_t)blockIdx.y * a.held.extent + held_row] = make_float2(all, sum);
+    const float2 other = make_float2(__shfl_xor(x, 32), __shfl_xor(sum, 32));
+    const float2 all = gs_xent::joined(make_float2(x, sum), other, fabsf(scale2));
+    if (held_in && half == 0) a.stats[(int64_t)blockIdx.y * a.held.extent + held_row] = all;
   } else {
     if (!held_in) return;
     const float factor = a.part_sums ? 0.0f : gs_xent::factor_of(a.alpha, a.unit);

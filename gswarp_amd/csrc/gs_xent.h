@@ -39,16 +39,28 @@ __device__ __forceinline__ float scale_of(float scale2, const float* units) {
 }
 
 // A row's maximum and sum are kept as the largest dot product itself, x (turned
-// upright: times the sign of the scale), and the sum of 2^((x_j - x) scale), in
-// which the largest is exactly 1: a label that is all but certain then has a
+// upright: times the sign of the scale), and the sum of 2^((x_j - x) scale) over all
+// others: x's own 1 is added in 64 bits.  A label that is all but certain then has a
 // loss, and p - 1, as small as fp32 can tell, not as small as the rounding of the logits' size.
-// Its terms are formed with one fma as 2^(x_j scale - top), top = x scale rounded;
-// this takes the sum of a set that holds x itself from there.
+// The terms are formed with one fma as 2^(x_j scale - top), top = x scale rounded;
+// this takes the sum of a set that holds x itself from there.  (1 added here would
+// round once more, and up wherever the first rounding left a tie.)
 constexpr float kLn2f = 0.6931471805599453f;
 __device__ __forceinline__ float settled(float x, float scale, float sum) {
   const float top = x * scale, off = __builtin_fmaf(x, scale, -top);
   const float rest = sum - __builtin_amdgcn_exp2f(off);  // all but x
-  return 1.0f + __builtin_fmaf(rest, -off * kLn2f, rest);
+  return __builtin_fmaf(rest, -off * kLn2f, rest);
+}
+
+// What a sum under x weighs under x_all >= x.
+__device__ __forceinline__ float weight(float x, float x_all, float scale) {
+  return x == x_all ? 1.0f : __builtin_amdgcn_exp2f((x - x_all) * scale);
+}
+
+// Two sets' (x, sum over all but x) as one.  That of nothing is (-inf, -1).
+__device__ __forceinline__ float2 joined(float2 a, float2 b, float scale) {
+  const float2 top = b.x > a.x ? b : a, low = b.x > a.x ? a : b;
+  return make_float2(fmaxf(a.x, b.x), top.y + (1.0f + low.y) * weight(low.x, top.x, scale));
 }
 
 // What the backward needs of a row, f the factor of its loss's gradient (held

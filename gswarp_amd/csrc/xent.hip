@@ -248,19 +248,14 @@ __device__ __forceinline__ int from_first(int64_t target, int64_t base, int firs
   return d >= 0 && d < wave_m ? d : -1;
 }
 
-// (x, sum) of a set from its largest and the sum that the fma formed; of nothing, (-inf, 0).
+// (x, sum over all but x) of a set from its largest and the sum that the fma formed (0, or NaN, where that is -inf).
 __device__ __forceinline__ float2 pair_of(float x, float scale, float sum) {
-  return make_float2(x, x == -INFINITY ? 0.0f : settled(x, scale, sum));
-}
-
-// What a sum under x weighs under x_all >= x.
-__device__ __forceinline__ float weight(float x, float x_all, float scale) {
-  return x == x_all ? 1.0f : __builtin_amdgcn_exp2f((x - x_all) * scale);
+  return make_float2(x, x == -INFINITY ? sum - 1.0f : settled(x, scale, sum));
 }
 
 // ------------------------------------------------------------------ forward
 // The logits of a tile (vocabulary m x rows n), reduced to one pair per row:
-// stats[tile * rows + row] = (x, sum), see settled().  The tile that holds a row's
+// stats[tile * rows + row] = (x, sum over all but x), see settled().  The tile that holds a row's
 // target also writes its dot product, upright.  Bound by the matrix cores (and the
 // power they may draw) where rows are many, 65536 x 32768 x 512 bf16 at 880 TFLOP/s;
 // by the read of the table where they are few, one row x 32000 x 512 in 11 us (3 TB/s).
@@ -342,10 +337,7 @@ __global__ __launch_bounds__(S::kThreads) void logits_fwd_kernel(Operand table, 
     float2 r = red[i];
 #pragma unroll
     for (int w = 1; w < S::kWavesM; ++w) {
-      const float2 o = red[w * S::BN + i];
-      const float x = fmaxf(r.x, o.x);
-      r.y = r.y * weight(r.x, x, scale2) + o.y * weight(o.x, x, scale2);
-      r.x = x;
+      r = joined(r, red[w * S::BN + i], scale2);
     }
     stats[(int64_t)tile.m * features.extent + n0 + i] = r;
   }
@@ -410,7 +402,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float2* __rest
   if (row < order.used(rows)) {
     for (int t = sub; t < tiles; t += kLanes) {
       const float2 o = stats[(int64_t)t * rows + row];
-      add(o.x, (double)o.y);
+      add(o.x, 1.0 + (double)o.y);
     }
   }
 #pragma unroll

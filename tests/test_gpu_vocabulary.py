@@ -619,3 +619,36 @@ def test_lookup_of_short_rows_is_few_launches(device, dim):
         torch.cuda.synchronize()
     assert torch.equal(out, table[tokens])
     assert sum(e.count for e in trace.key_averages() if "lookup" in e.key) <= 1
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab,dim,rows", [(5, 367, 40_000), (5, 64, 40_000), (129, 264, 20_000), (70, 200, 9)])
+def test_entropy_mean_of_small_losses_has_no_bias(device, dtype, vocab, dim, rows):
+    """Labels that lead by about 8: the rows' errors are roundings and average out.
+
+    A loss below 1/8 is the logarithm of 1 and a sum that fp32 rounds to 2^-24 once or twice, and of
+    terms whose exponents (up to 16 in base 2) are rounded to 2^-20: 2^-23 in all for a row, with
+    either sign, so 8 standard errors of the mean are 2^-20 / sqrt(rows), besides the fp32 scale's own 2^-25 of 8 times a loss.
+    """
+    gen = _gen(dim)
+    table = torch.randn(vocab, dim, generator=gen, dtype=torch.float64) / math.sqrt(dim)
+    label = torch.randint(0, vocab, (rows,), generator=gen)
+    features = torch.randn(rows, dim, generator=gen, dtype=torch.float64) + 8.0 * table[label]
+    features, table, label = features.to(device, dtype), table.to(device, dtype), label.to(device)
+    s = features.double() @ table.double().T
+    loss = torch.logsumexp(s, 1) - s.gather(1, label.unsqueeze(1)).squeeze(1)
+    got = vocabulary.linear_cross_entropy(features, table, label, reduction="none").double()
+    small = loss < 0.125
+    assert int(small.sum()) > rows // 4
+    bias = float((got - loss)[small].mean())
+    assert abs(bias) <= 2.0 ** -20 / math.sqrt(int(small.sum())) + 2.0 ** -22 * float(loss[small].mean()), bias
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab,dim", [(257, 320), (129, 320), (65, 64), (65, 320), (1025, 128)])
+def test_entropy_of_a_table_row_of_nan(device, dtype, vocab, dim):
+    """The last row of the table alone in its tile: no row's loss is a number."""
+    features, table, targets, gen = _problem(device, dtype, 700, vocab, dim, ignored=0.0)
+    table = table.detach().clone()
+    table[-1] = math.nan
+    assert torch.isnan(vocabulary.linear_cross_entropy(features.detach(), table, targets, reduction="none")).all()
