@@ -55,15 +55,18 @@ struct Operand {
 
 constexpr int kSplitPlanes = 2, kWidePlanes = 3;      // of an fp32 operand, of one of wide range
 constexpr int kSplitProducts = 3, kWideProducts = 4;  // of two fp32 operands, with a wide Y
+constexpr int kFinePlanes = 2, kFineProducts = 2;     // of a 16-bit X and a Y that is held more finely
 constexpr float kPlaneStep = 2048.0f;                 // what each plane is held times more than the one before
 // What is left of v behind its plane h, for the next one: exact, and two
 // instructions (the second takes h in 16 bits).
 __device__ __forceinline__ float behind(float v, _Float16 h) {
   return __builtin_fmaf((float)h, -kPlaneStep, v * kPlaneStep);
 }
-__device__ __forceinline__ float behind(float, __bf16) { return 0.0f; }  // (one plane only)
+__device__ __forceinline__ float behind(float v, __bf16 h) {
+  return __builtin_fmaf((float)h, -kPlaneStep, v * kPlaneStep);
+}
 // The planes of X and Y that product s of `products` takes: (hi, tiny) if there are
-// four, (lo, hi), (hi, lo), (hi, hi).  Before (lo, hi), if not the first, and
+// four, (lo, hi), (hi, lo), (hi, hi); of two, the last two.  Before (lo, hi), if not the first, and
 // before (hi, hi) the sums so far are divided by a step.
 __device__ __forceinline__ int plane_x(int products, int s) { return products > 1 && s == products - 3; }
 __device__ __forceinline__ int plane_y(int products, int s) {
@@ -281,7 +284,7 @@ __device__ __forceinline__ void multiply(Accumulators<S>& acc, int wm, int wn, c
 }
 
 // acc = the tile at (m0, n0), over K columns [k_begin, k_end) of
-// `products` products of planes (1, 3 or 4).  Every element outside the operands
+// `products` products of planes (1 to 4).  Every element outside the operands
 // counts as zero.  x_rows (X in K rows only, may be null): one bit per K row
 // (k_begin on a multiple of 64); rows whose bit is clear count as zero whatever
 // they hold.  lds: S::kLdsBytes, free for the caller after a barrier.

@@ -725,8 +725,17 @@ struct Problem {
   int64_t ld_table;
   int planes() const { return dtype == GS_FP32 ? gs_tile::kSplitPlanes : 1; }
   int products() const { return dtype == GS_FP32 ? gs_tile::kSplitProducts : 1; }
-  int ds_planes() const { return dtype == GS_FP32 ? gs_tile::kWidePlanes : 1; }
-  int ds_products() const { return dtype == GS_FP32 ? gs_tile::kWideProducts : 1; }
+  // Small problems of 16 bits hold ds in two planes: where few of its values decide a
+  // gradient their rounding does not average out (it came to 1.8 times the result's
+  // own), and there the products are not what takes the time: 38 x 8192 x 768 bf16
+  // with gradients 73 us in one plane, 78 in two.  Less so for short rows, which the
+  // kernels that hold them in registers have in one plane: 512 x 1024 x 64 39 and 62 us.
+  bool fine() const {
+    const int64_t logits = rows * vocab;
+    return dtype != GS_FP32 && logits <= 1ll << (dp() <= 128 ? 16 : 19) && logits * dim <= 1ll << 28;
+  }
+  int ds_planes() const { return dtype == GS_FP32 ? gs_tile::kWidePlanes : fine() ? gs_tile::kFinePlanes : 1; }
+  int ds_products() const { return dtype == GS_FP32 ? gs_tile::kWideProducts : fine() ? gs_tile::kFineProducts : 1; }
   int64_t dp() const { return round_up(dim, 8); }
   bool packs(int64_t ld) const { return dtype == GS_FP32 || dim % 8 || ld % 8 || ld > gs_tile::kMaxLd; }
   size_t element() const { return dtype == GS_FP32 ? 4 : 2; }
@@ -846,7 +855,7 @@ struct State {
 
 // Short rows: the kernels that hold one operand in registers (gs_resident.h).
 // The forward alone needs fewer of them, and goes twice as far.
-static bool resident(const Problem& p) { return p.dp() <= (p.dtype == GS_FP32 ? 64 : 128); }
+static bool resident(const Problem& p) { return p.dp() <= (p.dtype == GS_FP32 ? 64 : 128) && !p.fine(); }
 // Against tiles it needs logits enough to fill its parts: 4096 x 4096 bf16 17 and 18
 // us at D = 64, 25 and 22 at 256; 65536 x 1024 24 and 42, 48 and 61.
 static bool resident_forward(const Problem& p) {
@@ -1333,9 +1342,11 @@ extern "C" int gs_xent_bwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dty
   if (dtype == GS_FP32)
     return gs_xent::backward<_Float16, float, gs_tile::kWidePlanes>(
         p, t, logit_scale, reduction, kept, count, grad_loss, (float*)grad_features, (float*)grad_table, b, s);
-  if (dtype == GS_BF16)
-    return gs_xent::backward<__bf16, __bf16, 1>(p, t, logit_scale, reduction, kept, count, grad_loss,
-                                                (__bf16*)grad_features, (__bf16*)grad_table, b, s);
-  return gs_xent::backward<_Float16, _Float16, 1>(p, t, logit_scale, reduction, kept, count, grad_loss,
-                                                  (_Float16*)grad_features, (_Float16*)grad_table, b, s);
+  auto run = [&](auto* to_features, auto* to_table) {
+    typedef std::remove_pointer_t<decltype(to_table)> T;
+    auto* call = p.fine() ? gs_xent::backward<T, T, gs_tile::kFinePlanes> : gs_xent::backward<T, T, 1>;
+    return call(p, t, logit_scale, reduction, kept, count, grad_loss, to_features, to_table, b, s);
+  };
+  if (dtype == GS_BF16) return run((__bf16*)grad_features, (__bf16*)grad_table);
+  return run((_Float16*)grad_features, (_Float16*)grad_table);
 }

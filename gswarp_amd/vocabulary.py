@@ -228,8 +228,9 @@ def linear_cross_entropy(features: torch.Tensor, table: torch.Tensor, targets: t
     ``"mean"`` over the rows that count (NaN over none).  Rows whose target is ``ignore_index`` do not
     count: their loss and gradient are zero and they bring nothing to the table's gradient, whatever
     their features hold.  Any other target outside the vocabulary makes its row's loss NaN.
-    The logits' gradients enter the products in the inputs' type (float32: with 22 bits or more, in
-    steps of 2**-62 of the largest row's), and so rounded they decide the gradients' precision.
+    The logits' gradients enter the products in the inputs' type (in two parts of it where there are
+    few; float32: with 22 bits or more, in steps of 2**-62 of the largest row's), and so rounded they
+    decide the gradients' precision.
     """
     _check_table(table, "table", _MAX_CLASSES)
     device, dim = table.device, table.shape[1]

@@ -652,3 +652,34 @@ def test_entropy_of_a_table_row_of_nan(device, dtype, vocab, dim):
     table = table.detach().clone()
     table[-1] = math.nan
     assert torch.isnan(vocabulary.linear_cross_entropy(features.detach(), table, targets, reduction="none")).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("rows,vocab,dim", [(70_000, 1, 24), (40_000, 2, 16), (30_000, 3, 128), (40, 1700, 64),
+                                            (1, 66_000, 40), (5001, 67, 100), (1030, 65, 7), (300, 257, 72),
+                                            (2, 40_000, 128), (9000, 128, 1)])
+def test_entropy_of_short_rows_in_one_plane(device, dtype, rows, vocab, dim):
+    """16-bit rows of up to 128 values with logits enough for the kernels that keep them in registers."""
+    print(f"entropy {dtype} rows={rows} vocab={vocab} dim={dim}", flush=True)
+    features, table, targets, gen = _problem(device, dtype, rows, vocab, dim, ignored=0.2 if rows > 2 else 0.0)
+    features = features.detach().clone()
+    features[targets == -100] = math.nan
+    features.requires_grad_(True)
+    for reduction, logit_scale in (("mean", 1.0), ("none", -1.5), ("sum", 0.0)):
+        up = torch.rand(rows, generator=gen).to(device) if reduction == "none" else torch.tensor(0.5, device=device)
+        _compare(features, table, targets, up, reduction=reduction, logit_scale=logit_scale)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("rows,vocab,dim", [(5, 42, 640), (1, 2, 1), (38, 8192, 768), (700, 90, 128), (200, 2000, 300)])
+def test_entropy_of_few_rows_rounds_once(device, dtype, rows, vocab, dim):
+    """The gradients' distance from 64 bits is that of their own rounding and a tenth of it."""
+    print(f"entropy {dtype} rows={rows} vocab={vocab} dim={dim}", flush=True)
+    features, table, targets, gen = _problem(device, dtype, rows, vocab, dim, ignored=0.0)
+    want = ref.entropy(features.detach(), table.detach(), targets, 8.0, reduction="sum")
+    loss = vocabulary.linear_cross_entropy(features, table, targets, reduction="sum")
+    grads = torch.autograd.grad(loss, (features, table), torch.tensor(8.0, device=device))
+    for name, got in zip(("features", "table"), grads):
+        value = want[name][0]
+        own = (value.to(dtype).double() - value).norm()
+        assert float((got.double() - value).norm()) <= 1.1 * float(own) + 1e-6 * float(value.norm()), name
