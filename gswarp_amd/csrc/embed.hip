@@ -59,6 +59,17 @@ __device__ __forceinline__ Vec<T, V> load_vector(const T* __restrict__ p) {
   return x;
 }
 
+// The same, of what nothing else will read.
+template <bool kWhole, typename T, int V>
+__device__ __forceinline__ Vec<T, V> load_once(const T* __restrict__ p) {
+  if constexpr (kWhole && sizeof(T) * V == 16) {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(Vec<T, V>, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
+  } else {
+    return load_vector<kWhole, T, V>(p);
+  }
+}
+
 template <bool kWhole, typename T, int V>
 __device__ __forceinline__ void store_vector(T* __restrict__ p, const Vec<T, V>& x) {
   if (kWhole) *reinterpret_cast<Vec<T, V>*>(p) = x;
@@ -134,9 +145,12 @@ __device__ __forceinline__ void zero_rows(uint64_t absent, int64_t first, int D,
 }
 
 // One level of sums.  Reading grad_out row by row in the tokens' order bounds it:
-// 5M rows of 192 bytes take 300 us (3.2 TB/s, 4.3 of whole 128-byte lines), 65536
-// rows of 2 KB 54 us with the 32768 rows that they are summed to (3.7 TB/s).  Each
+// 5M rows of 192 bytes take 290 us (3.3 TB/s, 4.4 of whole 128-byte lines), 65536
+// rows of 2 KB 56 us with the 32768 rows that they are summed to (3.6 TB/s).  Each
 // lane has two batches of rows on their way, at addresses that are in LDS before.
+// Each row is read once, past the caches: what it would leave in them has to make
+// way for the next lookup's writes (a step of 5M x 48 fp32 takes 547 us, and 660
+// with cached reads; of 200000 x 64, which the caches hold, 81 and 79).
 // Entry e of n has key keys[e] (>= vocab: nothing) and its
 // row at src + (positions ? positions[e] : e) * ld.
 struct Level {
@@ -245,7 +259,7 @@ __global__ __launch_bounds__(kRunThreads, 4) void runs_kernel(Level v, const S* 
         const int e = e0 + j;
         if (e < e_end && in && keys[2 + e] < v.vocab) {
           const int64_t row = v.positions ? (int64_t)lds_positions[e] : begin + e;
-          to[j] = load_vector<kWhole, S, V>(src + row * v.ld + col);
+          to[j] = load_once<kWhole, S, V>(src + row * v.ld + col);
         }
       }
     };
