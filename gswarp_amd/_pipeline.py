@@ -101,8 +101,14 @@ def grid_dims(width: int, height: int) -> tuple[int, int]:
     return (width + BLOCK_X - 1) // BLOCK_X, (height + BLOCK_Y - 1) // BLOCK_Y
 
 
+# torch.cuda.current_stream(device).cuda_stream and torch.cuda.current_device() without the
+# objects and checks on the way, 2 and 0.5 us of a call (a lookup of a few rows takes 10 in all)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(_current_device() if device.index is None else device.index)
 
 
 def _f32c(t: torch.Tensor, align16: bool = False) -> torch.Tensor:
@@ -128,10 +134,13 @@ def _address_or_none(t: torch.Tensor | None, copies: list) -> int | None:
     return None if t is None else _address(t, copies)
 
 
+_NO_GUARD = contextlib.nullcontext()
+
+
 def _device_guard(device: torch.device):
     """torch.cuda.device(device), or nothing when it is the current device already."""
-    if device.index is None or torch.cuda.current_device() == device.index:
-        return contextlib.nullcontext()
+    if device.index is None or _current_device() == device.index:
+        return _NO_GUARD
     return torch.cuda.device(device)
 
 
