@@ -541,8 +541,8 @@ static int lanes_of(int D, int V) {
 }
 
 // Entries of a group.  On the first level 4 to 64, by how many make 512 chunks, two
-// a CU (1M x 16 bf16 into 256 rows, with the lookup: 153 us, and 190 at 1024 chunks;
-// 65536 x 1024 into 32768 rows: 126, 152 at 2048, 128 at 128); above, all of them
+// a CU (1M x 16 bf16 into 256 rows, with the lookup: 111 us, and 119 at 1024 chunks;
+// 65536 x 1024 into 32768 rows: 125, 131 at 1024, 126 at 256); above, all of them
 // where that is 8 at most, else 8 and on,
 // so that at most 64 chunks hand on to the next level: few levels, and none that
 // leaves many rows to one workgroup (2048 rows of 256 bytes take one 43 us).
