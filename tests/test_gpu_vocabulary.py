@@ -683,3 +683,22 @@ def test_entropy_of_few_rows_rounds_once(device, dtype, rows, vocab, dim):
         value = want[name][0]
         own = (value.to(dtype).double() - value).norm()
         assert float((got.double() - value).norm()) <= 1.1 * float(own) + 1e-6 * float(value.norm()), name
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [1, 2, 4, 7, 12, 33, 64, 130, 300])
+@pytest.mark.parametrize("lengths", [
+    [1, 2, 3, 4, 5, 7, 8, 9, 15, 16, 17] * 40, [63, 64, 65, 127, 128, 129, 255, 256, 257] * 4,
+    [511, 512, 513, 1, 1023, 1024, 1025, 1, 2047, 2048, 2049], [1, 30_000, 1], [4096] * 5])
+def test_lookup_gradient_runs_of_every_length(device, dtype, dim, lengths):
+    """Runs that begin and end at parts, waves and chunks, for rows of one lane to rows of many: of whole
+    numbers, so that every order of the sums gives the same."""
+    gen = _gen(dim + len(lengths))
+    vocab = 2 * len(lengths) + 1  # every other row is named by no token
+    tokens = torch.repeat_interleave(2 * torch.arange(len(lengths)) + 1, torch.tensor(lengths))
+    tokens = tokens[torch.randperm(tokens.numel(), generator=gen)]
+    up = torch.randint(-4, 5, (tokens.numel(), dim), generator=gen).float()
+    expected = torch.zeros(vocab, dim).index_add_(0, tokens, up).to(dtype)
+    table = torch.zeros(vocab, dim, dtype=dtype, device=device, requires_grad=True)
+    (grad,) = torch.autograd.grad(vocabulary.embed_tokens(tokens.to(device), table), table, up.to(device, dtype))
+    assert torch.equal(grad.cpu(), expected)
